@@ -23,15 +23,24 @@ E_NO_DEVICE = -3
 E_CAPTURE = -4
 
 OP_ADD, OP_SUB, OP_MUL, OP_DIV, OP_MAX, OP_MIN, OP_POW = range(7)
-DT_F32, DT_BF16, DT_F16 = range(3)
+DT_F32, DT_BF16, DT_F16, DT_E4M3 = range(4)
 (FN_SQUARE, FN_SQRT, FN_RSQRT, FN_LOG, FN_EXP, FN_ERF, FN_SIN, FN_COS, FN_ABS, FN_NEG, FN_RCP,
  FN_INVERSE, FN_SIGN) = range(13)
-ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_TANH, ACT_EXP = range(5)
+ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_TANH, ACT_EXP, ACT_GELU, ACT_SILU = range(7)
 
 _P = ctypes.c_void_p  # device pointer, stream or event handle
 _SZ = ctypes.c_size_t
 _I = ctypes.c_int
 _F = ctypes.c_float
+_D = ctypes.c_double
+_U64 = ctypes.c_uint64
+
+
+class AdamWTensor(ctypes.Structure):
+    """cxm_adamw_tensor_t."""
+    _fields_ = [("p", _P), ("g", _P), ("master", _P), ("m", _P), ("v", _P), ("m_scale", _P), ("v_scale", _P),
+                ("n", _SZ), ("decay", _F)]
+
 
 class PoolStats(ctypes.Structure):
     """cxm_pool_stats_t."""
@@ -118,6 +127,15 @@ SIGNATURES = {
     "cxm_softmax_xent_f32": [_P, _P, _P, _P, _SZ, _SZ, _P],
     "cxm_sgd_f32": [_P, _P, _F, _SZ, _P],
     "cxm_reduce_sum_bwd_f32": [_P, _P, _SZ, _SZ, _SZ, _I, _P],
+    "cxm_rmsnorm_fwd_t": [_P, _P, _P, _F, _P, _P, _P, _P, _P, _SZ, _SZ, _I, _P],
+    "cxm_rmsnorm_bwd_t": [_P, _P, _P, _P, _P, _P, _P, _SZ, _SZ, _I, _P],
+    "cxm_quant_rows_t": [_P, _P, _P, _SZ, _SZ, _I, _P],
+    "cxm_linear_fwd_t": [_P, _P, _P, _P, _P, _P, _SZ, _SZ, _SZ, _I, _I, _I, _P],
+    "cxm_linear_bwd_t": [_P, _P, _P, _P, _P, _P, _P, _P, _SZ, _SZ, _SZ, _I, _I, _I, _P],
+    "cxm_linear_q8_fwd": [_P, _P, _P, _P, _P, _P, _P, _P, _SZ, _SZ, _SZ, _I, _I, _P],
+    "cxm_adamw_create": [ctypes.POINTER(_P), ctypes.POINTER(AdamWTensor), _SZ, _I, _I, _I],
+    "cxm_adamw_step": [_P, _D, _D, _D, _D, _SZ, _P, _U64, _P],
+    "cxm_adamw_destroy": [_P],
     "cxm_mlp3_last_side": [_P, ctypes.POINTER(ctypes.c_uint)],
     "cxm_mlp3_create": [ctypes.POINTER(_P), _SZ, _SZ, _SZ, _SZ, _SZ],
     "cxm_mlp3_step_f32": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _F, _P, _P],

@@ -1,0 +1,397 @@
+// A dense layer: y = act(x W + bias) + residual in fp32, bf16, fp16 or from
+// e4m3 operands with scales, and its backward
+//   dz = dy act'(z),  db = column sums of dz,  dx = dz W^T,  dW = x^T dz.
+// The host side (plan, workspace, argument checks), the copies that bring
+// ragged operands into the ring's form, the backward's first kernel and the
+// fp32 epilogue.  The products are linear_ring.hip's and linear_skinny.hip's;
+// in fp32 they are cxm_gemm_f32's, and the activation and the residual a
+// pass over the result.
+#include "linear.hpp"
+#include "linear_act.hpp"
+
+namespace cxm {
+namespace {
+
+inline hipStream_t hs(cxm_stream_t s) { return reinterpret_cast<hipStream_t>(s); }
+inline size_t up(size_t v, size_t m) { return (v + m - 1) / m * m; }
+
+// ------------------------------------------------ operands for the ring
+//
+// The ring's direct-to-LDS loads take 16-byte aligned pieces and whole stages
+// of 64 bytes of k.  An operand that has other row lengths (or another base)
+// is copied once, its rows extended by zeros; one read and one write of it,
+// against the product's many.
+typedef unsigned u32x4b1 __attribute__((ext_vector_type(4), aligned(1)));
+
+__global__ __launch_bounds__(kBlock) void k_pad_rows(const uint8_t *__restrict__ X, uint8_t *__restrict__ Y, size_t rows,
+                                                    size_t bytes, size_t out_rows, unsigned pieces) {
+    const size_t i = static_cast<size_t>(blockIdx.x) * kBlock + threadIdx.x;
+    const size_t r = i / pieces, b = (i - r * pieces) * 16;
+    if (r >= out_rows) return;
+    unsigned v[4] = {0u, 0u, 0u, 0u};
+    if (r < rows && b < bytes) {
+        const uint8_t *p = X + r * bytes + b;
+        if (b + 16 <= bytes) {
+            const u32x4b1 t = *reinterpret_cast<const u32x4b1 *>(p);
+            v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+                if (b + k < bytes) v[k / 4] |= static_cast<unsigned>(p[k]) << (8 * (k & 3));
+        }
+    }
+    *reinterpret_cast<u32x4 *>(Y + i * 16) = u32x4{v[0], v[1], v[2], v[3]};
+}
+
+int pad_rows(const void *x, void *y, size_t rows, size_t bytes, size_t out_rows, size_t out_bytes, hipStream_t s) {
+    const size_t pieces = out_bytes / 16, wgs = (out_rows * pieces + kBlock - 1) / kBlock;
+    if (wgs > 0x7fffffffu || pieces > 0x7fffffffu) return CXM_E_TOO_LARGE;
+    hipLaunchKernelGGL(k_pad_rows, dim3(static_cast<unsigned>(wgs)), dim3(kBlock), 0, s, static_cast<const uint8_t *>(x),
+                       static_cast<uint8_t *>(y), rows, bytes, out_rows, static_cast<unsigned>(pieces));
+    return launch_status();
+}
+
+// ------------------------------------------------------------ fp32 layer
+
+// y = act(z) + res over z = x W + bias, which gemm_ex left in `from`.
+__global__ __launch_bounds__(kBlock) void k_linear_f32(const float *from, const float *res, float *y, size_t n, int act) {
+    const size_t i = (static_cast<size_t>(blockIdx.x) * kBlock + threadIdx.x) * 4;
+    if (i >= n) return;
+    const int own = n - i < 4 ? static_cast<int>(n - i) : 4;
+    float v[4] = {0.f, 0.f, 0.f, 0.f}, r[4] = {0.f, 0.f, 0.f, 0.f};
+    if (own == 4) {
+        Chunk<CXM_DT_F32, 4> c;
+        c.load(from + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = c.get(e);
+        if (res) {
+            c.load(res + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r[e] = c.get(e);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < own) {
+                v[e] = from[i + e];
+                r[e] = res ? res[i + e] : 0.0f;
+            }
+    }
+    act_apply<true, 4>(act, v);
+    if (res) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += r[e];
+    }
+    if (own == 4) {
+        Chunk<CXM_DT_F32, 4> c;
+        c.set(v);
+        c.store(y + i);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < own) y[i + e] = v[e];
+    }
+}
+
+int linear_f32(const float *x, const float *w, const float *bias, const float *res, float *z, float *y, size_t m,
+               size_t k, size_t n, int tw, int act, cxm_stream_t st) {
+    // without z, y holds x W + bias for a moment (so a residual in y itself is refused)
+    const bool fused = !z && !res && (act == CXM_ACT_NONE || act == CXM_ACT_RELU);
+    float *to = z ? z : y;
+    const Epilogue e{bias, nullptr, fused ? act : CXM_ACT_NONE, 0, 0.0f};
+    const int rc = gemm_ex(x, w, to, m, k, n, 0, tw, e, st);
+    if (rc || fused || (to == y && !res && act == CXM_ACT_NONE)) return rc;
+    const size_t wgs = (m * n + 4 * kBlock - 1) / (4 * kBlock);
+    if (wgs > 0x7fffffffu) return CXM_E_TOO_LARGE;
+    hipLaunchKernelGGL(k_linear_f32, dim3(static_cast<unsigned>(wgs)), dim3(kBlock), 0, hs(st), to, res, y, m * n, act);
+    return launch_status();
+}
+
+// ------------------------------------------------------- backward, first
+//
+// dz = dy act'(z) and the column sums of dz (unrounded, fp32): each of a
+// workgroup's waves takes rows of one tile of 64 chunks; the waves meet in
+// LDS, the workgroups' shares in k_col_sum, both in a fixed order.
+struct ActBwd {
+    const void *z, *dy;
+    void *dz;
+    float *part;  // null: no sums wanted
+    size_t rows;
+    unsigned cols, ld;
+    int act;
+};
+
+template <int DT, int VE>
+__global__ __launch_bounds__(kBlock) void k_act_bwd(ActBwd a) {
+    using S = typename Elem<DT>::S;
+    constexpr bool FINE = DT == CXM_DT_F32;
+    constexpr int W = kBlock / kWave;
+    __shared__ float lds[W][kWave * VE];
+    const unsigned lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
+    const unsigned c = blockIdx.x * kWave + lane;
+    const Span s = span_of<VE>(c, a.cols);
+    float acc[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) acc[e] = 0.0f;
+    for (size_t r = static_cast<size_t>(blockIdx.y) * W + w; r < a.rows; r += static_cast<size_t>(gridDim.y) * W) {
+        const size_t o = r * a.cols;
+        Chunk<DT, VE> cz, cd;
+        cd.load(static_cast<const S *>(a.dy) + o + s.off);
+        float z[VE], d[VE];
+        if (a.act != CXM_ACT_NONE) {
+            cz.load(static_cast<const S *>(a.z) + o + s.off);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) z[e] = cz.get(e);
+        }
+        act_slope<FINE, VE>(a.act, z, d);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+            d[e] *= cd.get(e);
+            acc[e] += d[e];
+        }
+        if (a.dz) {
+            cd.set(d);
+            store_span<DT, VE>(static_cast<S *>(a.dz) + o, s, cd);
+        }
+    }
+    if (!a.part) return;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) lds[w][e * kWave + lane] = acc[e];
+    __syncthreads();
+    if (w == 0) {
+        float *part = a.part + static_cast<size_t>(blockIdx.y) * a.ld;
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+            if (e >= static_cast<int>(s.dup))
+                part[s.off + e] = combine_pairwise<SumOp, W>(&lds[0][e * kWave + lane], kWave * VE);
+    }
+}
+
+// Row shares of the column sums.
+size_t act_bwd_parts(size_t rows, size_t cols, int dtype) {
+    const size_t ve = cols < (dtype == CXM_DT_F32 ? 4u : 8u) ? 1 : dtype == CXM_DT_F32 ? 4 : 8;
+    const size_t tiles = (cols + kWave * ve - 1) / (kWave * ve), need = (rows + kBlock / kWave - 1) / (kBlock / kWave);
+    size_t n = 4 * device_cus() / tiles;
+    n = n < 1 ? 1 : n;
+    n = n < need ? n : need;
+    return n < 65535 ? n : 65535;
+}
+
+template <int DT, int VE>
+int act_bwd_launch(const ActBwd &a, size_t parts, void *db, hipStream_t s) {
+    const size_t tiles = (a.cols + kWave * VE - 1) / (kWave * VE);
+    hipLaunchKernelGGL((k_act_bwd<DT, VE>), dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(parts)), dim3(kBlock),
+                       0, s, a);
+    const int r = launch_status();
+    if (r || !db) return r;
+    return col_sum(a.part, parts, a.cols, a.ld, db, DT, s);
+}
+template <int DT>
+int act_bwd(const ActBwd &a, size_t parts, void *db, hipStream_t s) {
+    if (a.cols < static_cast<unsigned>(Elem<DT>::kVec)) return act_bwd_launch<DT, 1>(a, parts, db, s);
+    return act_bwd_launch<DT, Elem<DT>::kVec>(a, parts, db, s);
+}
+
+bool act_ok(int act) { return act == CXM_ACT_NONE || act == CXM_ACT_RELU || act == CXM_ACT_SIGMOID || act == CXM_ACT_TANH ||
+                              act == CXM_ACT_GELU || act == CXM_ACT_SILU; }
+
+// Sizes whose element and byte counts stay far within 64 bits, and whose rows
+// the kernels number in 32.
+bool dims_ok(size_t m, size_t k, size_t n) {
+    constexpr size_t kRow = size_t(1) << 23;
+    return m < (size_t(1) << 31) && k < kRow && n < kRow;
+}
+
+int run_one(const LinProduct &p, cxm_stream_t st) {
+    LinPlan l;
+    int rc = linear_plan(p, &l);
+    if (rc) return rc;
+    Workspace ws{};
+    if (l.bytes() || l.counters()) {
+        rc = get_workspace(st, l.counters(), l.bytes(), &ws);
+        if (rc) return rc;
+    }
+    return linear_run(p, l, static_cast<char *>(ws.scratch), ws.counters, hs(st));
+}
+
+}  // namespace
+
+// The ring's tile and K splits.
+int linear_plan(const LinProduct &p, LinPlan *l) {
+    if (linear_skinny_plan(p, l) == CXM_OK) return CXM_OK;
+    *l = LinPlan{};
+    const size_t unit = 2, es = dtype_bytes(p.dtype), kb = p.K * es;
+    // rows of k: whole stages of 64 bytes; rows across k: whole chunks of 16 bytes, and whole stages of rows
+    const size_t kpad = up(kb, 64) / unit;  // units along K
+    l->stages = kpad / 32;
+    l->copy_a = !aligned16(p.a) || (p.ta ? p.M % 8 != 0 || p.K % 32 != 0 : kb % 64 != 0);
+    l->copy_b = !aligned16(p.b) || (p.tb ? kb % 64 != 0 : p.N % 8 != 0 || p.K % 32 != 0);
+    l->lda = p.ta ? up(p.M, 8) : kpad;
+    l->ldb = p.tb ? kpad : up(p.N, 8);
+    if (l->lda >= (size_t(1) << 23) || l->ldb >= (size_t(1) << 23)) return CXM_E_TOO_LARGE;
+    if (l->copy_a) l->bytes_a = up((p.ta ? kpad : p.M) * l->lda * unit, 256);
+    if (l->copy_b) l->bytes_b = up((p.tb ? p.N : kpad) * l->ldb * unit, 256);
+    const size_t cus = device_cus();
+    auto tiles = [&](size_t t) { return ((p.M + t - 1) / t) * ((p.N + t - 1) / t); };
+    l->kernel = tiles(256) >= cus * 3 / 4 ? 256 : tiles(128) >= cus * 5 / 8 ? 128 : 64;
+    const size_t t = static_cast<size_t>(l->kernel);
+    l->tiles_m = (p.M + t - 1) / t;
+    l->tiles_n = (p.N + t - 1) / t;
+    l->tiles = l->tiles_m * l->tiles_n;
+    l->splits = 1;
+    if (l->kernel == 64 && l->tiles < 2 * cus) {
+        l->splits = 2 * cus / l->tiles;
+        const size_t most = l->stages / 8;
+        if (l->splits > most) l->splits = most;
+        if (l->splits < 1) l->splits = 1;
+    }
+    l->per = (l->stages + l->splits - 1) / l->splits;
+    l->splits = (l->stages + l->per - 1) / l->per;
+    if (l->splits > 1) l->bytes_part = up(l->tiles * l->splits * t * t * sizeof(float), 256);
+    return CXM_OK;
+}
+
+int linear_run(const LinProduct &p, const LinPlan &l, char *scratch, unsigned *counters, hipStream_t s) {
+    if (l.kernel == 0)
+        return linear_skinny_run(p, l, l.bytes_part ? reinterpret_cast<float *>(scratch) : nullptr,
+                                 l.splits > 1 ? counters : nullptr, s);
+    const size_t es = dtype_bytes(p.dtype);
+    const void *a = p.a, *b = p.b;
+    const size_t krows = l.stages * 32;
+    if (l.copy_a) {
+        const int r = p.ta ? pad_rows(p.a, scratch, p.K, p.M * es, krows, l.lda * 2, s)
+                           : pad_rows(p.a, scratch, p.M, p.K * es, p.M, l.lda * 2, s);
+        if (r) return r;
+        a = scratch;
+    }
+    if (l.copy_b) {
+        char *to = scratch + l.bytes_a;
+        const int r = p.tb ? pad_rows(p.b, to, p.N, p.K * es, p.N, l.ldb * 2, s)
+                           : pad_rows(p.b, to, p.K, p.N * es, krows, l.ldb * 2, s);
+        if (r) return r;
+        b = to;
+    }
+    return linear_ring_run(p, l, a, b, reinterpret_cast<float *>(scratch + l.bytes_a + l.bytes_b), counters, s);
+}
+
+}  // namespace cxm
+
+extern "C" {
+
+int cxm_linear_fwd_t(const void *x, const void *w, const void *bias, const void *res, void *z, void *y, size_t m,
+                     size_t k, size_t n, int trans_w, int act, int dtype, cxm_stream_t s) {
+    using namespace cxm;
+    if (!is_float_dtype(dtype) || !act_ok(act)) return CXM_E_INVALID;
+    if (m == 0 || n == 0) return CXM_OK;
+    if (!x || !w || !y || k == 0) return CXM_E_INVALID;
+    if (!dims_ok(m, k, n)) return CXM_E_TOO_LARGE;
+    const size_t e = dtype_bytes(dtype), out = m * n * e;
+    const bool in_place = dtype != CXM_DT_F32 || z;  // y may be res itself
+    if ((in_place ? overlap_not_same(y, out, res, out) : overlap(y, out, res, out)) || overlap(z, out, res, out) ||
+        overlap(y, out, z, out))
+        return CXM_E_INVALID;
+    for (const void *o : {static_cast<const void *>(y), static_cast<const void *>(z)})
+        if (overlap(o, out, x, m * k * e) || overlap(o, out, w, k * n * e) || overlap(o, out, bias, n * e)) return CXM_E_INVALID;
+    if (dtype == CXM_DT_F32)
+        return linear_f32(static_cast<const float *>(x), static_cast<const float *>(w), static_cast<const float *>(bias),
+                          static_cast<const float *>(res), static_cast<float *>(z), static_cast<float *>(y), m, k, n,
+                          trans_w != 0, act, s);
+    const LinProduct p{x, w, m, k, n, false, trans_w != 0, dtype, dtype, {bias, res, z, y, nullptr, nullptr, act}};
+    return run_one(p, s);
+}
+
+int cxm_linear_q8_fwd(const uint8_t *x, const float *x_scale, const uint8_t *w, const float *w_scale, const void *bias,
+                      const void *res, void *z, void *y, size_t m, size_t k, size_t n, int act, int dtype,
+                      cxm_stream_t s) {
+    using namespace cxm;
+    if ((dtype != CXM_DT_BF16 && dtype != CXM_DT_F16) || !act_ok(act)) return CXM_E_INVALID;
+    if (m == 0 || n == 0) return CXM_OK;
+    if (!x || !w || !x_scale || !w_scale || !y || k == 0) return CXM_E_INVALID;
+    if (!dims_ok(m, k, n)) return CXM_E_TOO_LARGE;
+    const size_t out = m * n * 2;
+    if (overlap_not_same(y, out, res, out) || overlap(z, out, res, out) || overlap(y, out, z, out)) return CXM_E_INVALID;
+    for (const void *o : {static_cast<const void *>(y), static_cast<const void *>(z)})
+        if (overlap(o, out, x, m * k) || overlap(o, out, w, k * n) || overlap(o, out, bias, n * 2) ||
+            overlap(o, out, x_scale, m * 4) || overlap(o, out, w_scale, n * 4))
+            return CXM_E_INVALID;
+    const LinProduct p{x, w, m, k, n, false, true, CXM_DT_E4M3, dtype, {bias, res, z, y, x_scale, w_scale, act}};
+    return run_one(p, s);
+}
+
+int cxm_linear_bwd_t(const void *x, const void *w, const void *z, const void *dy, void *dz, void *dx, void *dw, void *db,
+                     size_t m, size_t k, size_t n, int trans_w, int act, int dtype, cxm_stream_t s) {
+    using namespace cxm;
+    if (!is_float_dtype(dtype) || !act_ok(act)) return CXM_E_INVALID;
+    if (m == 0 || n == 0 || k == 0) return CXM_E_INVALID;
+    if (!dims_ok(m, k, n) || m >= (size_t(1) << 23)) return CXM_E_TOO_LARGE;
+    const bool none = act == CXM_ACT_NONE;
+    if (!dy || (!none && (!z || !dz)) || (dx && !w) || (dw && !x)) return CXM_E_INVALID;
+    const size_t e = dtype_bytes(dtype), mn = m * n * e, mk = m * k * e, kn = k * n * e;
+    // dz may be z or dy itself; no other output meets an input or another output
+    if (overlap_not_same(dz, mn, z, mn) || overlap_not_same(dz, mn, dy, mn)) return CXM_E_INVALID;
+    const struct {
+        const void *p;
+        size_t n;
+    } out[4] = {{dz, mn}, {dx, mk}, {dw, kn}, {db, n * e}}, in[4] = {{x, mk}, {w, kn}, {z, mn}, {dy, mn}};
+    for (int i = 0; i < 4; ++i) {
+        for (int j = 0; j < 4; ++j)
+            if (!(i == 0 && j >= 2) && overlap(out[i].p, out[i].n, in[j].p, in[j].n)) return CXM_E_INVALID;
+        for (int j = 0; j < i; ++j)
+            if (overlap(out[i].p, out[i].n, out[j].p, out[j].n)) return CXM_E_INVALID;
+    }
+    const bool f32 = dtype == CXM_DT_F32;
+    const bool first = db || dz;  // dz to write or sums to make
+    const void *g = dz ? dz : dy;
+    const LinEpi plain{nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, CXM_ACT_NONE};
+    // dx [m, k] = dz W^T; dW [k, n] = x^T dz, or stored [n, k]: dz^T x
+    LinProduct px{g, w, m, n, k, false, trans_w == 0, dtype, dtype, plain};
+    LinProduct pw = trans_w ? LinProduct{g, x, n, m, k, true, false, dtype, dtype, plain}
+                            : LinProduct{x, g, k, m, n, true, false, dtype, dtype, plain};
+    px.e.y = dx;
+    pw.e.y = dw;
+    LinPlan lx{}, lw{};
+    size_t bytes = 0, counters = 0;
+    const size_t parts = act_bwd_parts(m, n, dtype), ld = (n + 3) / 4 * 4;
+    if (db) bytes = parts * ld * sizeof(float);
+    if (!f32) {
+        for (int i = 0; i < 2; ++i) {
+            if (!(i ? dw : dx)) continue;
+            LinPlan &l = i ? lw : lx;
+            const int rc = linear_plan(i ? pw : px, &l);
+            if (rc) return rc;
+            bytes = l.bytes() > bytes ? l.bytes() : bytes;
+            counters = l.counters() > counters ? l.counters() : counters;
+        }
+    }
+    Workspace ws{};
+    if (bytes || counters) {  // once, before the first launch
+        const int rc = get_workspace(s, counters, bytes, &ws);
+        if (rc) return rc;
+    }
+    if (first) {
+        const ActBwd a{z, dy, dz, db ? static_cast<float *>(ws.scratch) : nullptr, m, static_cast<unsigned>(n),
+                       static_cast<unsigned>(ld), act};
+        const int rc = f32 ? act_bwd<CXM_DT_F32>(a, parts, db, hs(s))
+                       : dtype == CXM_DT_BF16 ? act_bwd<CXM_DT_BF16>(a, parts, db, hs(s))
+                                              : act_bwd<CXM_DT_F16>(a, parts, db, hs(s));
+        if (rc) return rc;
+    }
+    if (f32) {
+        const auto *gf = static_cast<const float *>(g), *xf = static_cast<const float *>(x);
+        if (dx) {
+            const int rc = cxm_gemm_f32(gf, static_cast<const float *>(w), static_cast<float *>(dx), m, n, k, 0, !trans_w,
+                                        nullptr, CXM_ACT_NONE, nullptr, s);
+            if (rc) return rc;
+        }
+        if (!dw) return CXM_OK;
+        return trans_w ? cxm_gemm_f32(gf, xf, static_cast<float *>(dw), n, m, k, 1, 0, nullptr, CXM_ACT_NONE, nullptr, s)
+                       : cxm_gemm_f32(xf, gf, static_cast<float *>(dw), k, m, n, 1, 0, nullptr, CXM_ACT_NONE, nullptr, s);
+    }
+    if (dx) {
+        const int rc = linear_run(px, lx, static_cast<char *>(ws.scratch), ws.counters, hs(s));
+        if (rc) return rc;
+    }
+    return dw ? linear_run(pw, lw, static_cast<char *>(ws.scratch), ws.counters, hs(s)) : CXM_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,428 @@
+// Layer products on the matrix cores: bf16 / fp16 (v_mfma_f32_32x32x16) and
+// e4m3 (v_mfma_f32_32x32x64), fp32 accumulation, and the layer's epilogue
+// (scales, bias, activation, residual) before the only rounding.
+//
+// The ring of gemm16_ring.hpp with four additions:
+//  * any M and N: rows and columns past the end re-read the last ones, their
+//    sums are not stored;
+//  * either operand stored with k along its rows or across them (the
+//    transposing LDS reads serve both sides), so no product transposes first;
+//  * few tiles split K over workgroups; the last one to finish a tile adds
+//    the splits' partial sums in their order;
+//  * the epilogue goes through LDS, 32 rows at a time, so that a lane has 8
+//    consecutive elements of a row: 128-bit reads of the residual and writes
+//    of z and y, and the activation's code once per 8 elements.
+// An e4m3 product is the same ring over 16-bit units (two bytes of k): a stage
+// of 64 bytes per row is one 32x32x64 step, to which each lane gives the two
+// 16-byte pieces that the 16-bit form takes as two steps.  (Which k a lane
+// holds does not matter as long as both operands agree.)
+// The e4m3 steps align their products to the step's largest and drop what lies
+// below 2^-13 of it before the fp32 sum (measured: 2^16 - 2^16 + p keeps p =
+// 2^3 and loses 2^2; the 16-byte forms of the instruction do the same): 1e-5 of
+// the sum of magnitudes at K = 64 and 2e-6 at K = 1024, far below the
+// half step of the 16-bit result (4.9e-4 and 3.9e-3) and of the operands (6e-2).
+#include "gemm16_ring.hpp"
+#include "linear.hpp"
+#include "linear_act.hpp"
+
+namespace cxm {
+namespace {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+struct RingArgs {
+    const uint16_t *A, *B;
+    size_t lda, ldb;  // units
+    size_t M, N;
+    unsigned tiles_m, tiles_n, splits, stages, per, gm;
+    float *part;
+    unsigned *counters;
+    LinEpi e;
+};
+
+// Lane offsets of a stage's loads, rows (or chunks of 8 columns) clamped to
+// the operand's: `left` of them from the tile's first.
+template <int TM, bool KC>
+__device__ __forceinline__ RingOffs16<TM> lin_offs(size_t ld, size_t left) {
+    const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
+    RingOffs16<TM> f;
+    if constexpr (KC) {
+        const int rr = lane >> 2, p = lane & 3;
+#pragma unroll
+        for (int s = 0; s < Ring<TM>::ISSUES; ++s) {
+            const int row = w * (TM / 4) + s * 16 + rr;
+            const size_t r = static_cast<size_t>(row) < left ? row : left - 1;
+            f.o[s] = static_cast<unsigned>((r * ld + 8 * (p ^ rkey(row))) * sizeof(uint16_t));
+        }
+    } else {
+        constexpr int CPR = TM / 8, RPI = kWave / CPR;
+        const int rr = lane / CPR, p = lane % CPR;
+        const size_t last = (left + 7) / 8 - 1;  // rows are stored in whole chunks
+#pragma unroll
+        for (int s = 0; s < Ring<TM>::ISSUES; ++s) {
+            const int row = w * 8 + s * RPI + rr;
+            const size_t c = p ^ nkey<TM>(row);
+            f.o[s] = static_cast<unsigned>((row * ld + 8 * (c < last ? c : last)) * sizeof(uint16_t));
+        }
+    }
+    return f;
+}
+
+// Fragments of k block kb (16 units) of one operand's stage: rows w0 + 32 i +
+// l32, eight k at 16 kb + 8 lhi.
+template <int TM, bool KC>
+__device__ __forceinline__ void side_frags(const uint16_t *st, int kb, int w0, int l32, int lhi,
+                                           u32x4 (&f)[Ring<TM>::NB]) {
+    constexpr int NB = Ring<TM>::NB;
+    if constexpr (KC) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i) f[i] = *reinterpret_cast<const u32x4 *>(st + roff(w0 + i * 32 + l32, 2 * kb + lhi));
+    } else {
+        const int lane = threadIdx.x & (kWave - 1);
+        const int g = lane >> 4, jj = lane & 15;
+        const int r = 16 * kb + 8 * (g >> 1) + (jj >> 2);
+        const int c = 16 * (g & 1) + 4 * (jj & 3);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int n = w0 + i * 32 + c;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4 *)(st + noff<TM>(r, n)));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4 *)(st + noff<TM>(r + 4, n)));
+            const u32x2 ul = __builtin_bit_cast(u32x2, lo), uh = __builtin_bit_cast(u32x2, hi);
+            f[i] = u32x4{ul.x, ul.y, uh.x, uh.y};
+        }
+    }
+}
+
+template <int TM, bool KA, bool KB>
+struct RingLoads {
+    const uint16_t *A, *B;
+    size_t lda, ldb, m0, n0;
+    RingOffs16<TM> oa, ob;
+    __device__ __forceinline__ void issue(size_t k, uint16_t *stage) const {
+        ring_issue_at<TM, KA>(A, m0, k, lda, oa, stage);
+        ring_issue_at<TM, KB>(B, n0, k, ldb, ob, stage + Ring<TM>::TILE);
+    }
+};
+
+__device__ __forceinline__ f32x16 mfma8(u32x4 a0, u32x4 a1, u32x4 b0, u32x4 b1, f32x16 c) {
+    const i32x8 a = {static_cast<int>(a0.x), static_cast<int>(a0.y), static_cast<int>(a0.z), static_cast<int>(a0.w),
+                     static_cast<int>(a1.x), static_cast<int>(a1.y), static_cast<int>(a1.z), static_cast<int>(a1.w)};
+    const i32x8 b = {static_cast<int>(b0.x), static_cast<int>(b0.y), static_cast<int>(b0.z), static_cast<int>(b0.w),
+                     static_cast<int>(b1.x), static_cast<int>(b1.y), static_cast<int>(b1.z), static_cast<int>(b1.w)};
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
+}
+
+template <int TM>
+struct Frags {
+    u32x4 a[2][Ring<TM>::NB], b[2][Ring<TM>::NB];  // two k blocks of a stage
+};
+
+// Interleaves a k block's MFMAs with the fragment reads of the next.
+template <int NM, int ND>
+__device__ __forceinline__ void lin_interleave() {
+    constexpr int P = NM < ND ? NM : ND, PER = NM / P;
+#pragma unroll
+    for (int t = 0; t < P; ++t) {
+        __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, ND / P, 0);
+    }
+    if constexpr (NM > P * PER) __builtin_amdgcn_sched_group_barrier(0x008, NM - P * PER, 0);
+    if constexpr (ND > P * (ND / P)) __builtin_amdgcn_sched_group_barrier(0x100, ND - P * (ND / P), 0);
+}
+
+// 16-bit step on stage cur, as ring_step; f[0] holds block 0 of cur.
+template <int DT, int TM, bool KA, bool KB>
+__device__ __forceinline__ void lin_step16(const RingLoads<TM, KA, KB> &ld, size_t kf, uint16_t *cur,
+                                           const uint16_t *nxt, Frags<TM> &f, f32x16 (&acc)[Ring<TM>::NB][Ring<TM>::NB],
+                                           int am, int bn, int l32, int lhi) {
+    constexpr int NB = Ring<TM>::NB, TILE = Ring<TM>::TILE;
+    constexpr int NM = NB * NB, ND = NB * ((KA ? 1 : 2) + (KB ? 1 : 2));
+    side_frags<TM, KA>(cur, 1, am, l32, lhi, f.a[1]);
+    side_frags<TM, KB>(cur + TILE, 1, bn, l32, lhi, f.b[1]);
+    ring_mfma<DT, NB>(f.a[0], f.b[0], acc);
+    lin_interleave<NM, ND>();
+    ring_barrier<2 * Ring<TM>::PER_STAGE>();
+    side_frags<TM, KA>(nxt, 0, am, l32, lhi, f.a[0]);
+    side_frags<TM, KB>(nxt + TILE, 0, bn, l32, lhi, f.b[0]);
+    ld.issue(kf, cur);
+    ring_mfma<DT, NB>(f.a[1], f.b[1], acc);
+    lin_interleave<NM, ND>();
+    __builtin_amdgcn_sched_group_barrier(0x020, Ring<TM>::PER_STAGE, 0);
+}
+
+// e4m3 step: f holds all of cur's stage, g gets all of nxt's.
+template <int TM>
+__device__ __forceinline__ void lin_step8(const RingLoads<TM, true, true> &ld, size_t kf, uint16_t *cur,
+                                          const uint16_t *nxt, const Frags<TM> &f, Frags<TM> &g,
+                                          f32x16 (&acc)[Ring<TM>::NB][Ring<TM>::NB], int am, int bn, int l32, int lhi) {
+    constexpr int NB = Ring<TM>::NB, TILE = Ring<TM>::TILE;
+    ring_barrier<2 * Ring<TM>::PER_STAGE>();
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+        side_frags<TM, true>(nxt, kb, am, l32, lhi, g.a[kb]);
+        side_frags<TM, true>(nxt + TILE, kb, bn, l32, lhi, g.b[kb]);
+    }
+    ld.issue(kf, cur);
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[i][j] = mfma8(f.a[0][i], f.a[1][i], f.b[0][j], f.b[1][j], acc[i][j]);
+    lin_interleave<NB * NB, 4 * NB>();
+    __builtin_amdgcn_sched_group_barrier(0x020, Ring<TM>::PER_STAGE, 0);
+}
+
+// The tile's sums through the wave's LDS to rows of 8 elements per lane.
+template <int OT, int TM>
+__device__ __forceinline__ void lin_epilogue(const LinEpi &e, const f32x16 (&acc)[Ring<TM>::NB][Ring<TM>::NB],
+                                             float *lds, size_t m0, size_t n0, size_t M, size_t N, int l32, int lhi) {
+    constexpr int NB = Ring<TM>::NB, W = TM / 2, LP = W + 8;  // row stride: 4 rows on distinct halves of the banks
+    constexpr int LPR = W / 8, RPP = kWave / LPR;             // lanes per row, rows per pass
+    const int lane = threadIdx.x & (kWave - 1);
+    const int cl = 8 * (lane % LPR);
+    const size_t col = n0 + cl;
+    const int own = col >= N ? 0 : N - col < 8 ? static_cast<int>(N - col) : 8;  // elements of this lane's rows
+    const auto *res = static_cast<const uint16_t *>(e.res);
+    auto *z = static_cast<uint16_t *>(e.z);
+    auto *y = static_cast<uint16_t *>(e.y);
+    float bias[8], cs[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) bias[i] = 0.0f, cs[i] = 1.0f;
+    if (e.bias) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < own) bias[i] = H<OT>::load(static_cast<const uint16_t *>(e.bias)[col + i]);
+    }
+    if (e.cs) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < own) cs[i] = e.cs[col + i];
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) lds[(8 * (r / 4) + 4 * lhi + (r % 4)) * LP + 32 * j + l32] = acc[i][j][r];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int p = 0; p < 32 / RPP; ++p) {
+            const int rl = p * RPP + lane / LPR;
+            const size_t row = m0 + 32 * i + rl;
+            if (row >= M || own == 0) continue;
+            float v[8];
+            const float4 lo = *reinterpret_cast<const float4 *>(&lds[rl * LP + cl]);
+            const float4 hi = *reinterpret_cast<const float4 *>(&lds[rl * LP + cl + 4]);
+            v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
+            v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+            const size_t o = row * N + col;
+            Chunk<OT, 8> c;
+            if (e.res) {
+                if (own == 8) {
+                    c.load(res + o);
+                } else {
+                    uint16_t t[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (k < own) t[k] = res[o + k];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) c.r[k] = t[2 * k] | static_cast<unsigned>(t[2 * k + 1]) << 16;
+                }
+            }
+            const float rs = e.rs ? e.rs[row] : 1.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if (e.rs) v[k] = v[k] * rs * cs[k];
+                v[k] += bias[k];
+            }
+            auto put = [&](uint16_t *q) {
+                Chunk<OT, 8> d;
+                d.set(v);
+                if (own == 8) {
+                    d.store(q + o);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (k < own) q[o + k] = d.raw(k);
+                }
+            };
+            if (e.z) put(z);
+            act_apply<false, 8>(e.act, v);
+            if (e.res) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] += c.get(k);
+            }
+            put(y);
+        }
+    }
+}
+
+template <int DT, int OT, int TM, bool KA, bool KB>
+__global__ __launch_bounds__(kHThreads) void k_linear_ring(RingArgs a) {
+    constexpr int NB = Ring<TM>::NB, TILE = Ring<TM>::TILE, PS = Ring<TM>::PER_STAGE;
+    __shared__ __attribute__((aligned(16))) uint16_t s0[2 * TILE], s1[2 * TILE], s2[2 * TILE], s3[2 * TILE];
+    __shared__ int flag;
+    const unsigned wg = xcd_remap16(blockIdx.x, gridDim.x);
+    const unsigned tile = wg / a.splits, split = wg - tile * a.splits;
+    unsigned tm, tn;
+    group_tile(tile, a.tiles_m, a.tiles_n, a.gm, &tm, &tn);
+    const int wave = threadIdx.x / kWave;
+    const int am = (wave >> 1) * (TM / 2), bn = (wave & 1) * (TM / 2);
+    const int lane = threadIdx.x & (kWave - 1), l32 = lane & 31, lhi = lane >> 5;
+    const size_t first = static_cast<size_t>(split) * a.per;
+    const size_t T = a.stages - first < a.per ? a.stages - first : a.per;  // this split's stages, at least 1
+
+    f32x16 acc[NB][NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+    {
+        RingLoads<TM, KA, KB> ld;
+        ld.A = a.A;
+        ld.B = a.B;
+        ld.lda = a.lda;
+        ld.ldb = a.ldb;
+        ld.m0 = static_cast<size_t>(tm) * TM;
+        ld.n0 = static_cast<size_t>(tn) * TM;
+        ld.oa = lin_offs<TM, KA>(a.lda, a.M - ld.m0);
+        ld.ob = lin_offs<TM, KB>(a.ldb, a.N - ld.n0);
+        // stages past the last reload it into places whose fragments are not used
+        auto kt = [&](size_t t) { return (first + (t < T ? t : T - 1)) * kR_BK; };
+        ld.issue(kt(0), s0);
+        ld.issue(kt(1), s1);
+        ld.issue(kt(2), s2);
+        ld.issue(kt(3), s3);
+        ring_barrier<3 * PS>();
+        Frags<TM> f;
+        side_frags<TM, KA>(s0, 0, am, l32, lhi, f.a[0]);
+        side_frags<TM, KB>(s0 + TILE, 0, bn, l32, lhi, f.b[0]);
+        size_t t = 0;
+        if constexpr (DT == CXM_DT_E4M3) {
+            Frags<TM> g;
+            side_frags<TM, true>(s0, 1, am, l32, lhi, f.a[1]);
+            side_frags<TM, true>(s0 + TILE, 1, bn, l32, lhi, f.b[1]);
+            for (; t + 4 <= T; t += 4) {
+                lin_step8<TM>(ld, kt(t + 4), s0, s1, f, g, acc, am, bn, l32, lhi);
+                lin_step8<TM>(ld, kt(t + 5), s1, s2, g, f, acc, am, bn, l32, lhi);
+                lin_step8<TM>(ld, kt(t + 6), s2, s3, f, g, acc, am, bn, l32, lhi);
+                lin_step8<TM>(ld, kt(t + 7), s3, s0, g, f, acc, am, bn, l32, lhi);
+            }
+            if (t < T) lin_step8<TM>(ld, kt(t + 4), s0, s1, f, g, acc, am, bn, l32, lhi);
+            if (t + 1 < T) lin_step8<TM>(ld, kt(t + 5), s1, s2, g, f, acc, am, bn, l32, lhi);
+            if (t + 2 < T) lin_step8<TM>(ld, kt(t + 6), s2, s3, f, g, acc, am, bn, l32, lhi);
+        } else {
+            for (; t + 4 <= T; t += 4) {
+                lin_step16<DT, TM, KA, KB>(ld, kt(t + 4), s0, s1, f, acc, am, bn, l32, lhi);
+                lin_step16<DT, TM, KA, KB>(ld, kt(t + 5), s1, s2, f, acc, am, bn, l32, lhi);
+                lin_step16<DT, TM, KA, KB>(ld, kt(t + 6), s2, s3, f, acc, am, bn, l32, lhi);
+                lin_step16<DT, TM, KA, KB>(ld, kt(t + 7), s3, s0, f, acc, am, bn, l32, lhi);
+            }
+            if (t < T) lin_step16<DT, TM, KA, KB>(ld, kt(t + 4), s0, s1, f, acc, am, bn, l32, lhi);
+            if (t + 1 < T) lin_step16<DT, TM, KA, KB>(ld, kt(t + 5), s1, s2, f, acc, am, bn, l32, lhi);
+            if (t + 2 < T) lin_step16<DT, TM, KA, KB>(ld, kt(t + 6), s2, s3, f, acc, am, bn, l32, lhi);
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load into LDS is left
+
+    if (a.splits > 1) {
+        const unsigned ws = xcd_remap16(blockIdx.x, gridDim.x);
+        const unsigned ti = ws / a.splits, sp = ws - ti * a.splits;
+        float *base = a.part + static_cast<size_t>(ti) * a.splits * (TM * TM) + threadIdx.x;
+        float *my = base + static_cast<size_t>(sp) * (TM * TM);
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) st_dev(my + ((i * NB + j) * 16 + r) * kHThreads, acc[i][j][r]);
+        if (!last_block_ticket(ctr(a.counters, ti), a.splits, &flag)) return;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+        for (unsigned q = 0; q < a.splits; ++q) {
+            const float *p = base + static_cast<size_t>(q) * (TM * TM);
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int j = 0; j < NB; ++j)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[i][j][r] += ld_dev(p + ((i * NB + j) * 16 + r) * kHThreads);
+        }
+    }
+    __syncthreads();  // every wave's fragment reads are done: the stages become the epilogue's
+    // the tile origin again, from the workgroup index, so that it need not live across the K loop
+    group_tile(xcd_remap16(blockIdx.x, gridDim.x) / a.splits, a.tiles_m, a.tiles_n, a.gm, &tm, &tn);
+    uint16_t *mine = wave == 0 ? s0 : wave == 1 ? s1 : wave == 2 ? s2 : s3;
+    lin_epilogue<OT, TM>(a.e, acc, reinterpret_cast<float *>(mine), static_cast<size_t>(tm) * TM + am,
+                         static_cast<size_t>(tn) * TM + bn, a.M, a.N, l32, lhi);
+}
+
+template <int DT, int OT, int TM, bool KA, bool KB>
+void ring_launch(const RingArgs &a, unsigned wgs, hipStream_t s) {
+    hipLaunchKernelGGL((k_linear_ring<DT, OT, TM, KA, KB>), dim3(wgs), dim3(kHThreads), 0, s, a);
+}
+
+template <int DT, int OT, int TM>
+int ring_layout(const RingArgs &a, unsigned wgs, bool ta, bool tb, hipStream_t s) {
+    if constexpr (DT == CXM_DT_E4M3) {
+        ring_launch<DT, OT, TM, true, true>(a, wgs, s);
+    } else {
+        if (!ta && !tb) ring_launch<DT, OT, TM, true, false>(a, wgs, s);
+        else if (!ta) ring_launch<DT, OT, TM, true, true>(a, wgs, s);
+        else ring_launch<DT, OT, TM, false, false>(a, wgs, s);
+    }
+    return launch_status();
+}
+
+template <int DT, int OT>
+int ring_tile(const RingArgs &a, unsigned wgs, int tm, bool ta, bool tb, hipStream_t s) {
+    if (tm == 256) return ring_layout<DT, OT, 256>(a, wgs, ta, tb, s);
+    if (tm == 128) return ring_layout<DT, OT, 128>(a, wgs, ta, tb, s);
+    return ring_layout<DT, OT, 64>(a, wgs, ta, tb, s);
+}
+
+}  // namespace
+
+int linear_ring_run(const LinProduct &p, const LinPlan &l, const void *A, const void *B, float *part,
+                    unsigned *counters, hipStream_t s) {
+    const size_t wgs = l.tiles * l.splits;
+    // what the kernel assumes: 16-byte aligned rows, whole stages, lane offsets of a tile within 32 bits
+    if (!aligned16(A) || !aligned16(B) || l.lda % 8 != 0 || l.ldb % 8 != 0 || l.lda >= (size_t(1) << 23) ||
+        l.ldb >= (size_t(1) << 23) || l.stages == 0 || l.stages > 0x7fffffffu || l.per * (l.splits - 1) >= l.stages ||
+        l.per * l.splits < l.stages || wgs > 0x7fffffffu || (p.ta && p.tb))
+        return CXM_E_TOO_LARGE;
+    const RingArgs a{static_cast<const uint16_t *>(A),
+                     static_cast<const uint16_t *>(B),
+                     l.lda,
+                     l.ldb,
+                     p.M,
+                     p.N,
+                     static_cast<unsigned>(l.tiles_m),
+                     static_cast<unsigned>(l.tiles_n),
+                     static_cast<unsigned>(l.splits),
+                     static_cast<unsigned>(l.stages),
+                     static_cast<unsigned>(l.per),
+                     4,
+                     part,
+                     counters,
+                     p.e};
+    const unsigned n = static_cast<unsigned>(wgs);
+    if (p.dtype == CXM_DT_E4M3) {
+        if (p.out == CXM_DT_BF16) return ring_tile<CXM_DT_E4M3, CXM_DT_BF16>(a, n, l.kernel, false, true, s);
+        return ring_tile<CXM_DT_E4M3, CXM_DT_F16>(a, n, l.kernel, false, true, s);
+    }
+    if (p.dtype == CXM_DT_BF16) return ring_tile<CXM_DT_BF16, CXM_DT_BF16>(a, n, l.kernel, p.ta, p.tb, s);
+    return ring_tile<CXM_DT_F16, CXM_DT_F16>(a, n, l.kernel, p.ta, p.tb, s);
+}
+
+}  // namespace cxm

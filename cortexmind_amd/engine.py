@@ -14,12 +14,14 @@ import ctypes
 
 import numpy as np
 
-from ._lib import (ACT_EXP, ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_TANH, FN_ABS, FN_COS, FN_ERF,
+from ._lib import (ACT_EXP, ACT_GELU, ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_SILU, ACT_TANH, DT_E4M3, DT_F32, FN_ABS, FN_COS, FN_ERF,
                    FN_EXP, FN_INVERSE, FN_LOG, FN_NEG, FN_RCP, FN_RSQRT, FN_SIGN, FN_SIN, FN_SQRT,
-                   FN_SQUARE, OP_ADD, OP_DIV, OP_MAX, OP_MIN, OP_MUL, OP_POW, OP_SUB, call)
+                   FN_SQUARE, OP_ADD, OP_DIV, OP_MAX, OP_MIN, OP_MUL, OP_POW, OP_SUB,
+                   AdamWTensor, call)
 
 __all__ = ["reduce", "Broadcast", "matrix_t", "ScalarOp", "wise", "activation", "softmax", "gemm",
-           "train", "Mlp3", "ACT_NONE", "ACT_RELU", "ACT_SIGMOID", "ACT_TANH", "ACT_EXP"]
+           "rmsnorm", "quant", "linear", "train", "AdamW", "Mlp3", "ACT_NONE", "ACT_RELU", "ACT_SIGMOID", "ACT_TANH",
+           "ACT_EXP", "ACT_GELU", "ACT_SILU"]
 
 
 def _p(a):
@@ -316,6 +318,57 @@ def gemm(A, B, C, m, k, n, trans_a=False, trans_b=False, bias=None, act=ACT_NONE
          act, _p(gate), _s(stream))
 
 
+class rmsnorm:
+    """Root-mean-square norm of rows with the residual's addition, forward
+    (cxm_rmsnorm_fwd_t) and backward (cxm_rmsnorm_bwd_t), for a DT_* dtype."""
+
+    @staticmethod
+    def forward(X, W, Y, rows, cols, dtype, eps=1e-5, residual=None, H=None, Q=None, scale=None, rstd=None,
+                stream=None):
+        """H = X + residual, Y = norm(H) * W; Q and scale: Y's rows in 8 bits
+        (Y may then be None); rstd is what the backward reads."""
+        call("cxm_rmsnorm_fwd_t", _p(X), _p(residual), _p(W), float(eps), _p(H), _p(Y), _p(Q), _p(scale), _p(rstd),
+             rows, cols, dtype, _s(stream))
+
+    @staticmethod
+    def backward(H, rstd, W, dY, dX, dW, rows, cols, dtype, dH=None, stream=None):
+        """dX: the gradient of X and of the residual, dH (what reaches H past
+        the norm) included."""
+        call("cxm_rmsnorm_bwd_t", _p(H), _p(rstd), _p(W), _p(dY), _p(dH), _p(dX), _p(dW), rows, cols, dtype, _s(stream))
+
+
+class quant:
+    """Rows in 8 bits (e4m3) with a scale each."""
+
+    @staticmethod
+    def rows(X, Q, scale, rows, cols, dtype, stream=None):
+        call("cxm_quant_rows_t", _p(X), _p(Q), _p(scale), rows, cols, dtype, _s(stream))
+
+
+class linear:
+    """A dense layer, Y = act(X W + bias) + residual, for a DT_* dtype
+    (cxm_linear_fwd_t), from 8-bit operands (cxm_linear_q8_fwd), and its
+    backward (cxm_linear_bwd_t).  W is [k, n], or [n, k] with trans_w."""
+
+    @staticmethod
+    def forward(X, W, Y, m, k, n, dtype, bias=None, act=ACT_NONE, residual=None, Z=None, trans_w=False, stream=None):
+        """Z (X W + bias) is what the backward reads."""
+        call("cxm_linear_fwd_t", _p(X), _p(W), _p(bias), _p(residual), _p(Z), _p(Y), m, k, n, int(bool(trans_w)), act,
+             dtype, _s(stream))
+
+    @staticmethod
+    def forward_q8(X, x_scale, W, w_scale, Y, m, k, n, dtype, bias=None, act=ACT_NONE, residual=None, Z=None,
+                   stream=None):
+        """X [m, k] and W [n, k] in 8 bits with a scale per row."""
+        call("cxm_linear_q8_fwd", _p(X), _p(x_scale), _p(W), _p(w_scale), _p(bias), _p(residual), _p(Z), _p(Y), m, k, n,
+             act, dtype, _s(stream))
+
+    @staticmethod
+    def backward(X, W, Z, dY, dZ, dX, dW, db, m, k, n, dtype, act=ACT_NONE, trans_w=False, stream=None):
+        call("cxm_linear_bwd_t", _p(X), _p(W), _p(Z), _p(dY), _p(dZ), _p(dX), _p(dW), _p(db), m, k, n,
+             int(bool(trans_w)), act, dtype, _s(stream))
+
+
 class train:
     """Loss and optimizer pieces of the MLP step."""
 
@@ -327,6 +380,45 @@ class train:
     @staticmethod
     def sgd(W, G, lr, N, stream=None):
         call("cxm_sgd_f32", _p(W), _p(G), float(lr), N, _s(stream))
+
+
+class AdamW:
+    """The AdamW step over a list of tensors in one launch (cxm_adamw_*).
+
+    `tensors`: dicts of DeviceArrays p, g, m, v (and master; and m_scale,
+    v_scale with 8-bit moments), with the size n (default p.size) and the
+    weight decay (default 0).  The arrays are kept alive, and updated in place
+    by each step."""
+
+    def __init__(self, tensors, p_dtype=DT_F32, g_dtype=DT_F32, state_8bit=False):
+        self._h = ctypes.c_void_p(None)
+        self._kept = [dict(t) for t in tensors]
+        table = (AdamWTensor * len(self._kept))()
+        for rec, t in zip(table, self._kept):
+            for name in ("p", "g", "master", "m", "v", "m_scale", "v_scale"):
+                setattr(rec, name, _p(t.get(name)))
+            rec.n = t.get("n", t["p"].size)
+            rec.decay = float(t.get("decay", 0.0))
+        call("cxm_adamw_create", ctypes.byref(self._h), table, len(self._kept), p_dtype, g_dtype,
+             DT_E4M3 if state_8bit else DT_F32)
+
+    def step(self, lr, step, beta1=0.9, beta2=0.999, eps=1e-8, scalars=None, seed=0, stream=None):
+        """`step` counts from 1; `scalars`: a device array {lr, step, gradient
+        factor} read when the step runs; `seed`: of the 8-bit rounding, another
+        one for every step."""
+        call("cxm_adamw_step", self._h, float(lr), float(beta1), float(beta2), float(eps), int(step), _p(scalars),
+             int(seed), _s(stream))
+
+    def close(self):
+        if self._h.value:
+            call("cxm_adamw_destroy", self._h)
+            self._h = ctypes.c_void_p(None)
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 class Mlp3:

@@ -66,6 +66,9 @@ typedef struct ihipEvent_t *cxm_event_t;   /* a hipEvent_t */
 #define CXM_ACT_SIGMOID 2
 #define CXM_ACT_TANH 3
 #define CXM_ACT_EXP 4
+/* z Phi(z) and z / (1 + exp(-z)): the layer products (cxm_linear_*) only. */
+#define CXM_ACT_GELU 5
+#define CXM_ACT_SILU 6
 
 /* Elementwise math codes for cxm_wise_f32: nv::ElementWise
  * (Engine/CUDA/element_wise.cuh:11-27) and avx2::wise (Engine/AVX2/wise.hpp:28-42). */
@@ -88,6 +91,9 @@ typedef struct ihipEvent_t *cxm_event_t;   /* a hipEvent_t */
 #define CXM_DT_F32 0
 #define CXM_DT_BF16 1
 #define CXM_DT_F16 2
+/* 8-bit floats: 1 sign, 4 exponent and 3 mantissa bits, largest value 448, no
+ * infinities (OCP 8-bit floating point, E4M3).  Only where an entry names it. */
+#define CXM_DT_E4M3 3
 
 /* Human-readable text for a status code (never NULL). */
 const char *cxm_error_string(int status);
@@ -426,6 +432,112 @@ int cxm_reduce_sum_bwd_f32(const float *dz, float *dx, size_t outer, size_t dim,
                            cxm_stream_t s);
 /* w -= lr * g, as matrix_t::sub(w, ScalarOp::mul(g, lr)): two roundings. */
 int cxm_sgd_f32(float *w, const float *g, float lr, size_t n, cxm_stream_t s);
+
+/* ------------------------------------------------------------ RMS norm
+ * Root-mean-square norm of the rows of [rows, cols], CXM_DT_F32 / BF16 /
+ * F16, with the residual's addition before it.  No reference counterpart; it
+ * is the composition matrix_t::add, reduce::mean of squares per row,
+ * Broadcast::col::mul by rstd and Broadcast::row::mul by w:
+ *   h = x + res, rounded to the type (res NULL: h = x),
+ *   rstd = 1 / sqrt(mean(h*h) + eps), y = h * rstd * w.
+ * Each output may be NULL, but y or q is given: h [rows, cols] (needs res);
+ * y; q and scale, the rows of y in 8 bits (E4M3): scale[r] = max|y| / 448 and
+ * q = y / scale rounded to nearest even (a row whose scale is no normal
+ * float: scale 0 and zeros; a row with a NaN or an infinity has a NaN or
+ * infinite scale); rstd [rows], for the backward.  w has the rows' type; sums
+ * are fp32.  h and y may each be x or res itself; any other overlap of an
+ * output with an input or another output is CXM_E_INVALID.  rows == 0 does
+ * nothing; cols == 0 is CXM_E_INVALID. */
+int cxm_rmsnorm_fwd_t(const void *x, const void *res, const void *w, float eps, void *h, void *y, uint8_t *q,
+                      float *scale, float *rstd, size_t rows, size_t cols, int dtype, cxm_stream_t s);
+/* Backward from h and rstd of the forward: with n = h * rstd, g = dy * w,
+ * dx = rstd * (g - n * mean(g * n)) + dh, where dh (or NULL) is the gradient
+ * that reaches h past the norm; dx is the gradient of x and of res.
+ * dw[j] = sum over rows of dy * n, summed in fp32 in a fixed order.  dx may be
+ * h, dy or dh itself.  rows == 0 gives dw = 0.  Needs scratch (see
+ * CXM_E_CAPTURE). */
+int cxm_rmsnorm_bwd_t(const void *h, const float *rstd, const void *w, const void *dy, const void *dh, void *dx,
+                      void *dw, size_t rows, size_t cols, int dtype, cxm_stream_t s);
+/* The rows of x in 8 bits with a scale each, as above: for a weight [n, k]
+ * that cxm_linear_q8_fwd reads (once, when it is loaded) and for rows that
+ * reach it without a norm. */
+int cxm_quant_rows_t(const void *x, uint8_t *q, float *scale, size_t rows, size_t cols, int dtype, cxm_stream_t s);
+
+/* --------------------------------------------------------- dense layer
+ * z = x w + bias, y = act(z) + res over x [m, k], w [k, n] ([n, k] with
+ * trans_w), bias [n], res / z / y [m, n], all of `dtype` (CXM_DT_F32 / BF16 /
+ * F16); fp32 accumulation, the epilogue in fp32 before one rounding of each
+ * output.  act: NONE, RELU, SIGMOID, TANH, GELU (z times the normal
+ * distribution function), SILU.  bias, res and z may be NULL; z, what the
+ * backward reads, is rounded, y comes from the unrounded one.  y may be
+ * res itself (in fp32 only with z given); any other overlap of an output is
+ * CXM_E_INVALID.  k, n < 2^23, else CXM_E_TOO_LARGE.  m == 0 or n == 0 does
+ * nothing; k == 0 is CXM_E_INVALID.  Rows whose length is no multiple of 64
+ * bytes, and few tiles, need scratch (see CXM_E_CAPTURE).  Beside
+ * cxm_gemm_f32 and cxm_matmul_t; no reference counterpart. */
+int cxm_linear_fwd_t(const void *x, const void *w, const void *bias, const void *res, void *z, void *y, size_t m,
+                     size_t k, size_t n, int trans_w, int act, int dtype, cxm_stream_t s);
+/* Its backward from the saved z: dz = dy * act'(z) (rounded to the type,
+ * which the products read), db = column sums of the unrounded dz, dx = dz w^T,
+ * dw = x^T dz (stored as w).  The residual's gradient is dy.  dx, dw and db
+ * may be NULL; with act NONE also z, and dz (the products then read dy).  dz
+ * may be z or dy itself; no other overlap.  m, k, n > 0, m < 2^23. */
+int cxm_linear_bwd_t(const void *x, const void *w, const void *z, const void *dy, void *dz, void *dx, void *dw, void *db,
+                     size_t m, size_t k, size_t n, int trans_w, int act, int dtype, cxm_stream_t s);
+/* The same layer from 8-bit operands (E4M3): z[i, j] = x_scale[i] *
+ * w_scale[j] * sum over k of x[i, k] w[j, k], + bias; x [m, k] with a scale
+ * per row, w [n, k] with one per output (cxm_rmsnorm_fwd_t, cxm_quant_rows_t).
+ * bias, res, z, y of `dtype` CXM_DT_BF16 or F16.  Accumulation is fp32; the
+ * matrix cores drop what of a product lies below 2^-13 of the largest product
+ * of its 64 or 128 k. */
+int cxm_linear_q8_fwd(const uint8_t *x, const float *x_scale, const uint8_t *w, const float *w_scale, const void *bias,
+                      const void *res, void *z, void *y, size_t m, size_t k, size_t n, int act, int dtype,
+                      cxm_stream_t s);
+
+/* --------------------------------------------------------------- AdamW
+ * One step over all tensors of a model in one launch (beside cxm_sgd_f32):
+ *   g = factor * gradient, m = beta1 m + (1 - beta1) g,
+ *   v = beta2 v + (1 - beta2) g*g,
+ *   p = p (1 - lr decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps),
+ * in fp32.  A tensor with `master` keeps p there in fp32, and `p` gets its
+ * rounded copy (all tensors have one, or none; p_dtype BF16 or F16).
+ * state_dtype CXM_DT_F32: m and v are fp32, zero before the first step.
+ * state_dtype CXM_DT_E4M3: m and v hold m and sqrt(v) in 8 bits, value i
+ * times m_scale[i / 256] (v_scale[i / 256]); all zero before the first step.
+ * The scale is a block's largest finite magnitude / 448.  Rounding is to the
+ * neighbour above with the probability of the distance to the one below
+ * (towards the larger magnitude; a root above zero never becomes zero),
+ * decided by 16 of 32 random bits, the low ones for m: with c the value's
+ * number (i plus 256 times the blocks of the tensors before it) and key =
+ * low32(seed * 0x9E3779B1) ^ high32(seed),
+ *   x = low32(c) ^ key ^ low32(high32(c) * 0xC2B2AE35), twice
+ *   {x ^= x >> 16, x *= 0x85EBCA6B (then 0xC2B2AE35)}, x ^= x >> 16.
+ * Give every step another seed.  A NaN or an infinity is stored as NaN and
+ * leaves its block's other values as they are.
+ * The handle keeps the list (copied to the device by create, which blocks),
+ * not the tensors; they are on the device that was current then, where step
+ * has to be called too (else CXM_E_INVALID).  Nothing that a step writes may
+ * overlap anything else in the list (else CXM_E_INVALID); empty tensors are
+ * skipped. */
+typedef struct cxm_adamw_tensor_t {
+    void *p;         /* parameters (p_dtype) */
+    const void *g;   /* gradients (g_dtype: p_dtype or CXM_DT_F32) */
+    float *master;   /* fp32 parameters, or NULL */
+    void *m, *v;     /* moments, fp32 or 8 bits */
+    float *m_scale, *v_scale; /* [ceil(n / 256)], 8-bit moments only */
+    size_t n;
+    float decay;     /* weight decay of this tensor, >= 0 */
+} cxm_adamw_tensor_t;
+typedef struct cxm_adamw cxm_adamw;
+int cxm_adamw_create(cxm_adamw **handle, const cxm_adamw_tensor_t *tensors, size_t count, int p_dtype, int g_dtype,
+                     int state_dtype);
+/* `step` is t, from 1.  `scalars`: NULL, or three floats on the device, read
+ * when the step runs, that stand for lr, t and factor (1 without them): a
+ * captured step takes its arguments from there on every replay.  (Its seed
+ * stays the captured one.) */
+int cxm_adamw_step(cxm_adamw *handle, double lr, double beta1, double beta2, double eps, size_t step,
+                   const float *scalars, uint64_t seed, cxm_stream_t s);
+int cxm_adamw_destroy(cxm_adamw *handle);
 
 /* ------------------------------------------------------------- MLP step
  * One SGD training step of a 3-layer ReLU MLP, d0 -> d1 -> d2 -> d3, on a

@@ -1,0 +1,354 @@
+"""The dense layer (bias, activation, residual in the product's epilogue), its
+8-bit form and its backward, through the C ABI, against float64.
+
+Tolerances.  The product's fp32 accumulation is allowed 1e-5 of the sum of
+|x| |w| (the bar of the library's other products; a bias adds its magnitude),
+times the activation's largest slope (GELU 1.13, SILU 1.10, else 1): together
+1.2e-5.  The activation itself is 1e-5 relative (GELU's normal distribution
+is fitted to 7.5e-6; the exponentials' arguments are off by 2^-24 of up to
+90 / ln 2, 8e-6), for fp32 2e-6 where that argument is below 16.  Each
+output then has half a step of its type."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from cortexmind_amd._lib import (ACT_GELU, ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_SILU, ACT_TANH, DT_BF16, DT_F16, DT_F32,
+                                 call)
+from cortexmind_amd.data import SplitMix64
+from cortexmind_amd.device import DeviceArray, Stream
+from gpu_util import dev
+from layer_util import (DTYPES, E4M3, HALF, NAMES, TINY, close, from_bits, get, out, ptr, quant_rows, rounded, to_bits, up)
+
+pytestmark = pytest.mark.gpu
+ACTS = {"none": ACT_NONE, "relu": ACT_RELU, "sigmoid": ACT_SIGMOID, "tanh": ACT_TANH, "gelu": ACT_GELU, "silu": ACT_SILU}
+H16 = [DT_BF16, DT_F16]
+ids = lambda s: "x".join(map(str, s))  # noqa: E731
+
+
+def cdf(v):
+    """The normal distribution, digits kept in the negative tail."""
+    return 0.5 * torch.special.erfc(v * -math.sqrt(0.5))
+
+
+def act64(name, z):
+    t = torch.from_numpy(np.asarray(z, np.float64))
+    return {"none": lambda v: v, "relu": lambda v: v.clamp(min=0), "sigmoid": torch.sigmoid, "tanh": torch.tanh,
+            "gelu": lambda v: v * cdf(v), "silu": lambda v: v * torch.sigmoid(v)}[name](t).numpy()
+
+
+def slope64(name, z):
+    """act'(z), written so that no digits cancel."""
+    t = torch.from_numpy(np.asarray(z, np.float64))
+    sg = torch.sigmoid
+    return {"none": torch.ones_like, "relu": lambda v: (v > 0).double(), "sigmoid": lambda v: sg(v) * sg(-v),
+            "tanh": lambda v: 4 * sg(2 * v) * sg(-2 * v), "silu": lambda v: sg(v) * (1 + v * sg(-v)),
+            "gelu": lambda v: cdf(v) + v * torch.exp(-v * v / 2) / math.sqrt(2 * math.pi)}[name](t).numpy()
+
+
+def data(seed, shape, dt, std=1.0):
+    return rounded(SplitMix64(seed + sum(shape) + dt).normal(shape, 0.0, std), dt)
+
+
+def layer(m, k, n, dt, tw, bias, res, seed=1):
+    v = {"x": data(seed, (m, k), dt), "w": data(seed + 1, (k, n), dt, 1 / math.sqrt(k))}
+    v["bias"] = data(seed + 2, (n,), dt) if bias else None
+    v["res"] = data(seed + 3, (m, n), dt, 2.0) if res else None
+    return v
+
+
+def forward(v, dt, act, tw=False, save=False, off=0, in_place=False, stream=None):
+    (m, k), n = v["x"].shape, v["w"].shape[1]
+    d = {name: None if a is None else up(a.T if name == "w" and tw else a, dt, off) for name, a in v.items()}
+    y = d["res"] if in_place else out((m, n), dt, off)
+    z = out((m, n), dt, off) if save else None
+    call("cxm_linear_fwd_t", d["x"].ptr, d["w"].ptr, ptr(d["bias"]), ptr(d["res"]), ptr(z), y.ptr, m, k, n, int(tw),
+         ACTS[act], dt, stream)
+    call("cxm_stream_sync", stream)
+    return get(y, dt), (get(z, dt) if save else None)
+
+
+def check(v, dt, act, y, z, zsize=None, z64=None, lost=0.0):
+    if z64 is None:
+        z64 = v["x"] @ v["w"]
+        zsize = np.abs(v["x"]) @ np.abs(v["w"])
+    if v["bias"] is not None:
+        z64, zsize = z64 + v["bias"], zsize + np.abs(v["bias"])
+    a = act64(act, z64)
+    want = a if v["res"] is None else a + v["res"]
+    fit = 2e-6 if dt == DT_F32 else 1e-5
+    tol = HALF[dt] * np.abs(want) + 1.2e-5 * zsize + 1.13 * lost + fit * np.abs(a) + TINY[dt]
+    close(y, want, tol * (1 + 2.0 ** -8), "y")
+    if z is not None:
+        close(z, z64, (HALF[dt] * np.abs(z64) + 1e-5 * zsize + lost + TINY[dt]) * (1 + 2.0 ** -8), "z")
+
+
+# one row to many, each kernel's tiles whole and cut, K below a step, odd lengths
+SHAPES = [(1, 1, 1), (1, 7, 5), (3, 33, 9), (1, 4096, 512), (5, 100, 1000), (16, 1003, 131), (17, 256, 128),
+          (40, 520, 77), (64, 999, 300), (65, 64, 64), (100, 40, 200), (129, 1003, 259), (300, 2048, 190),
+          (70, 5, 70), (256, 160, 512), (1000, 96, 1100), (257, 4100, 70)]
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=NAMES.get)
+@pytest.mark.parametrize("tw", [False, True], ids=["w", "wT"])
+@pytest.mark.parametrize("shape", SHAPES, ids=ids)
+def test_forward_shapes(hip, shape, tw, dt):
+    for bias, res, act, save in ((False, False, "none", False), (True, True, "gelu", True)):
+        v = layer(*shape, dt, tw, bias, res)
+        check(v, dt, act, *forward(v, dt, act, tw, save))
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=NAMES.get)
+@pytest.mark.parametrize("act", list(ACTS))
+@pytest.mark.parametrize("shape", [(3, 64, 40), (200, 136, 104)], ids=ids)
+def test_forward_activations(hip, shape, act, dt):
+    """Every activation with and without bias, residual and saved z; y in res's place."""
+    for bias in (False, True):
+        for res in (False, True):
+            for save in (False, True):
+                v = layer(*shape, dt, False, bias, res, 40)
+                y, z = forward(v, dt, act, save=save)
+                check(v, dt, act, y, z)
+                if res and (save or dt != DT_F32):
+                    y2, z2 = forward(v, dt, act, save=save, in_place=True)
+                    assert np.array_equal(y, y2)
+
+
+# tiles of 256 and 128, whole and cut, K in whole ring turns and not; few tiles over a long K
+BIG = [(4096, 256, 4096), (3000, 352, 4100), (2048, 96, 1600), (2048, 1003, 1500), (512, 512, 512), (130, 8192, 300),
+       (1537, 64, 3001)]
+
+
+@pytest.mark.parametrize("dt", H16, ids=NAMES.get)
+@pytest.mark.parametrize("tw", [False, True], ids=["w", "wT"])
+@pytest.mark.parametrize("shape", BIG, ids=ids)
+def test_forward_large(hip, shape, tw, dt):
+    v = layer(*shape, dt, tw, True, True, 60)
+    check(v, dt, "silu", *forward(v, dt, "silu", tw, True))
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=NAMES.get)
+@pytest.mark.parametrize("shape", [(2, 64, 64), (40, 128, 200), (300, 128, 264)], ids=ids)
+def test_misaligned(hip, shape, dt):
+    for tw in (False, True):
+        v = layer(*shape, dt, tw, True, True, 80)
+        y, z = forward(v, dt, "tanh", tw, True, off=1)
+        check(v, dt, "tanh", y, z)
+
+
+@pytest.mark.parametrize("dt", H16, ids=NAMES.get)
+@pytest.mark.parametrize("act", ["gelu", "silu", "sigmoid", "tanh"])
+def test_activation_range(hip, act, dt):
+    """The activation over its whole range through a product by 1: relative to
+    the exact value, into the negative tail."""
+    zs = np.concatenate([np.linspace(-12, 12, 4001), [0.0, -0.0, 30.0, -30.0, 80.0, -80.0, 1e-3, -1e-3]])
+    x = rounded(zs, dt)[:, None]
+    v = {"x": x, "w": np.ones((1, 1)), "bias": None, "res": None}
+    y, _ = forward(v, dt, act)
+    want = act64(act, x)
+    # |z|^2 / 2 of up to 72 (gelu) or |z| of up to 80 in the exponent: 2^-24 of its binary logarithm each, three roundings
+    close(y, want, (HALF[dt] + 7.5e-6 + 3 * 2.0 ** -24 * 116) * np.abs(want) + TINY[dt] + 2.0 ** -126, act)
+
+
+def test_activation_range_f32(hip):
+    zs = rounded(np.linspace(-13, 13, 20001), DT_F32)[:, None]
+    for act in ("gelu", "silu", "sigmoid", "tanh"):
+        y, _ = forward({"x": zs, "w": np.ones((1, 1)), "bias": None, "res": None}, DT_F32, act)
+        want = act64(act, zs)
+        # fit 2.4e-7, then |z|^2 / 2 (1.44) <= 122 in the exponent: three roundings of it, and six more
+        close(y, want, (2.4e-7 + (3 * 122 * 0.7 + 6) * 2.0 ** -24) * np.abs(want) + 1e-30, act)
+
+
+def test_special_values(hip):
+    """A NaN or infinity of x stays in its row, one of w in its column; so at
+    every size (few rows, tiles, ragged)."""
+    for m, k, n in ((5, 100, 30), (70, 130, 90), (300, 256, 264)):
+        for tw in (False, True):
+            v = layer(m, k, n, DT_BF16, tw, False, False, 90)
+            v["w"] = np.abs(v["w"]) + 0.01
+            v["x"] = np.abs(v["x"]) + 0.01
+            v["w"] = rounded(v["w"], DT_BF16)
+            v["x"] = rounded(v["x"], DT_BF16)
+            v["x"][1, k - 1] = np.nan
+            v["x"][2, 0] = np.inf
+            v["w"][k - 1, n - 1] = np.inf
+            y, _ = forward(v, DT_BF16, "none", tw)
+            assert np.all(np.isnan(y[1])) and np.all(y[2] == np.inf)
+            rest = np.delete(y, [1, 2], axis=0)
+            assert np.all(rest[:, n - 1] == np.inf) and np.all(np.isfinite(rest[:, :n - 1]))
+
+
+def test_neighbours_untouched(hip):
+    for m, k, n in ((3, 64, 37), (70, 64, 61), (260, 128, 261)):
+        v = layer(m, k, n, DT_F16, False, True, False, 95)
+        d = {a: up(v[a], DT_F16) for a in ("x", "w", "bias")}
+        buf = DeviceArray.from_numpy(np.full(m * n + 64, 0x1234, np.uint16))
+        call("cxm_linear_fwd_t", d["x"].ptr, d["w"].ptr, d["bias"].ptr, None, None, buf.ptr + 64, m, k, n, 0, ACT_NONE,
+             DT_F16, None)
+        b = buf.numpy()
+        assert np.all(b[:32] == 0x1234) and np.all(b[-32:] == 0x1234)
+        check(v, DT_F16, "none", from_bits(b[32:-32].reshape(m, n), DT_F16), None)
+
+
+def test_runs_repeat_and_streams_agree(hip):
+    s = Stream()
+    for shape in ((1, 8192, 256), (130, 8192, 300), (1024, 512, 1024)):
+        v = layer(*shape, DT_BF16, True, True, False, 97)
+        want, _ = forward(v, DT_BF16, "gelu", True)
+        for stream in (None, s.handle, s.handle):
+            got, _ = forward(v, DT_BF16, "gelu", True, stream=stream)
+            assert np.array_equal(got, want)
+    s.close()
+
+
+def test_offsets_past_32_bits(hip):
+    """An output of more than 2^32 elements; its last rows are checked."""
+    m, k, n = 270000, 16, 16384
+    x = DeviceArray((m * k,), np.uint16)
+    x.fill_bytes(0)
+    v = layer(40, k, n, DT_BF16, False, True, False, 99)
+    bits = to_bits(v["x"], DT_BF16)
+    call("cxm_memcpy_h2d", x.ptr + 2 * (m - 40) * k, bits.ctypes.data, bits.nbytes, None)
+    w, b, y = up(v["w"], DT_BF16), up(v["bias"], DT_BF16), DeviceArray((m * n,), np.uint16)
+    call("cxm_linear_fwd_t", x.ptr, w.ptr, b.ptr, None, None, y.ptr, m, k, n, 0, ACT_NONE, DT_BF16, None)
+    got = np.empty((41, n), np.uint16)
+    call("cxm_memcpy_d2h", got.ctypes.data, y.ptr + 2 * (m - 41) * n, got.nbytes, None)
+    g = from_bits(got, DT_BF16)
+    check(v, DT_BF16, "none", g[1:], None)
+    assert np.array_equal(g[0], v["bias"])
+
+
+# ----------------------------------------------------------- 8-bit operands
+
+
+def forward_q8(m, k, n, dt, act, bias, res, seed=1, off=0, save=True):
+    g = SplitMix64(seed + m + k + n)
+    qx, sx = quant_rows(g.normal((m, k)).astype(np.float64))
+    qw, sw = quant_rows(g.normal((n, k), 0.0, 1 / math.sqrt(k)).astype(np.float64))
+    v = {"bias": data(seed, (n,), dt) if bias else None, "res": data(seed + 1, (m, n), dt) if res else None}
+    d = {"x": dev(qx, off), "sx": dev(sx), "w": dev(qw, off), "sw": dev(sw)}
+    db, dr = (None if a is None else up(a, dt) for a in (v["bias"], v["res"]))
+    y, z = out((m, n), dt), out((m, n), dt) if save else None
+    call("cxm_linear_q8_fwd", d["x"].ptr, d["sx"].ptr, d["w"].ptr, d["sw"].ptr, ptr(db), ptr(dr), ptr(z), y.ptr, m, k, n,
+         ACTS[act], dt, None)
+    scale = sx.astype(np.float64)[:, None] * sw.astype(np.float64)[None, :]
+    z64, size = (E4M3[qx] @ E4M3[qw].T) * scale, (np.abs(E4M3[qx]) @ np.abs(E4M3[qw]).T) * scale
+    # The matrix cores drop what of an 8-bit product lies below 2^-13 of the
+    # step's largest, P at most: k errors within 2^-13 P, uniform, so with a
+    # standard deviation of sqrt(k / 12) 2^-13 P; six of them (none at k = 1)
+    p = np.abs(E4M3[qx]).max(1)[:, None] * np.abs(E4M3[qw]).max(1)[None, :] * scale
+    lost = 6 * math.sqrt(k / 12) * 2.0 ** -13 * p if k > 1 else 0.0
+    check(v, dt, act, get(y, dt), get(z, dt) if save else None, size, z64, lost)
+
+
+@pytest.mark.parametrize("dt", H16, ids=NAMES.get)
+@pytest.mark.parametrize("shape", [(1, 1, 1), (3, 31, 9), (1, 4096, 512), (16, 1003, 131), (33, 200, 77), (64, 640, 48),
+                                   (65, 64, 64), (100, 65, 200), (300, 2050, 190), (2048, 320, 2100), (4096, 512, 4096),
+                                   (130, 8192, 300)], ids=ids)
+def test_q8_shapes(hip, shape, dt):
+    forward_q8(*shape, dt, "none", False, False)
+    forward_q8(*shape, dt, "gelu", True, True, 5, save=False)
+
+
+@pytest.mark.parametrize("off", [1, 3, 4])
+def test_q8_misaligned(hip, off):
+    for shape in ((2, 256, 64), (200, 256, 136)):
+        forward_q8(*shape, DT_BF16, "relu", True, False, 9, off)
+
+
+# ---------------------------------------------------------------- backward
+
+
+def backward(v, z, dy, dt, act, tw, off=0, want=("dx", "dw", "db"), dz_in=None, stream=None):
+    (m, k), n = v["x"].shape, v["w"].shape[1]
+    d = {"x": up(v["x"], dt, off), "w": up(v["w"].T if tw else v["w"], dt, off), "z": up(z, dt, off), "dy": up(dy, dt, off)}
+    o = {"dx": out((m, k), dt, off), "dw": out((n, k) if tw else (k, n), dt, off), "db": out(n, dt, off)}
+    dz = d[dz_in] if dz_in else out((m, n), dt, off)
+    call("cxm_linear_bwd_t", d["x"].ptr, d["w"].ptr, d["z"].ptr, d["dy"].ptr, dz.ptr,
+         *(o[name].ptr if name in want else None for name in ("dx", "dw", "db")), m, k, n, int(tw), ACTS[act], dt, stream)
+    got = {name: get(o[name], dt) for name in want}
+    got["dz"] = get(dz, dt)
+    if tw and "dw" in got:
+        got["dw"] = got["dw"].T
+    return got
+
+
+def check_backward(v, z, dy, dt, act, got):
+    dz = dy * slope64(act, z)
+    # the slope: 1e-5 of its parts (at most 1 + |z phi| and the like, below 1.3)
+    slope_tol = (2e-6 if dt == DT_F32 else 1e-5) * 1.3 * np.abs(dy)
+    tol = HALF[dt] * np.abs(dz) + slope_tol + TINY[dt]
+    close(got["dz"], dz, tol * (1 + 2.0 ** -8), "dz")
+    if "db" in got:
+        close(got["db"], dz.sum(0), HALF[dt] * np.abs(dz.sum(0)) + slope_tol.sum(0) + 128 * 2.0 ** -24 * np.abs(dz).sum(0)
+              + TINY[dt], "db")
+    g = got["dz"]  # what the products read
+    if "dx" in got:
+        want = g @ v["w"].T
+        close(got["dx"], want, HALF[dt] * np.abs(want) + 1e-5 * (np.abs(g) @ np.abs(v["w"].T)) + TINY[dt], "dx")
+    if "dw" in got:
+        want = v["x"].T @ g
+        close(got["dw"], want, HALF[dt] * np.abs(want) + 1e-5 * (np.abs(v["x"].T) @ np.abs(g)) + TINY[dt], "dw")
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=NAMES.get)
+@pytest.mark.parametrize("tw", [False, True], ids=["w", "wT"])
+@pytest.mark.parametrize("shape", [(1, 1, 1), (1, 64, 40), (7, 33, 5), (64, 100, 72), (65, 64, 64), (129, 67, 259),
+                                   (300, 520, 190), (1000, 96, 1100), (2500, 40, 30)], ids=ids)
+def test_backward(hip, shape, tw, dt):
+    m, k, n = shape
+    for act in ("gelu", "none"):
+        v = layer(m, k, n, dt, tw, False, False, 110)
+        z, dy = data(111, (m, n), dt), data(112, (m, n), dt)
+        check_backward(v, z, dy, dt, act, backward(v, z, dy, dt, act, tw))
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=NAMES.get)
+@pytest.mark.parametrize("act", list(ACTS))
+def test_backward_activations(hip, act, dt):
+    m, k, n = 90, 48, 136
+    v = layer(m, k, n, dt, False, False, False, 120)
+    z, dy = data(121, (m, n), dt, 3.0), data(122, (m, n), dt)
+    want = backward(v, z, dy, dt, act, False)
+    check_backward(v, z, dy, dt, act, want)
+    for kw in ({"dz_in": "z"}, {"dz_in": "dy"}, {"off": 1}):
+        got = backward(v, z, dy, dt, act, False, **kw)
+        assert np.array_equal(got["dz"], want["dz"]) and np.array_equal(got["db"], want["db"]), kw
+        check_backward(v, z, dy, dt, act, got)
+    for only in ("dx", "dw", "db"):
+        got = backward(v, z, dy, dt, act, False, want=(only,))
+        assert np.array_equal(got[only], want[only])
+
+
+def test_backward_slope_range(hip):
+    """act'(z) into both tails, in fp32."""
+    z = rounded(np.concatenate([np.linspace(-12, 12, 3001), [0.0, 50.0, -50.0]]), DT_F32)[:, None]
+    v = {"x": np.ones((z.size, 1)), "w": np.ones((1, 1))}
+    for act in ("sigmoid", "tanh", "gelu", "silu"):
+        got = backward(v, z, np.ones_like(z), DT_F32, act, False)["dz"]
+        want = slope64(act, z)
+        # the gelu and silu slopes cross zero, where two parts of size |z| phi cancel
+        part = np.abs(z) * np.exp(-z * z / 2) * 0.4 if act == "gelu" else np.abs(z) * want if act == "silu" else 0.0
+        tol = (2.4e-7 + 3 * 110 * 2.0 ** -24) * (np.abs(want) + np.abs(part) + act64("sigmoid", z) * (act == "silu"))
+        close(got, want, tol + 1e-30, act)
+
+
+def test_backward_against_differences(hip):
+    """fp32 gradients against central differences of the definition in float64."""
+    m, k, n = 5, 7, 6
+    v = layer(m, k, n, DT_F32, False, True, False, 130)
+    dy = data(131, (m, n), DT_F32)
+    for act in ("gelu", "silu", "tanh"):
+        _, z = forward(v, DT_F32, act, save=True)
+        got = backward(v, z, dy, DT_F32, act, False)
+
+        def f(x, w, b):
+            return float((act64(act, x @ w + b) * dy).sum())
+
+        step = 1e-5
+        for name, i in (("x", (1, 2)), ("w", (3, 4)), ("bias", (5,))):
+            e = {a: np.zeros_like(v[a]) for a in ("x", "w", "bias")}
+            e[name][i] = step
+            num = (f(*(v[a] + e[a] for a in e)) - f(*(v[a] - e[a] for a in e))) / (2 * step)
+            assert abs(num - got[{"x": "dx", "w": "dw", "bias": "db"}[name]][i]) <= 2e-5, (act, name)

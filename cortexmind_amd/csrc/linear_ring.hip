@@ -2,7 +2,11 @@
 // e4m3 (v_mfma_f32_32x32x64), fp32 accumulation, and the layer's epilogue
 // (scales, bias, activation, residual) before the only rounding.
 //
-// The ring of gemm16_ring.hpp with four additions:
+// The ring of gemm16_ring.hpp (stages of 64 bytes per row) with these changes:
+//  * eight waves, two per SIMD, on tiles of 256 and 128: one hides the
+//    other's barriers and the epilogue's latency (four waves of 128x128 ran
+//    4096x1024x4096 in 46.3 us against 37.5, 8192^3 at 1200 TFLOP/s against
+//    1320; 2500x1024x1504 on 128 tiles 15.1 against 13.3);
 //  * any M and N: rows and columns past the end re-read the last ones, their
 //    sums are not stored;
 //  * either operand stored with k along its rows or across them (the
@@ -40,69 +44,92 @@ struct RingArgs {
     LinEpi e;
 };
 
-// Lane offsets of a stage's loads, rows (or chunks of 8 columns) clamped to
-// the operand's: `left` of them from the tile's first.
-template <int TM, bool KC>
-__device__ __forceinline__ RingOffs16<TM> lin_offs(size_t ld, size_t left) {
-    const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
-    RingOffs16<TM> f;
-    if constexpr (KC) {
-        const int rr = lane >> 2, p = lane & 3;
+// A TM x TN tile by WM x WN waves: each wave's share of it and of the stages'
+// loads (one load instruction of a wave brings 1 KiB).
+template <int TM_, int TN_, int WM_, int WN_>
+struct Geo {
+    static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_;
+    static constexpr int WAVES = WM * WN, NT = WAVES * kWave;
+    static constexpr int HM = TM / WM, HN = TN / WN;         // a wave's rows and columns
+    static constexpr int MB = HM / 32, NB = HN / 32;         // its 32x32 blocks
+    static constexpr int IA = TM / (16 * WAVES), IB = TN / (16 * WAVES);
+    static constexpr int PS = IA + IB;                       // loads of a wave per stage
+    static constexpr int TA = TM * kR_BK, STAGE = (TM + TN) * kR_BK;  // 16-bit units
+    static_assert(IA >= 1 && IB >= 1 && MB >= 1 && NB >= 1, "every wave loads and multiplies");
+};
+
+// Byte offsets of this lane's loads of an operand's stage (T rows of 64 bytes
+// where k runs along the rows, else 32 k rows of T columns), rows (or chunks
+// of 8 columns) past the operand's last clamped to it: `left` of them count
+// from the tile's first.
+template <int T, int ISSUES, bool KC>
+struct SideLoads {
+    unsigned o[ISSUES];
+    __device__ __forceinline__ void init(size_t ld, size_t left) {
+        const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
+        if constexpr (KC) {
+            const int rr = lane >> 2, p = lane & 3;
 #pragma unroll
-        for (int s = 0; s < Ring<TM>::ISSUES; ++s) {
-            const int row = w * (TM / 4) + s * 16 + rr;
-            const size_t r = static_cast<size_t>(row) < left ? row : left - 1;
-            f.o[s] = static_cast<unsigned>((r * ld + 8 * (p ^ rkey(row))) * sizeof(uint16_t));
-        }
-    } else {
-        constexpr int CPR = TM / 8, RPI = kWave / CPR;
-        const int rr = lane / CPR, p = lane % CPR;
-        const size_t last = (left + 7) / 8 - 1;  // rows are stored in whole chunks
+            for (int s = 0; s < ISSUES; ++s) {
+                const int row = (w * ISSUES + s) * 16 + rr;
+                const size_t r = static_cast<size_t>(row) < left ? row : left - 1;
+                o[s] = static_cast<unsigned>((r * ld + 8 * (p ^ rkey(row))) * sizeof(uint16_t));
+            }
+        } else {
+            constexpr int CPR = T / 8, RPI = kWave / CPR;
+            const int rr = lane / CPR, p = lane % CPR;
+            const size_t last = (left + 7) / 8 - 1;  // rows are stored in whole chunks
 #pragma unroll
-        for (int s = 0; s < Ring<TM>::ISSUES; ++s) {
-            const int row = w * 8 + s * RPI + rr;
-            const size_t c = p ^ nkey<TM>(row);
-            f.o[s] = static_cast<unsigned>((row * ld + 8 * (c < last ? c : last)) * sizeof(uint16_t));
+            for (int s = 0; s < ISSUES; ++s) {
+                const int row = (w * ISSUES + s) * RPI + rr;
+                const size_t c = p ^ nkey<T>(row);
+                o[s] = static_cast<unsigned>((row * ld + 8 * (c < last ? c : last)) * sizeof(uint16_t));
+            }
         }
     }
-    return f;
-}
+    __device__ __forceinline__ void issue(const uint16_t *X, size_t r0, size_t k, size_t ld, uint16_t *stage) const {
+        const unsigned w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+        const uint16_t *base = KC ? X + r0 * ld + k : X + k * ld + r0;
+        const unsigned l0 = lds_addr(stage) + w * (ISSUES * kWave * 16);
+#pragma unroll
+        for (int s = 0; s < ISSUES; ++s) lds_load16_at(base, o[s], l0 + s * kWave * 16);
+    }
+};
 
-// Fragments of k block kb (16 units) of one operand's stage: rows w0 + 32 i +
-// l32, eight k at 16 kb + 8 lhi.
-template <int TM, bool KC>
-__device__ __forceinline__ void side_frags(const uint16_t *st, int kb, int w0, int l32, int lhi,
-                                           u32x4 (&f)[Ring<TM>::NB]) {
-    constexpr int NB = Ring<TM>::NB;
+// Fragments of k block kb (16 units) of one operand's stage of T rows (or
+// columns): rows w0 + 32 i + l32, eight k at 16 kb + 8 lhi.
+template <int T, bool KC, int N>
+__device__ __forceinline__ void side_frags(const uint16_t *st, int kb, int w0, int l32, int lhi, u32x4 (&f)[N]) {
     if constexpr (KC) {
 #pragma unroll
-        for (int i = 0; i < NB; ++i) f[i] = *reinterpret_cast<const u32x4 *>(st + roff(w0 + i * 32 + l32, 2 * kb + lhi));
+        for (int i = 0; i < N; ++i) f[i] = *reinterpret_cast<const u32x4 *>(st + roff(w0 + i * 32 + l32, 2 * kb + lhi));
     } else {
         const int lane = threadIdx.x & (kWave - 1);
         const int g = lane >> 4, jj = lane & 15;
         const int r = 16 * kb + 8 * (g >> 1) + (jj >> 2);
         const int c = 16 * (g & 1) + 4 * (jj & 3);
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
+        for (int i = 0; i < N; ++i) {
             const int n = w0 + i * 32 + c;
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4 *)(st + noff<TM>(r, n)));
+                (__attribute__((address_space(3))) s16x4 *)(st + noff<T>(r, n)));
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4 *)(st + noff<TM>(r + 4, n)));
+                (__attribute__((address_space(3))) s16x4 *)(st + noff<T>(r + 4, n)));
             const u32x2 ul = __builtin_bit_cast(u32x2, lo), uh = __builtin_bit_cast(u32x2, hi);
             f[i] = u32x4{ul.x, ul.y, uh.x, uh.y};
         }
     }
 }
 
-template <int TM, bool KA, bool KB>
+template <class G, bool KA, bool KB>
 struct RingLoads {
     const uint16_t *A, *B;
     size_t lda, ldb, m0, n0;
-    RingOffs16<TM> oa, ob;
+    SideLoads<G::TM, G::IA, KA> oa;
+    SideLoads<G::TN, G::IB, KB> ob;
     __device__ __forceinline__ void issue(size_t k, uint16_t *stage) const {
-        ring_issue_at<TM, KA>(A, m0, k, lda, oa, stage);
-        ring_issue_at<TM, KB>(B, n0, k, ldb, ob, stage + Ring<TM>::TILE);
+        oa.issue(A, m0, k, lda, stage);
+        ob.issue(B, n0, k, ldb, stage + G::TA);
     }
 };
 
@@ -114,70 +141,77 @@ __device__ __forceinline__ f32x16 mfma8(u32x4 a0, u32x4 a1, u32x4 b0, u32x4 b1, 
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
 }
 
-template <int TM>
+template <class G>
 struct Frags {
-    u32x4 a[2][Ring<TM>::NB], b[2][Ring<TM>::NB];  // two k blocks of a stage
+    u32x4 a[2][G::MB], b[2][G::NB];  // two k blocks of a stage
 };
+template <class G>
+using Acc = f32x16[G::MB][G::NB];
 
-// Interleaves a k block's MFMAs with the fragment reads of the next.
+// Interleaves NM MFMAs with the ND LDS reads of the next fragments.
 template <int NM, int ND>
 __device__ __forceinline__ void lin_interleave() {
-    constexpr int P = NM < ND ? NM : ND, PER = NM / P;
+    constexpr int P = NM < ND ? NM : ND, M = NM / P, D = ND / P;
 #pragma unroll
     for (int t = 0; t < P; ++t) {
-        __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, ND / P, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, D, 0);
     }
-    if constexpr (NM > P * PER) __builtin_amdgcn_sched_group_barrier(0x008, NM - P * PER, 0);
-    if constexpr (ND > P * (ND / P)) __builtin_amdgcn_sched_group_barrier(0x100, ND - P * (ND / P), 0);
+    if constexpr (NM > P * M) __builtin_amdgcn_sched_group_barrier(0x008, NM - P * M, 0);
+    if constexpr (ND > P * D) __builtin_amdgcn_sched_group_barrier(0x100, ND - P * D, 0);
+}
+
+template <int DT, class G>
+__device__ __forceinline__ void lin_mfma(const u32x4 (&a)[G::MB], const u32x4 (&b)[G::NB], Acc<G> &acc) {
+#pragma unroll
+    for (int i = 0; i < G::MB; ++i)
+#pragma unroll
+        for (int j = 0; j < G::NB; ++j) acc[i][j] = mfma16<DT>(a[i], b[j], acc[i][j]);
 }
 
 // 16-bit step on stage cur, as ring_step; f[0] holds block 0 of cur.
-template <int DT, int TM, bool KA, bool KB>
-__device__ __forceinline__ void lin_step16(const RingLoads<TM, KA, KB> &ld, size_t kf, uint16_t *cur,
-                                           const uint16_t *nxt, Frags<TM> &f, f32x16 (&acc)[Ring<TM>::NB][Ring<TM>::NB],
-                                           int am, int bn, int l32, int lhi) {
-    constexpr int NB = Ring<TM>::NB, TILE = Ring<TM>::TILE;
-    constexpr int NM = NB * NB, ND = NB * ((KA ? 1 : 2) + (KB ? 1 : 2));
-    side_frags<TM, KA>(cur, 1, am, l32, lhi, f.a[1]);
-    side_frags<TM, KB>(cur + TILE, 1, bn, l32, lhi, f.b[1]);
-    ring_mfma<DT, NB>(f.a[0], f.b[0], acc);
+template <int DT, class G, bool KA, bool KB>
+__device__ __forceinline__ void lin_step16(const RingLoads<G, KA, KB> &ld, size_t kf, uint16_t *cur, const uint16_t *nxt,
+                                           Frags<G> &f, Acc<G> &acc, int am, int bn, int l32, int lhi) {
+    constexpr int NM = G::MB * G::NB, ND = G::MB * (KA ? 1 : 2) + G::NB * (KB ? 1 : 2);
+    side_frags<G::TM, KA>(cur, 1, am, l32, lhi, f.a[1]);
+    side_frags<G::TN, KB>(cur + G::TA, 1, bn, l32, lhi, f.b[1]);
+    lin_mfma<DT, G>(f.a[0], f.b[0], acc);
     lin_interleave<NM, ND>();
-    ring_barrier<2 * Ring<TM>::PER_STAGE>();
-    side_frags<TM, KA>(nxt, 0, am, l32, lhi, f.a[0]);
-    side_frags<TM, KB>(nxt + TILE, 0, bn, l32, lhi, f.b[0]);
+    ring_barrier<2 * G::PS>();
+    side_frags<G::TM, KA>(nxt, 0, am, l32, lhi, f.a[0]);
+    side_frags<G::TN, KB>(nxt + G::TA, 0, bn, l32, lhi, f.b[0]);
     ld.issue(kf, cur);
-    ring_mfma<DT, NB>(f.a[1], f.b[1], acc);
+    lin_mfma<DT, G>(f.a[1], f.b[1], acc);
     lin_interleave<NM, ND>();
-    __builtin_amdgcn_sched_group_barrier(0x020, Ring<TM>::PER_STAGE, 0);
+    __builtin_amdgcn_sched_group_barrier(0x020, G::PS, 0);
 }
 
 // e4m3 step: f holds all of cur's stage, g gets all of nxt's.
-template <int TM>
-__device__ __forceinline__ void lin_step8(const RingLoads<TM, true, true> &ld, size_t kf, uint16_t *cur,
-                                          const uint16_t *nxt, const Frags<TM> &f, Frags<TM> &g,
-                                          f32x16 (&acc)[Ring<TM>::NB][Ring<TM>::NB], int am, int bn, int l32, int lhi) {
-    constexpr int NB = Ring<TM>::NB, TILE = Ring<TM>::TILE;
-    ring_barrier<2 * Ring<TM>::PER_STAGE>();
+template <class G>
+__device__ __forceinline__ void lin_step8(const RingLoads<G, true, true> &ld, size_t kf, uint16_t *cur,
+                                          const uint16_t *nxt, const Frags<G> &f, Frags<G> &g, Acc<G> &acc, int am,
+                                          int bn, int l32, int lhi) {
+    ring_barrier<2 * G::PS>();
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-        side_frags<TM, true>(nxt, kb, am, l32, lhi, g.a[kb]);
-        side_frags<TM, true>(nxt + TILE, kb, bn, l32, lhi, g.b[kb]);
+        side_frags<G::TM, true>(nxt, kb, am, l32, lhi, g.a[kb]);
+        side_frags<G::TN, true>(nxt + G::TA, kb, bn, l32, lhi, g.b[kb]);
     }
     ld.issue(kf, cur);
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
+    for (int i = 0; i < G::MB; ++i)
 #pragma unroll
-        for (int j = 0; j < NB; ++j) acc[i][j] = mfma8(f.a[0][i], f.a[1][i], f.b[0][j], f.b[1][j], acc[i][j]);
-    lin_interleave<NB * NB, 4 * NB>();
-    __builtin_amdgcn_sched_group_barrier(0x020, Ring<TM>::PER_STAGE, 0);
+        for (int j = 0; j < G::NB; ++j) acc[i][j] = mfma8(f.a[0][i], f.a[1][i], f.b[0][j], f.b[1][j], acc[i][j]);
+    lin_interleave<G::MB * G::NB, 2 * (G::MB + G::NB)>();
+    __builtin_amdgcn_sched_group_barrier(0x020, G::PS, 0);
 }
 
 // The tile's sums through the wave's LDS to rows of 8 elements per lane.
-template <int OT, int TM>
-__device__ __forceinline__ void lin_epilogue(const LinEpi &e, const f32x16 (&acc)[Ring<TM>::NB][Ring<TM>::NB],
-                                             float *lds, size_t m0, size_t n0, size_t M, size_t N, int l32, int lhi) {
-    constexpr int NB = Ring<TM>::NB, W = TM / 2, LP = W + 8;  // row stride: 4 rows on distinct halves of the banks
+template <int OT, class G>
+__device__ __forceinline__ void lin_epilogue(const LinEpi &e, const Acc<G> &acc, float *lds, size_t m0, size_t n0,
+                                             size_t M, size_t N, int l32, int lhi) {
+    constexpr int W = G::HN, LP = W + 8;  // row stride: 4 rows on distinct halves of the banks
     constexpr int LPR = W / 8, RPP = kWave / LPR;             // lanes per row, rows per pass
     const int lane = threadIdx.x & (kWave - 1);
     const int cl = 8 * (lane % LPR);
@@ -200,11 +234,11 @@ __device__ __forceinline__ void lin_epilogue(const LinEpi &e, const f32x16 (&acc
             if (i < own) cs[i] = e.cs[col + i];
     }
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
+    for (int i = 0; i < G::MB; ++i) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int j = 0; j < NB; ++j)
+        for (int j = 0; j < G::NB; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) lds[(8 * (r / 4) + 4 * lhi + (r % 4)) * LP + 32 * j + l32] = acc[i][j][r];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -261,72 +295,71 @@ __device__ __forceinline__ void lin_epilogue(const LinEpi &e, const f32x16 (&acc
     }
 }
 
-template <int DT, int OT, int TM, bool KA, bool KB>
-__global__ __launch_bounds__(kHThreads) void k_linear_ring(RingArgs a) {
-    constexpr int NB = Ring<TM>::NB, TILE = Ring<TM>::TILE, PS = Ring<TM>::PER_STAGE;
-    __shared__ __attribute__((aligned(16))) uint16_t s0[2 * TILE], s1[2 * TILE], s2[2 * TILE], s3[2 * TILE];
+template <int DT, int OT, class G, bool KA, bool KB>
+__global__ __launch_bounds__(G::NT) void k_linear_ring(RingArgs a) {
+    __shared__ __attribute__((aligned(16))) uint16_t s0[G::STAGE], s1[G::STAGE], s2[G::STAGE], s3[G::STAGE];
     __shared__ int flag;
     const unsigned wg = xcd_remap16(blockIdx.x, gridDim.x);
     const unsigned tile = wg / a.splits, split = wg - tile * a.splits;
     unsigned tm, tn;
     group_tile(tile, a.tiles_m, a.tiles_n, a.gm, &tm, &tn);
     const int wave = threadIdx.x / kWave;
-    const int am = (wave >> 1) * (TM / 2), bn = (wave & 1) * (TM / 2);
+    const int am = wave / G::WN * G::HM, bn = wave % G::WN * G::HN;
     const int lane = threadIdx.x & (kWave - 1), l32 = lane & 31, lhi = lane >> 5;
     const size_t first = static_cast<size_t>(split) * a.per;
     const size_t T = a.stages - first < a.per ? a.stages - first : a.per;  // this split's stages, at least 1
 
-    f32x16 acc[NB][NB];
+    Acc<G> acc;
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
+    for (int i = 0; i < G::MB; ++i)
 #pragma unroll
-        for (int j = 0; j < NB; ++j)
+        for (int j = 0; j < G::NB; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
     {
-        RingLoads<TM, KA, KB> ld;
+        RingLoads<G, KA, KB> ld;
         ld.A = a.A;
         ld.B = a.B;
         ld.lda = a.lda;
         ld.ldb = a.ldb;
-        ld.m0 = static_cast<size_t>(tm) * TM;
-        ld.n0 = static_cast<size_t>(tn) * TM;
-        ld.oa = lin_offs<TM, KA>(a.lda, a.M - ld.m0);
-        ld.ob = lin_offs<TM, KB>(a.ldb, a.N - ld.n0);
+        ld.m0 = static_cast<size_t>(tm) * G::TM;
+        ld.n0 = static_cast<size_t>(tn) * G::TN;
+        ld.oa.init(a.lda, a.M - ld.m0);
+        ld.ob.init(a.ldb, a.N - ld.n0);
         // stages past the last reload it into places whose fragments are not used
         auto kt = [&](size_t t) { return (first + (t < T ? t : T - 1)) * kR_BK; };
         ld.issue(kt(0), s0);
         ld.issue(kt(1), s1);
         ld.issue(kt(2), s2);
         ld.issue(kt(3), s3);
-        ring_barrier<3 * PS>();
-        Frags<TM> f;
-        side_frags<TM, KA>(s0, 0, am, l32, lhi, f.a[0]);
-        side_frags<TM, KB>(s0 + TILE, 0, bn, l32, lhi, f.b[0]);
+        ring_barrier<3 * G::PS>();
+        Frags<G> f;
+        side_frags<G::TM, KA>(s0, 0, am, l32, lhi, f.a[0]);
+        side_frags<G::TN, KB>(s0 + G::TA, 0, bn, l32, lhi, f.b[0]);
         size_t t = 0;
         if constexpr (DT == CXM_DT_E4M3) {
-            Frags<TM> g;
-            side_frags<TM, true>(s0, 1, am, l32, lhi, f.a[1]);
-            side_frags<TM, true>(s0 + TILE, 1, bn, l32, lhi, f.b[1]);
+            Frags<G> g;
+            side_frags<G::TM, true>(s0, 1, am, l32, lhi, f.a[1]);
+            side_frags<G::TN, true>(s0 + G::TA, 1, bn, l32, lhi, f.b[1]);
             for (; t + 4 <= T; t += 4) {
-                lin_step8<TM>(ld, kt(t + 4), s0, s1, f, g, acc, am, bn, l32, lhi);
-                lin_step8<TM>(ld, kt(t + 5), s1, s2, g, f, acc, am, bn, l32, lhi);
-                lin_step8<TM>(ld, kt(t + 6), s2, s3, f, g, acc, am, bn, l32, lhi);
-                lin_step8<TM>(ld, kt(t + 7), s3, s0, g, f, acc, am, bn, l32, lhi);
+                lin_step8<G>(ld, kt(t + 4), s0, s1, f, g, acc, am, bn, l32, lhi);
+                lin_step8<G>(ld, kt(t + 5), s1, s2, g, f, acc, am, bn, l32, lhi);
+                lin_step8<G>(ld, kt(t + 6), s2, s3, f, g, acc, am, bn, l32, lhi);
+                lin_step8<G>(ld, kt(t + 7), s3, s0, g, f, acc, am, bn, l32, lhi);
             }
-            if (t < T) lin_step8<TM>(ld, kt(t + 4), s0, s1, f, g, acc, am, bn, l32, lhi);
-            if (t + 1 < T) lin_step8<TM>(ld, kt(t + 5), s1, s2, g, f, acc, am, bn, l32, lhi);
-            if (t + 2 < T) lin_step8<TM>(ld, kt(t + 6), s2, s3, f, g, acc, am, bn, l32, lhi);
+            if (t < T) lin_step8<G>(ld, kt(t + 4), s0, s1, f, g, acc, am, bn, l32, lhi);
+            if (t + 1 < T) lin_step8<G>(ld, kt(t + 5), s1, s2, g, f, acc, am, bn, l32, lhi);
+            if (t + 2 < T) lin_step8<G>(ld, kt(t + 6), s2, s3, f, g, acc, am, bn, l32, lhi);
         } else {
             for (; t + 4 <= T; t += 4) {
-                lin_step16<DT, TM, KA, KB>(ld, kt(t + 4), s0, s1, f, acc, am, bn, l32, lhi);
-                lin_step16<DT, TM, KA, KB>(ld, kt(t + 5), s1, s2, f, acc, am, bn, l32, lhi);
-                lin_step16<DT, TM, KA, KB>(ld, kt(t + 6), s2, s3, f, acc, am, bn, l32, lhi);
-                lin_step16<DT, TM, KA, KB>(ld, kt(t + 7), s3, s0, f, acc, am, bn, l32, lhi);
+                lin_step16<DT, G, KA, KB>(ld, kt(t + 4), s0, s1, f, acc, am, bn, l32, lhi);
+                lin_step16<DT, G, KA, KB>(ld, kt(t + 5), s1, s2, f, acc, am, bn, l32, lhi);
+                lin_step16<DT, G, KA, KB>(ld, kt(t + 6), s2, s3, f, acc, am, bn, l32, lhi);
+                lin_step16<DT, G, KA, KB>(ld, kt(t + 7), s3, s0, f, acc, am, bn, l32, lhi);
             }
-            if (t < T) lin_step16<DT, TM, KA, KB>(ld, kt(t + 4), s0, s1, f, acc, am, bn, l32, lhi);
-            if (t + 1 < T) lin_step16<DT, TM, KA, KB>(ld, kt(t + 5), s1, s2, f, acc, am, bn, l32, lhi);
-            if (t + 2 < T) lin_step16<DT, TM, KA, KB>(ld, kt(t + 6), s2, s3, f, acc, am, bn, l32, lhi);
+            if (t < T) lin_step16<DT, G, KA, KB>(ld, kt(t + 4), s0, s1, f, acc, am, bn, l32, lhi);
+            if (t + 1 < T) lin_step16<DT, G, KA, KB>(ld, kt(t + 5), s1, s2, f, acc, am, bn, l32, lhi);
+            if (t + 2 < T) lin_step16<DT, G, KA, KB>(ld, kt(t + 6), s2, s3, f, acc, am, bn, l32, lhi);
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load into LDS is left
@@ -334,61 +367,60 @@ __global__ __launch_bounds__(kHThreads) void k_linear_ring(RingArgs a) {
     if (a.splits > 1) {
         const unsigned ws = xcd_remap16(blockIdx.x, gridDim.x);
         const unsigned ti = ws / a.splits, sp = ws - ti * a.splits;
-        float *base = a.part + static_cast<size_t>(ti) * a.splits * (TM * TM) + threadIdx.x;
-        float *my = base + static_cast<size_t>(sp) * (TM * TM);
+        float *base = a.part + static_cast<size_t>(ti) * a.splits * (G::TM * G::TN) + threadIdx.x;
+        float *my = base + static_cast<size_t>(sp) * (G::TM * G::TN);
 #pragma unroll
-        for (int i = 0; i < NB; ++i)
+        for (int i = 0; i < G::MB; ++i)
 #pragma unroll
-            for (int j = 0; j < NB; ++j)
+            for (int j = 0; j < G::NB; ++j)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) st_dev(my + ((i * NB + j) * 16 + r) * kHThreads, acc[i][j][r]);
+                for (int r = 0; r < 16; ++r) st_dev(my + ((i * G::NB + j) * 16 + r) * G::NT, acc[i][j][r]);
         if (!last_block_ticket(ctr(a.counters, ti), a.splits, &flag)) return;
 #pragma unroll
-        for (int i = 0; i < NB; ++i)
+        for (int i = 0; i < G::MB; ++i)
 #pragma unroll
-            for (int j = 0; j < NB; ++j)
+            for (int j = 0; j < G::NB; ++j)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
         for (unsigned q = 0; q < a.splits; ++q) {
-            const float *p = base + static_cast<size_t>(q) * (TM * TM);
+            const float *p = base + static_cast<size_t>(q) * (G::TM * G::TN);
 #pragma unroll
-            for (int i = 0; i < NB; ++i)
+            for (int i = 0; i < G::MB; ++i)
 #pragma unroll
-                for (int j = 0; j < NB; ++j)
+                for (int j = 0; j < G::NB; ++j)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) acc[i][j][r] += ld_dev(p + ((i * NB + j) * 16 + r) * kHThreads);
+                    for (int r = 0; r < 16; ++r) acc[i][j][r] += ld_dev(p + ((i * G::NB + j) * 16 + r) * G::NT);
         }
     }
     __syncthreads();  // every wave's fragment reads are done: the stages become the epilogue's
     // the tile origin again, from the workgroup index, so that it need not live across the K loop
     group_tile(xcd_remap16(blockIdx.x, gridDim.x) / a.splits, a.tiles_m, a.tiles_n, a.gm, &tm, &tn);
-    uint16_t *mine = wave == 0 ? s0 : wave == 1 ? s1 : wave == 2 ? s2 : s3;
-    lin_epilogue<OT, TM>(a.e, acc, reinterpret_cast<float *>(mine), static_cast<size_t>(tm) * TM + am,
-                         static_cast<size_t>(tn) * TM + bn, a.M, a.N, l32, lhi);
+    constexpr int SH = G::WAVES / 4;  // waves sharing a stage's array
+    static_assert(32 * (G::HN + 8) * 4 <= G::STAGE * 2 / SH, "a wave's 32 rows fit its part of a stage");
+    const int st = wave / SH;
+    uint16_t *mine = (st == 0 ? s0 : st == 1 ? s1 : st == 2 ? s2 : s3) + wave % SH * (G::STAGE / SH);
+    lin_epilogue<OT, G>(a.e, acc, reinterpret_cast<float *>(mine), static_cast<size_t>(tm) * G::TM + am,
+                        static_cast<size_t>(tn) * G::TN + bn, a.M, a.N, l32, lhi);
 }
 
-template <int DT, int OT, int TM, bool KA, bool KB>
-void ring_launch(const RingArgs &a, unsigned wgs, hipStream_t s) {
-    hipLaunchKernelGGL((k_linear_ring<DT, OT, TM, KA, KB>), dim3(wgs), dim3(kHThreads), 0, s, a);
-}
-
-template <int DT, int OT, int TM>
+template <int DT, int OT, class G>
 int ring_layout(const RingArgs &a, unsigned wgs, bool ta, bool tb, hipStream_t s) {
+    const dim3 grid(wgs), block(G::NT);
     if constexpr (DT == CXM_DT_E4M3) {
-        ring_launch<DT, OT, TM, true, true>(a, wgs, s);
+        hipLaunchKernelGGL((k_linear_ring<DT, OT, G, true, true>), grid, block, 0, s, a);
     } else {
-        if (!ta && !tb) ring_launch<DT, OT, TM, true, false>(a, wgs, s);
-        else if (!ta) ring_launch<DT, OT, TM, true, true>(a, wgs, s);
-        else ring_launch<DT, OT, TM, false, false>(a, wgs, s);
+        if (!ta && !tb) hipLaunchKernelGGL((k_linear_ring<DT, OT, G, true, false>), grid, block, 0, s, a);
+        else if (!ta) hipLaunchKernelGGL((k_linear_ring<DT, OT, G, true, true>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((k_linear_ring<DT, OT, G, false, false>), grid, block, 0, s, a);
     }
     return launch_status();
 }
 
 template <int DT, int OT>
 int ring_tile(const RingArgs &a, unsigned wgs, int tm, bool ta, bool tb, hipStream_t s) {
-    if (tm == 256) return ring_layout<DT, OT, 256>(a, wgs, ta, tb, s);
-    if (tm == 128) return ring_layout<DT, OT, 128>(a, wgs, ta, tb, s);
-    return ring_layout<DT, OT, 64>(a, wgs, ta, tb, s);
+    if (tm == 256) return ring_layout<DT, OT, Geo<256, 256, 2, 4>>(a, wgs, ta, tb, s);
+    if (tm == 128) return ring_layout<DT, OT, Geo<128, 128, 2, 4>>(a, wgs, ta, tb, s);
+    return ring_layout<DT, OT, Geo<64, 64, 2, 2>>(a, wgs, ta, tb, s);
 }
 
 }  // namespace

@@ -16,12 +16,13 @@
 // changes it by 1 - b2 = 0.1% would never leave a value (half a step is 3 to
 // 6%).  A root above zero is never stored as zero, which would divide a
 // moment by eps alone.
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <memory>
 #include <new>
+#include <type_traits>
 #include <vector>
-#include <algorithm>
 
 #include "chunk.hpp"
 
@@ -30,9 +31,13 @@ struct cxm_adamw;
 namespace cxm {
 namespace {
 
-constexpr unsigned kLane = 8;                // values per thread
-constexpr unsigned kPiece = kBlock * kLane;  // values per workgroup
-constexpr unsigned kBlock8 = 256;            // values per scale: 32 lanes
+typedef unsigned u32x2a __attribute__((ext_vector_type(2)));
+
+typedef unsigned u32x2a __attribute__((ext_vector_type(2)));
+
+constexpr unsigned kBlock8 = 256;                   // values per scale: 64 lanes of 4
+constexpr unsigned kLane = 4, kUnits = 2;           // values of a thread: kUnits times kLane, a wave's lanes side by side
+constexpr unsigned kPiece = kBlock * kLane * kUnits;  // values per workgroup
 
 struct AdamTensor {
     void *p;
@@ -68,90 +73,106 @@ __device__ __forceinline__ unsigned noise32(unsigned long long c, unsigned key) 
     return x ^ (x >> 16);
 }
 
-// a in [0, 448] to e4m3's neighbour above with the probability of a's distance
-// to the one below: 16 random bits are added below the 3 kept mantissa bits and
-// the rest cut off.  Below 2^-6 the steps are even (2^-9): 2^-6 is added
-// first and taken off after.
-__device__ __forceinline__ float round_e4m3(float a, unsigned bits) {
-    const float low = a < 0x1p-6f ? 0x1p-6f : 0.0f;
-    const float b = a + low;
-    const unsigned u = (__builtin_bit_cast(unsigned, b) + (bits << 4)) & ~0xFFFFFu;
-    return __builtin_bit_cast(float, u) - low;
+// Byte SEL of `w` becomes v (|v| up to 448) as e4m3, its magnitude rounded to
+// the neighbour above with the probability of the distance to the one below:
+// v_cvt_sr_fp8_f32 adds the upper 20 bits of `rnd` below the 3 kept mantissa
+// bits and cuts the rest off (below 2^-6 below the even steps of 2^-9).
+template <int SEL>
+__device__ __forceinline__ unsigned round_e4m3(float v, unsigned rnd, unsigned w) {
+    return static_cast<unsigned>(__builtin_amdgcn_cvt_sr_fp8_f32(v, static_cast<int>(rnd), static_cast<int>(w), SEL));
 }
+// The largest of |v| that is finite, over the wave (a block).
+__device__ __forceinline__ float block_amax(const float (&v)[kLane]) {
+    float m = 0.0f;
+#pragma unroll
+    for (unsigned e = 0; e < kLane; ++e) m = fmaxf(m, fabsf(v[e]));  // a NaN is passed over
+    m = group_reduce<MaxOp, kWave>(m);
+    if (__builtin_expect(m > FLT_MAX, 0)) {  // the same in every lane
+        m = 0.0f;
+#pragma unroll
+        for (unsigned e = 0; e < kLane; ++e) m = fabsf(v[e]) <= FLT_MAX ? fmaxf(m, fabsf(v[e])) : m;
+        m = group_reduce<MaxOp, kWave>(m);
+    }
+    return m;
+}
+
+// Four elements of a type in registers, whole or one by one.
+template <int DT>
+struct Quad {
+    float v[kLane];
+    __device__ __forceinline__ void load(const typename Elem<DT>::S *p) {
+        if constexpr (DT == CXM_DT_F32) {
+            const float4 x = ld4_stream(p);
+            v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+        } else {
+            const u32x2a x = __builtin_nontemporal_load(reinterpret_cast<const u32x2a *>(p));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = H<DT>::load(static_cast<uint16_t>(x[e / 2] >> (16 * (e & 1))));
+        }
+    }
+    __device__ __forceinline__ void store(typename Elem<DT>::S *p) const {
+        if constexpr (DT == CXM_DT_F32) st4_stream(p, make_float4(v[0], v[1], v[2], v[3]));
+        else
+            __builtin_nontemporal_store(u32x2a{pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])},
+                                        reinterpret_cast<u32x2a *>(p));
+    }
+};
 
 template <int PD, int GD, bool MASTER, bool Q8>
 __global__ __launch_bounds__(kBlock) void k_adamw(AdamStep a) {
     using PS = typename Elem<PD>::S;
     using GS = typename Elem<GD>::S;
     const AdamTensor t = a.tensors[a.owner[blockIdx.x]];
-    const size_t i0 = static_cast<size_t>(blockIdx.x - t.piece0) * kPiece + threadIdx.x * kLane;
-    const bool whole = t.vec && i0 + kLane <= t.n;
     PS *p = static_cast<PS *>(t.p);
     const GS *g = static_cast<const GS *>(t.g);
+    auto *m8 = static_cast<uint8_t *>(t.m), *v8 = static_cast<uint8_t *>(t.v);
+    auto *m32 = static_cast<float *>(t.m), *v32 = static_cast<float *>(t.v);
+    const unsigned lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
+    const size_t i00 = static_cast<size_t>(blockIdx.x - t.piece0) * kPiece + w * (kBlock8 * kUnits) + lane * kLane;
 
-    float vp[kLane], vg[kLane], vm[kLane], vv[kLane];
-    size_t blk = i0 / kBlock8;
+    Quad<CXM_DT_F32> m[kUnits], v[kUnits], wt[kUnits];
+    Quad<GD> gr[kUnits];
+    Quad<PD> pp[kUnits];
+    unsigned qm[kUnits], qv[kUnits];
+    float sm[kUnits], sv[kUnits];
+    bool whole[kUnits];
+    size_t blk[kUnits];
     const size_t blocks = (t.n + kBlock8 - 1) / kBlock8;
-    const bool leads = Q8 && blk < blocks && i0 % kBlock8 == 0;
-    if (blk >= blocks) blk = blocks - 1;
-    float sm = 0.0f, sv = 0.0f;
-    if constexpr (Q8) {
-        sm = t.ms[blk];
-        sv = t.vs[blk];
-    }
-    auto load_f = [](const float *q, float (&o)[kLane]) {
-        const float4 x = ld4(q), y = ld4(q + 4);
-        o[0] = x.x; o[1] = x.y; o[2] = x.z; o[3] = x.w;
-        o[4] = y.x; o[5] = y.y; o[6] = y.z; o[7] = y.w;
-    };
-    if (whole) {
-        if constexpr (MASTER) {
-            load_f(t.w + i0, vp);
-        } else if constexpr (PD == CXM_DT_F32) {
-            load_f(p + i0, vp);
-        } else {
-            Chunk<PD, 8> c;
-            c.load(p + i0);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) vp[e] = c.get(e);
+    for (unsigned u = 0; u < kUnits; ++u) {
+        const size_t i = i00 + u * kBlock8;
+        whole[u] = t.vec && i + kLane <= t.n;
+        blk[u] = i / kBlock8;
+        if constexpr (Q8) {  // a wave past the end takes the last block's scales and stores nothing
+            const size_t b = blk[u] < blocks ? blk[u] : blocks - 1;
+            sm[u] = t.ms[b];
+            sv[u] = t.vs[b];
         }
-        if constexpr (GD == CXM_DT_F32) {
-            load_f(g + i0, vg);
+        if (whole[u]) {
+            if constexpr (MASTER) wt[u].load(t.w + i);
+            else pp[u].load(p + i);
+            gr[u].load(g + i);
+            if constexpr (Q8) {
+                qm[u] = __builtin_nontemporal_load(reinterpret_cast<const unsigned *>(m8 + i));
+                qv[u] = __builtin_nontemporal_load(reinterpret_cast<const unsigned *>(v8 + i));
+            } else {
+                m[u].load(m32 + i);
+                v[u].load(v32 + i);
+            }
         } else {
-            Chunk<GD, 8> c;
-            c.load(g + i0);
+            qm[u] = qv[u] = 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) vg[e] = c.get(e);
-        }
-        if constexpr (Q8) {
-            const uint2 qm = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(t.m) + i0);
-            const uint2 qv = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(t.v) + i0);
-            unpack_e4m3(qm.x, vm);
-            unpack_e4m3(qm.y, vm + 4);
-            unpack_e4m3(qv.x, vv);
-            unpack_e4m3(qv.y, vv + 4);
-        } else {
-            load_f(static_cast<const float *>(t.m) + i0, vm);
-            load_f(static_cast<const float *>(t.v) + i0, vv);
-        }
-    } else {
-#pragma unroll
-        for (unsigned e = 0; e < kLane; ++e) {
-            const size_t i = i0 + e;
-            vp[e] = vg[e] = vm[e] = vv[e] = 0.0f;
-            if (i < t.n) {
-                if constexpr (MASTER) vp[e] = t.w[i];
-                else vp[e] = Elem<PD>::load(p[i]);
-                vg[e] = Elem<GD>::load(g[i]);
+            for (unsigned e = 0; e < kLane; ++e) {
+                const bool in = i + e < t.n;
+                wt[u].v[e] = MASTER && in ? t.w[i + e] : 0.0f;
+                pp[u].v[e] = !MASTER && in ? Elem<PD>::load(p[i + e]) : 0.0f;
+                gr[u].v[e] = in ? Elem<GD>::load(g[i + e]) : 0.0f;
                 if constexpr (Q8) {
-                    float u[4];
-                    unpack_e4m3(static_cast<const uint8_t *>(t.m)[i], u);
-                    vm[e] = u[0];
-                    unpack_e4m3(static_cast<const uint8_t *>(t.v)[i], u);
-                    vv[e] = u[0];
+                    qm[u] |= (in ? static_cast<unsigned>(m8[i + e]) : 0u) << (8 * e);
+                    qv[u] |= (in ? static_cast<unsigned>(v8[i + e]) : 0u) << (8 * e);
                 } else {
-                    vm[e] = static_cast<const float *>(t.m)[i];
-                    vv[e] = static_cast<const float *>(t.v)[i];
+                    m[u].v[e] = in ? m32[i + e] : 0.0f;
+                    v[u].v[e] = in ? v32[i + e] : 0.0f;
                 }
             }
         }
@@ -171,85 +192,78 @@ __global__ __launch_bounds__(kBlock) void k_adamw(AdamStep a) {
     }
     const float keep = static_cast<float>(1.0 - lr * static_cast<double>(t.decay));
 
-    float am = 0.0f, av = 0.0f;
 #pragma unroll
-    for (unsigned e = 0; e < kLane; ++e) {
-        const float gr = a.scalars ? vg[e] * factor : vg[e];
-        float m0 = vm[e], v0 = vv[e];
+    for (unsigned u = 0; u < kUnits; ++u) {
+        const size_t i = i00 + u * kBlock8;
         if constexpr (Q8) {
-            m0 *= sm;
-            v0 *= sv;
-            v0 *= v0;
+            unpack_e4m3(qm[u], m[u].v);
+            unpack_e4m3(qv[u], v[u].v);
         }
-        const float m1 = a.b1 * m0, m2 = a.b1c * gr, gg = gr * gr, v1 = a.b2 * v0, v2 = a.b2c * gg;
-        const float m = m1 + m2, v = v1 + v2, r = __builtin_sqrtf(v);
-        const float d = r * c2 + a.eps, u = c1 * m / d, q = vp[e] * keep;
-        vp[e] = q - u;
-        vm[e] = m;
-        vv[e] = Q8 ? r : v;
-        if constexpr (Q8) {  // the largest finite magnitudes
-            am = fabsf(m) <= FLT_MAX && fabsf(m) > am ? fabsf(m) : am;
-            av = r <= FLT_MAX && r > av ? r : av;
-        }
-    }
-    uint2 qm{0, 0}, qv{0, 0};
-    if constexpr (Q8) {
-        am = group_reduce<MaxOp, 32>(am);
-        av = group_reduce<MaxOp, 32>(av);
-        const Scale8 km = scale_e4m3(am), kv = scale_e4m3(av);
-        if (leads) {
-            t.ms[blk] = km.scale;
-            t.vs[blk] = kv.scale;
-        }
-        float em[kLane], ev[kLane];
+        float pn[kLane];
 #pragma unroll
         for (unsigned e = 0; e < kLane; ++e) {
-            const unsigned bits = noise32(t.first + i0 + e, a.key);
-            const float x = fabsf(vm[e]) * km.inv, y = vv[e] * kv.inv;
+            const float gv = a.scalars ? gr[u].v[e] * factor : gr[u].v[e];
+            float m0 = m[u].v[e], v0 = v[u].v[e];
+            if constexpr (Q8) {
+                m0 *= sm[u];
+                v0 *= sv[u];
+                v0 *= v0;
+            }
+            const float m1 = a.b1 * m0, m2 = a.b1c * gv, gg = gv * gv, v1 = a.b2 * v0, v2 = a.b2c * gg;
+            const float mn = m1 + m2, vn = v1 + v2, r = __builtin_sqrtf(vn);
+            const float d = r * c2 + a.eps, q = (MASTER ? wt[u].v[e] : pp[u].v[e]) * keep;
+            // the quotient by the reciprocal estimate (1 ulp) of a normal divisor: its
+            // error is 2^-23 of an update that is itself a small part of p
+            const float up = c1 * mn * (d >= FLT_MIN ? __builtin_amdgcn_rcpf(d) : 1.0f / d);
+            pn[e] = q - up;
+            m[u].v[e] = mn;
+            v[u].v[e] = Q8 ? r : vn;
+        }
+        if constexpr (Q8) {
+            const Scale8 km = scale_e4m3(block_amax(m[u].v)), kv = scale_e4m3(block_amax(v[u].v));
+            if (lane == 0 && blk[u] < blocks) {
+                t.ms[blk[u]] = km.scale;
+                t.vs[blk[u]] = kv.scale;
+            }
             // NaN and infinity are stored as NaN, where they are alone
-            const float qx = round_e4m3(x < kE4M3Max ? x : kE4M3Max, bits & 0xFFFFu);
-            float qy = round_e4m3(y < kE4M3Max ? y : kE4M3Max, bits >> 16);
-            qy = qy == 0.0f && y > 0.0f ? 0x1p-9f : qy;
-            em[e] = fabsf(vm[e]) <= FLT_MAX ? __builtin_copysignf(qx, vm[e]) : __builtin_nanf("");
-            ev[e] = vv[e] <= FLT_MAX ? qy : __builtin_nanf("");
+            auto put = [&](auto sel) {
+                constexpr int S = decltype(sel)::value;
+                const unsigned bits = noise32(t.first + i + S, a.key);
+                const float x = m[u].v[S] * km.inv, y = v[u].v[S] * kv.inv;
+                // a root above zero that would be 0 or 2^-9 is 2^-9
+                const float yy = y > 0.0f && y < 0x1p-9f ? 0x1p-9f : y;
+                qm[u] = round_e4m3<S>(fabsf(m[u].v[S]) <= FLT_MAX ? x : __builtin_nanf(""), bits << 16, qm[u]);
+                qv[u] = round_e4m3<S>(v[u].v[S] <= FLT_MAX ? yy : __builtin_nanf(""), bits & 0xFFFF0000u, qv[u]);
+            };
+            put(std::integral_constant<int, 0>{});
+            put(std::integral_constant<int, 1>{});
+            put(std::integral_constant<int, 2>{});
+            put(std::integral_constant<int, 3>{});
         }
-        qm = uint2{pack_e4m3(em[0], em[1], em[2], em[3]), pack_e4m3(em[4], em[5], em[6], em[7])};
-        qv = uint2{pack_e4m3(ev[0], ev[1], ev[2], ev[3]), pack_e4m3(ev[4], ev[5], ev[6], ev[7])};
-    }
-
-    auto store_f = [](float *q, const float (&o)[kLane]) {
-        st4(q, make_float4(o[0], o[1], o[2], o[3]));
-        st4(q + 4, make_float4(o[4], o[5], o[6], o[7]));
-    };
-    if (whole) {
-        if constexpr (MASTER) store_f(t.w + i0, vp);
-        if constexpr (PD == CXM_DT_F32) {
-            store_f(p + i0, vp);
-        } else {
-            Chunk<PD, 8> c;
-            c.set(vp);
-            c.store(p + i0);
-        }
-        if constexpr (Q8) {
-            *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(t.m) + i0) = qm;
-            *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(t.v) + i0) = qv;
-        } else {
-            store_f(static_cast<float *>(t.m) + i0, vm);
-            store_f(static_cast<float *>(t.v) + i0, vv);
-        }
-    } else {
 #pragma unroll
-        for (unsigned e = 0; e < kLane; ++e) {
-            const size_t i = i0 + e;
-            if (i < t.n) {
-                if constexpr (MASTER) t.w[i] = vp[e];
-                p[i] = Elem<PD>::store(vp[e]);
+        for (unsigned e = 0; e < kLane; ++e) wt[u].v[e] = pp[u].v[e] = pn[e];
+        if (whole[u]) {
+            if constexpr (MASTER) wt[u].store(t.w + i);
+            pp[u].store(p + i);
+            if constexpr (Q8) {
+                __builtin_nontemporal_store(qm[u], reinterpret_cast<unsigned *>(m8 + i));
+                __builtin_nontemporal_store(qv[u], reinterpret_cast<unsigned *>(v8 + i));
+            } else {
+                m[u].store(m32 + i);
+                v[u].store(v32 + i);
+            }
+        } else {
+#pragma unroll
+            for (unsigned e = 0; e < kLane; ++e) {
+                if (i + e >= t.n) break;
+                if constexpr (MASTER) t.w[i + e] = pn[e];
+                p[i + e] = Elem<PD>::store(pn[e]);
                 if constexpr (Q8) {
-                    static_cast<uint8_t *>(t.m)[i] = static_cast<uint8_t>((e < 4 ? qm.x : qm.y) >> (8 * (e & 3)));
-                    static_cast<uint8_t *>(t.v)[i] = static_cast<uint8_t>((e < 4 ? qv.x : qv.y) >> (8 * (e & 3)));
+                    m8[i + e] = static_cast<uint8_t>(qm[u] >> (8 * e));
+                    v8[i + e] = static_cast<uint8_t>(qv[u] >> (8 * e));
                 } else {
-                    static_cast<float *>(t.m)[i] = vm[e];
-                    static_cast<float *>(t.v)[i] = vv[e];
+                    m32[i + e] = m[u].v[e];
+                    v32[i + e] = v[u].v[e];
                 }
             }
         }

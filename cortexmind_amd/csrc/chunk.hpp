@@ -41,6 +41,7 @@ __device__ __forceinline__ unsigned pack2(float a, float b) {
     else return __builtin_bit_cast(unsigned, f16x2{static_cast<_Float16>(a), static_cast<_Float16>(b)});
 }
 
+// load_nt and store_nt set the non-temporal hint, for what is touched once.
 // VE consecutive elements in registers: kVec (one 128-bit access) or 1.
 template <int DT, int VE>
 struct Chunk;
@@ -55,6 +56,14 @@ struct Chunk<CXM_DT_F32, VE> {
             r[0] = *p;
         }
     }
+    __device__ __forceinline__ void load_nt(const float *p) {
+        if constexpr (VE == 4) {
+            const f32x4e v = __builtin_nontemporal_load(reinterpret_cast<const f32x4e *>(p));
+            r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
+        } else {
+            r[0] = *p;
+        }
+    }
     __device__ __forceinline__ float get(int e) const { return r[e]; }
     __device__ __forceinline__ void set(const float (&v)[VE]) {
 #pragma unroll
@@ -62,6 +71,10 @@ struct Chunk<CXM_DT_F32, VE> {
     }
     __device__ __forceinline__ void store(float *p) const {
         if constexpr (VE == 4) *reinterpret_cast<f32x4e *>(p) = f32x4e{r[0], r[1], r[2], r[3]};
+        else *p = r[0];
+    }
+    __device__ __forceinline__ void store_nt(float *p) const {
+        if constexpr (VE == 4) __builtin_nontemporal_store(f32x4e{r[0], r[1], r[2], r[3]}, reinterpret_cast<f32x4e *>(p));
         else *p = r[0];
     }
     __device__ __forceinline__ float raw(int e) const { return r[e]; }
@@ -72,6 +85,14 @@ struct Chunk {
     __device__ __forceinline__ void load(const uint16_t *p) {
         if constexpr (VE == 8) {
             const u32x4e v = *reinterpret_cast<const u32x4e *>(p);
+            r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
+        } else {
+            r[0] = *p;
+        }
+    }
+    __device__ __forceinline__ void load_nt(const uint16_t *p) {
+        if constexpr (VE == 8) {
+            const u32x4e v = __builtin_nontemporal_load(reinterpret_cast<const u32x4e *>(p));
             r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
         } else {
             r[0] = *p;
@@ -89,6 +110,10 @@ struct Chunk {
     }
     __device__ __forceinline__ void store(uint16_t *p) const {
         if constexpr (VE == 8) *reinterpret_cast<u32x4e *>(p) = u32x4e{r[0], r[1], r[2], r[3]};
+        else *p = static_cast<uint16_t>(r[0]);
+    }
+    __device__ __forceinline__ void store_nt(uint16_t *p) const {
+        if constexpr (VE == 8) __builtin_nontemporal_store(u32x4e{r[0], r[1], r[2], r[3]}, reinterpret_cast<u32x4e *>(p));
         else *p = static_cast<uint16_t>(r[0]);
     }
 };

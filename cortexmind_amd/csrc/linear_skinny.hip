@@ -116,50 +116,73 @@ __device__ __forceinline__ void skinny_join(const SkinnyArgs &a, unsigned tile, 
     }
 }
 
-// Weight [N, K], k along its rows: 16 columns n per workgroup.
-template <int DT, int OT, int MT>
+// Weight [N, K], k along its rows: 16 NR columns n per workgroup.  The two
+// 16-byte loads of a step take the halves of its 128 bytes, so that the four
+// lanes of a row read 64 contiguous bytes.
+template <int DT, int OT, int MT, int NR>
 __global__ __launch_bounds__(kSW *kWave) void k_linear_rows(SkinnyArgs a) {
     constexpr int D = MT == 4 ? 2 : 4;  // steps in flight
-    constexpr int E = MT * 256;
+    constexpr int NC = 16 * NR, E = MT * 16 * NC;
     __shared__ float sums[kSW * E];
     __shared__ int flag;
     const unsigned tile = blockIdx.x / a.splits, split = blockIdx.x - tile * a.splits;
-    const unsigned n0 = tile * 16;
+    const unsigned n0 = tile * NC;
     const int lane = threadIdx.x & (kWave - 1), r16 = lane & 15, q = lane >> 4;
     const unsigned w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const unsigned n = n0 + r16 < a.N ? n0 + r16 : a.N - 1;
-    const uint8_t *wp = a.w + static_cast<size_t>(n) * a.kb + 32 * q;
-    const uint8_t *xp[MT];
+    const uint8_t *wp[NR], *xp[MT];
+#pragma unroll
+    for (int j = 0; j < NR; ++j) {
+        const unsigned n = n0 + 16 * j + r16 < a.N ? n0 + 16 * j + r16 : a.N - 1;
+        wp[j] = a.w + static_cast<size_t>(n) * a.kb + 16 * q;
+    }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         const unsigned m = 16 * i + r16 < a.M ? 16 * i + r16 : a.M - 1;
-        xp[i] = a.x + static_cast<size_t>(m) * a.kb + 32 * q;
+        xp[i] = a.x + static_cast<size_t>(m) * a.kb + 16 * q;
     }
-    f32x4v acc[MT];
+    f32x4v acc[MT][NR];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) acc[i] = f32x4v{0.f, 0.f, 0.f, 0.f};
-    auto mul = [&](u32x4 w0, u32x4 w1, u32x4 x0, u32x4 x1, int i) {
-        if constexpr (DT == CXM_DT_E4M3) {
-            acc[i] = mfma_16x16_8(w0, w1, x0, x1, acc[i]);
-        } else {
-            acc[i] = mfma_16x16<DT>(w0, x0, acc[i]);
-            acc[i] = mfma_16x16<DT>(w1, x1, acc[i]);
-        }
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NR; ++j) acc[i][j] = f32x4v{0.f, 0.f, 0.f, 0.f};
+    auto mul = [&](const u32x4 (&u)[NR][2], const u32x4 (&v)[MT][2]) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NR; ++j) {
+                if constexpr (DT == CXM_DT_E4M3) {
+                    acc[i][j] = mfma_16x16_8(u[j][0], u[j][1], v[i][0], v[i][1], acc[i][j]);
+                } else {
+                    acc[i][j] = mfma_16x16<DT>(u[j][0], v[i][0], acc[i][j]);
+                    acc[i][j] = mfma_16x16<DT>(u[j][1], v[i][1], acc[i][j]);
+                }
+            }
     };
-    // whole steps of 128 bytes: this split's [s0, s1), every kSW-th of them
+    // whole steps of 128 bytes: wave w's share of this split's [s0, s1), one
+    // after the other from a place that moves with the tile: rows a power of
+    // two apart, read by every workgroup at the same k, meet in few of the
+    // memory channels
     const unsigned whole = static_cast<unsigned>(a.kb / 128);
     const unsigned s0 = split * a.per, s1 = s0 + a.per < whole ? s0 + a.per : whole;
-    const unsigned T = s1 > s0 + w ? (s1 - s0 - w + kSW - 1) / kSW : 0;
-    auto at = [&](unsigned t) { return static_cast<size_t>(s0 + w + (t < T ? t : T - 1) * kSW) * 128; };
-    u32x4 fw[D][2], fx[D][MT][2];
+    const unsigned all = s1 > s0 ? s1 - s0 : 0, each = (all + kSW - 1) / kSW;
+    const unsigned T = all > w * each ? (all - w * each < each ? all - w * each : each) : 0;
+    const unsigned turn = T ? tile % T : 0;
+    auto at = [&](unsigned t) {
+        const unsigned u = (t < T ? t : T - 1) + turn;
+        return static_cast<size_t>(s0 + w * each + (u < T ? u : u - T)) * 128;
+    };
+    u32x4 fw[D][NR][2], fx[D][MT][2];
     auto load = [&](int d, unsigned t) {
         const size_t o = at(t);
-        fw[d][0] = ld16(wp + o);
-        fw[d][1] = ld16(wp + o + 16);
+#pragma unroll
+        for (int j = 0; j < NR; ++j) {
+            fw[d][j][0] = ld16(wp[j] + o);
+            fw[d][j][1] = ld16(wp[j] + o + 64);
+        }
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             fx[d][i][0] = ld16(xp[i] + o);
-            fx[d][i][1] = ld16(xp[i] + o + 16);
+            fx[d][i][1] = ld16(xp[i] + o + 64);
         }
     };
     if (T > 0) {
@@ -169,40 +192,38 @@ __global__ __launch_bounds__(kSW *kWave) void k_linear_rows(SkinnyArgs a) {
         for (; t + D <= T; t += D) {
 #pragma unroll
             for (int d = 0; d < D; ++d) {
-#pragma unroll
-                for (int i = 0; i < MT; ++i) mul(fw[d][0], fw[d][1], fx[d][i][0], fx[d][i][1], i);
+                mul(fw[d], fx[d]);
                 load(d, t + d + D);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
 #pragma unroll
         for (int d = 0; d < D; ++d)
-            if (t + d < T) {
-#pragma unroll
-                for (int i = 0; i < MT; ++i) mul(fw[d][0], fw[d][1], fx[d][i][0], fx[d][i][1], i);
-            }
+            if (t + d < T) mul(fw[d], fx[d]);
     }
-    const unsigned rest = static_cast<unsigned>(a.kb % 128);
-    if (rest != 0 && split == a.splits - 1 && w == whole % kSW) {
+    const int rest = static_cast<int>(a.kb % 128);
+    if (rest != 0 && split == a.splits - 1 && w == kSW - 1) {  // the last wave's share is the shortest
         const size_t o = static_cast<size_t>(whole) * 128;
-        u32x4 u[2], v[2];
+        u32x4 u[NR][2], v[MT][2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) u[h] = ld16_part(wp + o + 16 * h, static_cast<int>(rest) - 32 * q - 16 * h);
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
+            for (int j = 0; j < NR; ++j) u[j][h] = ld16_part(wp[j] + o + 64 * h, rest - 16 * q - 64 * h);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) v[h] = ld16_part(xp[i] + o + 16 * h, static_cast<int>(rest) - 32 * q - 16 * h);
-            mul(u[0], u[1], v[0], v[1], i);
+            for (int i = 0; i < MT; ++i) v[i][h] = ld16_part(xp[i] + o + 64 * h, rest - 16 * q - 64 * h);
         }
+        mul(u, v);
     }
     // accumulator register r of lane l: n = 4 (l / 16) + r, m = l % 16
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sums[w * E + (16 * i + r16) * 16 + 4 * q + r] = acc[i][r];
+        for (int j = 0; j < NR; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sums[w * E + (16 * i + r16) * NC + 16 * j + 4 * q + r] = acc[i][j][r];
     __syncthreads();
     skinny_join<E>(a, tile, split, sums, &flag, [&](int p, float v) {
-        const unsigned m = p / 16, c = n0 + p % 16;
+        const unsigned m = p / NC, c = n0 + p % NC;
         if (m < a.M && c < a.N) skinny_store<OT>(a.e, v, m, c, a.N);
     });
 }
@@ -314,18 +335,27 @@ __global__ __launch_bounds__(kSW *kWave) void k_linear_cols(SkinnyArgs a) {
 }
 
 template <int DT, int OT>
-int skinny_launch(const SkinnyArgs &a, bool tb, hipStream_t s) {
+int skinny_launch(const SkinnyArgs &a, bool tb, int nr, hipStream_t s) {
     const dim3 grid(a.tiles * a.splits), block(kSW * kWave);
     if (tb) {
-        if (a.M <= 16) hipLaunchKernelGGL((k_linear_rows<DT, OT, 1>), grid, block, 0, s, a);
-        else if (a.M <= 32) hipLaunchKernelGGL((k_linear_rows<DT, OT, 2>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((k_linear_rows<DT, OT, 4>), grid, block, 0, s, a);
+        if (a.M <= 16 && nr == 1) hipLaunchKernelGGL((k_linear_rows<DT, OT, 1, 1>), grid, block, 0, s, a);
+        else if (a.M <= 16) hipLaunchKernelGGL((k_linear_rows<DT, OT, 1, 2>), grid, block, 0, s, a);
+        else if (a.M <= 32) hipLaunchKernelGGL((k_linear_rows<DT, OT, 2, 2>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((k_linear_rows<DT, OT, 4, 1>), grid, block, 0, s, a);
     } else if constexpr (DT != CXM_DT_E4M3) {
         if (a.M <= 16) hipLaunchKernelGGL((k_linear_cols<DT, OT, 1>), grid, block, 0, s, a);
         else if (a.M <= 32) hipLaunchKernelGGL((k_linear_cols<DT, OT, 2>), grid, block, 0, s, a);
         else hipLaunchKernelGGL((k_linear_cols<DT, OT, 4>), grid, block, 0, s, a);
     }
     return launch_status();
+}
+
+// Tiles of 16 outputs per workgroup, weight [N, K].
+int rows_tiles(size_t M, size_t N) {
+    if (M > 32) return 1;
+    if (M > 16) return 2;
+    (void)N;
+    return 1;
 }
 
 }  // namespace
@@ -337,7 +367,7 @@ int linear_skinny_plan(const LinProduct &p, LinPlan *l) {
     if (p.M > 64 || p.ta || (!p.tb && p.N < 8) || kb >= (size_t(1) << 31) || p.N >= kMax) return kDeclined;
     *l = LinPlan{};
     l->kernel = 0;
-    const size_t width = p.tb ? 16 : 128, step = p.tb ? 128 : 32;
+    const size_t width = p.tb ? 16 * rows_tiles(p.M, p.N) : 128, step = p.tb ? 128 : 32;
     l->tiles = (p.N + width - 1) / width;
     const size_t whole = kb / step, target = 2 * device_cus();
     l->splits = 1;
@@ -370,12 +400,13 @@ int linear_skinny_run(const LinProduct &p, const LinPlan &l, float *part, unsign
                        part,
                        counters,
                        p.e};
+    const int nr = rows_tiles(p.M, p.N);
     if (p.dtype == CXM_DT_E4M3) {
-        if (p.out == CXM_DT_BF16) return skinny_launch<CXM_DT_E4M3, CXM_DT_BF16>(a, true, s);
-        return skinny_launch<CXM_DT_E4M3, CXM_DT_F16>(a, true, s);
+        if (p.out == CXM_DT_BF16) return skinny_launch<CXM_DT_E4M3, CXM_DT_BF16>(a, true, nr, s);
+        return skinny_launch<CXM_DT_E4M3, CXM_DT_F16>(a, true, nr, s);
     }
-    if (p.dtype == CXM_DT_BF16) return skinny_launch<CXM_DT_BF16, CXM_DT_BF16>(a, p.tb, s);
-    return skinny_launch<CXM_DT_F16, CXM_DT_F16>(a, p.tb, s);
+    if (p.dtype == CXM_DT_BF16) return skinny_launch<CXM_DT_BF16, CXM_DT_BF16>(a, p.tb, nr, s);
+    return skinny_launch<CXM_DT_F16, CXM_DT_F16>(a, p.tb, nr, s);
 }
 
 }  // namespace cxm

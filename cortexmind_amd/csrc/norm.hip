@@ -43,6 +43,12 @@ struct AmaxOp : MaxOp {
     __device__ static T identity() { return 0.0f; }
 };
 
+template <bool ONCE, int DT, int VE>
+__device__ __forceinline__ void load_once(Chunk<DT, VE> &c, const typename Elem<DT>::S *p) {
+    if constexpr (ONCE) c.load_nt(p);
+    else c.load(p);
+}
+
 template <class Op, int G, int NT>
 __device__ __forceinline__ float row_reduce(float v, float *lds) {
     if constexpr (G <= kWave) return group_reduce<Op, G>(v);
@@ -78,8 +84,11 @@ __device__ __forceinline__ void store_q(uint8_t *row, Span s, const float (&v)[V
     }
 }
 
-// G lanes per row, C chunks of VE elements per lane, NT threads.
-template <int DT, int VE, int G, int C, int NT>
+// G lanes per row, C chunks of VE elements per lane, NT threads.  AL: rows of
+// whole 128-byte lines, read with the non-temporal hint (4096x4096 bf16 to 8
+// bits 23.3 -> 21.2 us; rows of 1003 floats, whose waves share lines, 7.4 ->
+// 8.6, so those do without).  Outputs are what the next call reads: no hint.
+template <int DT, int VE, int G, int C, int NT, bool AL>
 __global__ __launch_bounds__(NT) void k_rms_fwd(RmsFwd a) {
     using S = typename Elem<DT>::S;
     constexpr int R = G <= kWave ? NT / G : 1;
@@ -97,10 +106,10 @@ __global__ __launch_bounds__(NT) void k_rms_fwd(RmsFwd a) {
 #pragma unroll
     for (int i = 0; i < C; ++i) s[i] = span_of<VE>(i * G + lane, a.cols);
 #pragma unroll
-    for (int i = 0; i < C; ++i) cx[i].load(x + s[i].off);
+    for (int i = 0; i < C; ++i) load_once<AL>(cx[i], x + s[i].off);
     if (a.res) {
 #pragma unroll
-        for (int i = 0; i < C; ++i) cr[i].load(res + s[i].off);
+        for (int i = 0; i < C; ++i) load_once<AL>(cr[i], res + s[i].off);
     }
     if (a.norm) {
 #pragma unroll
@@ -261,7 +270,7 @@ __global__ __launch_bounds__(NT) void k_rms_fwd_long(RmsFwd a) {
 // Backward: workgroup b takes rows b R, b R + 1, ... of every gridDim.x R,
 // loads a row while the one before it is reduced, and keeps its share of dw
 // in registers; the workgroups' shares meet in col_sum in a fixed order.
-template <int DT, int VE, int G, int C, int NT>
+template <int DT, int VE, int G, int C, int NT, bool AL>
 __global__ __launch_bounds__(NT) void k_rms_bwd(RmsBwd a) {
     using S = typename Elem<DT>::S;
     constexpr int R = G <= kWave ? NT / G : 1;
@@ -286,12 +295,12 @@ __global__ __launch_bounds__(NT) void k_rms_bwd(RmsBwd a) {
         const size_t base = (r < a.rows ? r : a.rows - 1) * a.cols;
 #pragma unroll
         for (int i = 0; i < C; ++i) {
-            ch[i].load(static_cast<const S *>(a.h) + base + s[i].off);
-            cd[i].load(static_cast<const S *>(a.dy) + base + s[i].off);
+            load_once<AL>(ch[i], static_cast<const S *>(a.h) + base + s[i].off);
+            load_once<AL>(cd[i], static_cast<const S *>(a.dy) + base + s[i].off);
         }
         if (a.dh) {
 #pragma unroll
-            for (int i = 0; i < C; ++i) ca[i].load(static_cast<const S *>(a.dh) + base + s[i].off);
+            for (int i = 0; i < C; ++i) load_once<AL>(ca[i], static_cast<const S *>(a.dh) + base + s[i].off);
         }
         rstd = a.rstd[r < a.rows ? r : a.rows - 1];
     };
@@ -444,12 +453,21 @@ __global__ __launch_bounds__(kBlock) void k_rms_dw_part(RmsBwd a) {
 
 inline hipStream_t hs(cxm_stream_t s) { return reinterpret_cast<hipStream_t>(s); }
 
+// Rows of whole 128-byte lines (null: yes).
+inline bool whole_lines(const void *p, size_t cols, size_t bytes) {
+    return (reinterpret_cast<uintptr_t>(p) | cols * bytes) % 128 == 0;
+}
+
 template <int DT, int VE, int G, int C, int NT>
 int fwd_launch(const RmsFwd &a, hipStream_t s) {
     constexpr int R = G <= kWave ? NT / G : 1;
     const size_t wgs = (a.rows + R - 1) / R;
     if (wgs > 0x7fffffffu) return CXM_E_TOO_LARGE;
-    hipLaunchKernelGGL((k_rms_fwd<DT, VE, G, C, NT>), dim3(static_cast<unsigned>(wgs)), dim3(NT), 0, s, a);
+    const dim3 grid(static_cast<unsigned>(wgs));
+    if (whole_lines(a.x, a.cols, sizeof(typename Elem<DT>::S)) && whole_lines(a.res, a.cols, sizeof(typename Elem<DT>::S)))
+        hipLaunchKernelGGL((k_rms_fwd<DT, VE, G, C, NT, true>), grid, dim3(NT), 0, s, a);
+    else
+        hipLaunchKernelGGL((k_rms_fwd<DT, VE, G, C, NT, false>), grid, dim3(NT), 0, s, a);
     return launch_status();
 }
 
@@ -482,8 +500,8 @@ int fwd_any(const RmsFwd &a, int dtype, hipStream_t s) {
 
 // Workgroups of the backward: enough to fill the chip, few enough that their
 // shares of dw are a small part of the traffic.
-size_t bwd_wgs(size_t rows, int per_wg, int nt) {
-    const size_t need = (rows + per_wg - 1) / per_wg, most = device_cus() * (nt <= 256 ? 4 : 2);
+size_t bwd_wgs(size_t rows, int per_wg) {
+    const size_t need = (rows + per_wg - 1) / per_wg, most = device_cus() * 2;
     return need < most ? need : most;
 }
 
@@ -499,10 +517,15 @@ int bwd_parts(RmsBwd *a, size_t parts, cxm_stream_t st) {
 template <int DT, int VE, int G, int C, int NT>
 int bwd_launch(RmsBwd a, void *dw, cxm_stream_t st) {
     constexpr int R = G <= kWave ? NT / G : 1;
-    const size_t wgs = bwd_wgs(a.rows, R, NT);
+    const size_t wgs = bwd_wgs(a.rows, R);
     const int rc = bwd_parts(&a, wgs, st);
     if (rc) return rc;
-    hipLaunchKernelGGL((k_rms_bwd<DT, VE, G, C, NT>), dim3(static_cast<unsigned>(wgs)), dim3(NT), 0, hs(st), a);
+    const dim3 grid(static_cast<unsigned>(wgs));
+    constexpr size_t E = sizeof(typename Elem<DT>::S);
+    if (whole_lines(a.h, a.cols, E) && whole_lines(a.dy, a.cols, E) && whole_lines(a.dh, a.cols, E))
+        hipLaunchKernelGGL((k_rms_bwd<DT, VE, G, C, NT, true>), grid, dim3(NT), 0, hs(st), a);
+    else
+        hipLaunchKernelGGL((k_rms_bwd<DT, VE, G, C, NT, false>), grid, dim3(NT), 0, hs(st), a);
     const int r = launch_status();
     return r ? r : col_sum(a.part, wgs, a.cols, a.ld, dw, DT, hs(st));
 }
@@ -515,7 +538,7 @@ int bwd_dispatch(RmsBwd a, void *dw, cxm_stream_t st) {
     if (chunks <= 16) return bwd_launch<DT, VE, 16, 1, 256>(a, dw, st);
     if (chunks <= 64) return bwd_launch<DT, VE, 64, 1, 256>(a, dw, st);
     if (chunks <= 128) return bwd_launch<DT, VE, 64, 2, 256>(a, dw, st);
-    if (chunks <= 256) return bwd_launch<DT, VE, 256, 1, 256>(a, dw, st);
+    if (chunks <= 256) return bwd_launch<DT, VE, 64, 4, 256>(a, dw, st);
     if (chunks <= 512) return bwd_launch<DT, VE, 256, 2, 256>(a, dw, st);
     if (chunks <= 1024) return bwd_launch<DT, VE, 512, 2, 512>(a, dw, st);
     if (chunks <= 2048) return bwd_launch<DT, VE, 1024, 2, 1024>(a, dw, st);

@@ -270,7 +270,7 @@ int run_one(const LinProduct &p, cxm_stream_t st) {
 
 // The ring's tile and K splits.
 int linear_plan(const LinProduct &p, LinPlan *l) {
-    if (linear_skinny_plan(p, l) == CXM_OK) return CXM_OK;
+    if (linear_skinny_plan(p, l)) return CXM_OK;
     *l = LinPlan{};
     const size_t unit = 2, es = dtype_bytes(p.dtype), kb = p.K * es;
     // rows of k: whole stages of 64 bytes; rows across k: whole chunks of 16 bytes, and whole stages of rows
@@ -284,22 +284,34 @@ int linear_plan(const LinProduct &p, LinPlan *l) {
     if (l->copy_a) l->bytes_a = up((p.ta ? kpad : p.M) * l->lda * unit, 256);
     if (l->copy_b) l->bytes_b = up((p.tb ? p.N : kpad) * l->ldb * unit, 256);
     const size_t cus = device_cus();
-    auto tiles = [&](size_t t) { return ((p.M + t - 1) / t) * ((p.N + t - 1) / t); };
-    l->kernel = tiles(256) >= cus * 3 / 4 ? 256 : tiles(128) >= cus * 5 / 8 ? 128 : 64;
-    const size_t t = static_cast<size_t>(l->kernel);
-    l->tiles_m = (p.M + t - 1) / t;
-    l->tiles_n = (p.N + t - 1) / t;
+    auto tiles = [&](size_t tm, size_t tn) { return ((p.M + tm - 1) / tm) * ((p.N + tn - 1) / tn); };
+    // The tile, by what these cost at K = 1024 (us; CUs of 256):
+    //  * 256: a round of up to one tile per CU about 37 (64 of them 27);
+    //  * 128: 10 and 11 for each 256 of them (64 of them 9.8, 240 13.3, 1024 45);
+    //  * 64, several on a CU: 3 and 3.9 for each 256 (256 of them 6.8, 960 19.2),
+    //    so 128 from half as many tiles as CUs;
+    //  * 32x64 up to 32 rows (16x4096x4096 10.1, on 64s 10.5; x8192 18.7 / 20.6).
+    const size_t t256 = tiles(256, 256), t128 = tiles(128, 128);
+    const double c256 = 3.4 * static_cast<double>((t256 + cus - 1) / cus), c128 = 1.0 + static_cast<double>(t128) / cus;
+    const bool few = p.M <= 32 && !p.ta;
+    l->kernel = few ? 32 : c256 <= c128 ? 256 : t128 >= cus / 2 ? 128 : 64;
+    const size_t tm = static_cast<size_t>(l->kernel), tn = few ? 64 : tm;
+    l->tiles_m = (p.M + tm - 1) / tm;
+    l->tiles_n = (p.N + tn - 1) / tn;
     l->tiles = l->tiles_m * l->tiles_n;
+    // K over up to one workgroup per CU, each split worth its meeting: 32
+    // stages where four groups share them, else 8 (16x1024x4096 on 64 tiles 5.8,
+    // in two 6.7; 512x4096x512 on 64 tiles 15.9, in four 10.0, in eight 10.6)
     l->splits = 1;
-    if (l->kernel == 64 && l->tiles < 2 * cus) {
-        l->splits = 2 * cus / l->tiles;
-        const size_t most = l->stages / 8;
+    if (tm <= 64 && l->tiles < cus) {
+        l->splits = cus / l->tiles;
+        const size_t most = l->stages / (few ? 32 : 8);
         if (l->splits > most) l->splits = most;
         if (l->splits < 1) l->splits = 1;
     }
     l->per = (l->stages + l->splits - 1) / l->splits;
     l->splits = (l->stages + l->per - 1) / l->per;
-    if (l->splits > 1) l->bytes_part = up(l->tiles * l->splits * t * t * sizeof(float), 256);
+    if (l->splits > 1) l->bytes_part = up(l->tiles * l->splits * tm * tn * sizeof(float), 256);
     return CXM_OK;
 }
 

@@ -28,7 +28,7 @@ struct LinProduct {
 };
 
 struct LinPlan {
-    int kernel;       // 0 skinny, else the ring's tile edge
+    int kernel;       // 0 skinny, else the rows of the ring's tile
     bool copy_a, copy_b;
     size_t lda, ldb;  // of what the ring reads, in its 16-bit units
     size_t stages;    // of 32 units along K
@@ -43,7 +43,7 @@ int linear_plan(const LinProduct &p, LinPlan *plan);
 // `scratch` holds plan.bytes() (256-byte aligned), `counters` plan.counters().
 int linear_run(const LinProduct &p, const LinPlan &plan, char *scratch, unsigned *counters, hipStream_t s);
 
-int linear_skinny_plan(const LinProduct &p, LinPlan *plan);
+bool linear_skinny_plan(const LinProduct &p, LinPlan *plan);
 int linear_skinny_run(const LinProduct &p, const LinPlan &plan, float *part, unsigned *counters, hipStream_t s);
 int linear_ring_run(const LinProduct &p, const LinPlan &plan, const void *a, const void *b, float *part,
                     unsigned *counters, hipStream_t s);

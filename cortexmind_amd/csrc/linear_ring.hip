@@ -6,7 +6,9 @@
 //  * eight waves, two per SIMD, on tiles of 256 and 128: one hides the
 //    other's barriers and the epilogue's latency (four waves of 128x128 ran
 //    4096x1024x4096 in 46.3 us against 37.5, 8192^3 at 1200 TFLOP/s against
-//    1320; 2500x1024x1504 on 128 tiles 15.1 against 13.3);
+//    1320; 2500x1024x1504 on 128 tiles 15.1 against 13.3, two K groups of
+//    four 14.8);
+//  * few rows: 32x64 tiles by four K groups of two waves;
 //  * any M and N: rows and columns past the end re-read the last ones, their
 //    sums are not stored;
 //  * either operand stored with k along its rows or across them (the
@@ -44,18 +46,28 @@ struct RingArgs {
     LinEpi e;
 };
 
-// A TM x TN tile by WM x WN waves: each wave's share of it and of the stages'
-// loads (one load instruction of a wave brings 1 KiB).
-template <int TM_, int TN_, int WM_, int WN_>
+// A TM x TN tile by KG groups of WM x WN waves.  The groups take the stages
+// of K in turns, each with a ring of its own, and add their sums in LDS at the
+// end (in their order): more waves and loads in flight where the tiles are few
+// and small.
+// One load instruction of a wave brings 1 KiB; a group of more waves than
+// an operand has such pieces loads some of them twice (the same bytes to the
+// same place).
+template <int TM_, int TN_, int WM_, int WN_, int KG_>
 struct Geo {
-    static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_;
-    static constexpr int WAVES = WM * WN, NT = WAVES * kWave;
+    static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, KG = KG_;
+    static constexpr int GW = WM * WN, WAVES = KG * GW, NT = WAVES * kWave;
     static constexpr int HM = TM / WM, HN = TN / WN;         // a wave's rows and columns
     static constexpr int MB = HM / 32, NB = HN / 32;         // its 32x32 blocks
-    static constexpr int IA = TM / (16 * WAVES), IB = TN / (16 * WAVES);
+    static constexpr int IA = TM >= 16 * GW ? TM / (16 * GW) : 1, IB = TN >= 16 * GW ? TN / (16 * GW) : 1;
     static constexpr int PS = IA + IB;                       // loads of a wave per stage
     static constexpr int TA = TM * kR_BK, STAGE = (TM + TN) * kR_BK;  // 16-bit units
-    static_assert(IA >= 1 && IB >= 1 && MB >= 1 && NB >= 1, "every wave loads and multiplies");
+    static constexpr int OWN = MB % KG == 0 ? MB / KG : MB;  // row blocks that a group finishes (else group 0 all)
+    static constexpr int EPI = 32 * (HN + 8);                // floats of a wave's epilogue rows
+    static_assert(MB >= 1 && NB >= 1, "every wave multiplies");
+    static constexpr int PER = WAVES / 4;                    // waves whose epilogue rows share a stage's array
+    static_assert(PER * EPI * 4 <= KG * STAGE * 2, "the epilogue fits the rings");
+    static_assert(KG <= 5 && (KG == 1 || GW * MB * NB * 1024 * 4 <= KG * STAGE * 2), "the groups' sums fit the rings");
 };
 
 // Byte offsets of this lane's loads of an operand's stage (T rows of 64 bytes
@@ -65,13 +77,18 @@ struct Geo {
 template <int T, int ISSUES, bool KC>
 struct SideLoads {
     unsigned o[ISSUES];
-    __device__ __forceinline__ void init(size_t ld, size_t left) {
-        const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
+    unsigned to;  // byte offset of the wave's first piece in the operand's stage
+    // w: the wave in its group
+    __device__ __forceinline__ void init(size_t ld, size_t left, unsigned w) {
+        constexpr unsigned PARTS = T / (16 * ISSUES);  // waves that share the stage
+        w %= PARTS;
+        to = w * (ISSUES * kWave * 16);
+        const int lane = threadIdx.x & (kWave - 1);
         if constexpr (KC) {
             const int rr = lane >> 2, p = lane & 3;
 #pragma unroll
             for (int s = 0; s < ISSUES; ++s) {
-                const int row = (w * ISSUES + s) * 16 + rr;
+                const int row = static_cast<int>(w * ISSUES + s) * 16 + rr;
                 const size_t r = static_cast<size_t>(row) < left ? row : left - 1;
                 o[s] = static_cast<unsigned>((r * ld + 8 * (p ^ rkey(row))) * sizeof(uint16_t));
             }
@@ -81,16 +98,15 @@ struct SideLoads {
             const size_t last = (left + 7) / 8 - 1;  // rows are stored in whole chunks
 #pragma unroll
             for (int s = 0; s < ISSUES; ++s) {
-                const int row = (w * ISSUES + s) * RPI + rr;
+                const int row = static_cast<int>(w * ISSUES + s) * RPI + rr;
                 const size_t c = p ^ nkey<T>(row);
                 o[s] = static_cast<unsigned>((row * ld + 8 * (c < last ? c : last)) * sizeof(uint16_t));
             }
         }
     }
     __device__ __forceinline__ void issue(const uint16_t *X, size_t r0, size_t k, size_t ld, uint16_t *stage) const {
-        const unsigned w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
         const uint16_t *base = KC ? X + r0 * ld + k : X + k * ld + r0;
-        const unsigned l0 = lds_addr(stage) + w * (ISSUES * kWave * 16);
+        const unsigned l0 = lds_addr(stage) + __builtin_amdgcn_readfirstlane(to);
 #pragma unroll
         for (int s = 0; s < ISSUES; ++s) lds_load16_at(base, o[s], l0 + s * kWave * 16);
     }
@@ -169,10 +185,25 @@ __device__ __forceinline__ void lin_mfma(const u32x4 (&a)[G::MB], const u32x4 (&
         for (int j = 0; j < G::NB; ++j) acc[i][j] = mfma16<DT>(a[i], b[j], acc[i][j]);
 }
 
-// 16-bit step on stage cur, as ring_step; f[0] holds block 0 of cur.
-template <int DT, class G, bool KA, bool KB>
+// 16-bit step on stage cur, as ring_step; f[0] holds block 0 of cur.  LAST:
+// one of the steps after the unrolled loop, where a group may have no stage
+// left (`live` false) and only keeps the barrier.
+template <int DT, class G, bool KA, bool KB, bool LAST>
 __device__ __forceinline__ void lin_step16(const RingLoads<G, KA, KB> &ld, size_t kf, uint16_t *cur, const uint16_t *nxt,
-                                           Frags<G> &f, Acc<G> &acc, int am, int bn, int l32, int lhi) {
+                                           Frags<G> &f, Acc<G> &acc, int am, int bn, int l32, int lhi, bool live) {
+    if constexpr (LAST) {
+        side_frags<G::TM, KA>(cur, 1, am, l32, lhi, f.a[1]);
+        side_frags<G::TN, KB>(cur + G::TA, 1, bn, l32, lhi, f.b[1]);
+        if (live) {
+            lin_mfma<DT, G>(f.a[0], f.b[0], acc);
+            lin_mfma<DT, G>(f.a[1], f.b[1], acc);
+        }
+        ring_barrier<2 * G::PS>();
+        side_frags<G::TM, KA>(nxt, 0, am, l32, lhi, f.a[0]);
+        side_frags<G::TN, KB>(nxt + G::TA, 0, bn, l32, lhi, f.b[0]);
+        ld.issue(kf, cur);
+        return;
+    }
     constexpr int NM = G::MB * G::NB, ND = G::MB * (KA ? 1 : 2) + G::NB * (KB ? 1 : 2);
     side_frags<G::TM, KA>(cur, 1, am, l32, lhi, f.a[1]);
     side_frags<G::TN, KB>(cur + G::TA, 1, bn, l32, lhi, f.b[1]);
@@ -187,30 +218,56 @@ __device__ __forceinline__ void lin_step16(const RingLoads<G, KA, KB> &ld, size_
     __builtin_amdgcn_sched_group_barrier(0x020, G::PS, 0);
 }
 
-// e4m3 step: f holds all of cur's stage, g gets all of nxt's.
-template <class G>
+// e4m3 step: f holds all of cur's stage and is refilled from nxt as its parts
+// have had their last product, the columns before the last ones before the
+// barrier: one set of fragments, where a second one spilled (the same 66 us at
+// 4096^3).
+template <class G, bool LAST>
 __device__ __forceinline__ void lin_step8(const RingLoads<G, true, true> &ld, size_t kf, uint16_t *cur,
-                                          const uint16_t *nxt, const Frags<G> &f, Frags<G> &g, Acc<G> &acc, int am,
-                                          int bn, int l32, int lhi) {
-    ring_barrier<2 * G::PS>();
+                                          const uint16_t *nxt, Frags<G> &f, Acc<G> &acc, int am, int bn, int l32, int lhi,
+                                          bool live) {
+    constexpr int J = G::NB - 1;
+    const uint16_t *nb = nxt + G::TA;
+    auto mul = [&](int i, int j) { acc[i][j] = mfma8(f.a[0][i], f.a[1][i], f.b[0][j], f.b[1][j], acc[i][j]); };
+    if (!LAST || live) {
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-        side_frags<G::TM, true>(nxt, kb, am, l32, lhi, g.a[kb]);
-        side_frags<G::TN, true>(nxt + G::TA, kb, bn, l32, lhi, g.b[kb]);
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+            for (int i = 0; i < G::MB; ++i) mul(i, j);
+        if constexpr (!LAST) __builtin_amdgcn_sched_group_barrier(0x008, J * G::MB, 0);
     }
+    ring_barrier<2 * G::PS>();
     ld.issue(kf, cur);
+    auto read_b = [&](int j) {
 #pragma unroll
-    for (int i = 0; i < G::MB; ++i)
+        for (int kb = 0; kb < 2; ++kb)
+            f.b[kb][j] = *reinterpret_cast<const u32x4 *>(nb + roff(bn + j * 32 + l32, 2 * kb + lhi));
+    };
 #pragma unroll
-        for (int j = 0; j < G::NB; ++j) acc[i][j] = mfma8(f.a[0][i], f.a[1][i], f.b[0][j], f.b[1][j], acc[i][j]);
-    lin_interleave<G::MB * G::NB, 2 * (G::MB + G::NB)>();
-    __builtin_amdgcn_sched_group_barrier(0x020, G::PS, 0);
+    for (int j = 0; j < J; ++j) read_b(j);
+#pragma unroll
+    for (int i = 0; i < G::MB; ++i) {
+        if (!LAST || live) mul(i, J);
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+            f.a[kb][i] = *reinterpret_cast<const u32x4 *>(nxt + roff(am + i * 32 + l32, 2 * kb + lhi));
+    }
+    read_b(J);
+    if constexpr (!LAST) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 * J, 0);
+#pragma unroll
+        for (int i = 0; i < G::MB; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
 }
 
 // The tile's sums through the wave's LDS to rows of 8 elements per lane.
 template <int OT, class G>
 __device__ __forceinline__ void lin_epilogue(const LinEpi &e, const Acc<G> &acc, float *lds, size_t m0, size_t n0,
-                                             size_t M, size_t N, int l32, int lhi) {
+                                             size_t M, size_t N, int l32, int lhi, int group) {
     constexpr int W = G::HN, LP = W + 8;  // row stride: 4 rows on distinct halves of the banks
     constexpr int LPR = W / 8, RPP = kWave / LPR;             // lanes per row, rows per pass
     const int lane = threadIdx.x & (kWave - 1);
@@ -235,6 +292,7 @@ __device__ __forceinline__ void lin_epilogue(const LinEpi &e, const Acc<G> &acc,
     }
 #pragma unroll
     for (int i = 0; i < G::MB; ++i) {
+        if (i / G::OWN != group) continue;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -297,17 +355,18 @@ __device__ __forceinline__ void lin_epilogue(const LinEpi &e, const Acc<G> &acc,
 
 template <int DT, int OT, class G, bool KA, bool KB>
 __global__ __launch_bounds__(G::NT) void k_linear_ring(RingArgs a) {
-    __shared__ __attribute__((aligned(16))) uint16_t s0[G::STAGE], s1[G::STAGE], s2[G::STAGE], s3[G::STAGE];
+    // an array per stage of the rings, each holding the groups'
+    constexpr int RS = G::KG * G::STAGE;
+    __shared__ __attribute__((aligned(16))) uint16_t r0[RS], r1[RS], r2[RS], r3[RS];
     __shared__ int flag;
     const unsigned wg = xcd_remap16(blockIdx.x, gridDim.x);
     const unsigned tile = wg / a.splits, split = wg - tile * a.splits;
     unsigned tm, tn;
     group_tile(tile, a.tiles_m, a.tiles_n, a.gm, &tm, &tn);
-    const int wave = threadIdx.x / kWave;
-    const int am = wave / G::WN * G::HM, bn = wave % G::WN * G::HN;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int group = G::KG > 1 ? wave / G::GW : 0, gw = G::KG > 1 ? wave % G::GW : wave;
+    const int am = gw / G::WN * G::HM, bn = gw % G::WN * G::HN;
     const int lane = threadIdx.x & (kWave - 1), l32 = lane & 31, lhi = lane >> 5;
-    const size_t first = static_cast<size_t>(split) * a.per;
-    const size_t T = a.stages - first < a.per ? a.stages - first : a.per;  // this split's stages, at least 1
 
     Acc<G> acc;
 #pragma unroll
@@ -317,6 +376,13 @@ __global__ __launch_bounds__(G::NT) void k_linear_ring(RingArgs a) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
     {
+        uint16_t *s0 = r0 + group * G::STAGE, *s1 = r1 + group * G::STAGE, *s2 = r2 + group * G::STAGE,
+                 *s3 = r3 + group * G::STAGE;
+        const size_t first = static_cast<size_t>(split) * a.per;
+        const size_t T = a.stages - first < a.per ? a.stages - first : a.per;  // this split's stages, at least 1
+        // group g takes stages g, g + KG, ...; all make the same number of steps
+        const size_t all = T / G::KG, steps = G::KG > 1 ? (T + G::KG - 1) / G::KG : T;
+        const size_t mine = G::KG > 1 ? (T + G::KG - 1 - group) / G::KG : T;
         RingLoads<G, KA, KB> ld;
         ld.A = a.A;
         ld.B = a.B;
@@ -324,10 +390,14 @@ __global__ __launch_bounds__(G::NT) void k_linear_ring(RingArgs a) {
         ld.ldb = a.ldb;
         ld.m0 = static_cast<size_t>(tm) * G::TM;
         ld.n0 = static_cast<size_t>(tn) * G::TN;
-        ld.oa.init(a.lda, a.M - ld.m0);
-        ld.ob.init(a.ldb, a.N - ld.n0);
+        ld.oa.init(a.lda, a.M - ld.m0, gw);
+        ld.ob.init(a.ldb, a.N - ld.n0, gw);
         // stages past the last reload it into places whose fragments are not used
-        auto kt = [&](size_t t) { return (first + (t < T ? t : T - 1)) * kR_BK; };
+        auto kt = [&](size_t t) {
+            const size_t u = t < mine ? t : mine - 1;
+            if constexpr (G::KG > 1) return (first + (mine ? group + u * G::KG : 0)) * kR_BK;
+            else return (first + u) * kR_BK;
+        };
         ld.issue(kt(0), s0);
         ld.issue(kt(1), s1);
         ld.issue(kt(2), s2);
@@ -338,69 +408,109 @@ __global__ __launch_bounds__(G::NT) void k_linear_ring(RingArgs a) {
         side_frags<G::TN, KB>(s0 + G::TA, 0, bn, l32, lhi, f.b[0]);
         size_t t = 0;
         if constexpr (DT == CXM_DT_E4M3) {
-            Frags<G> g;
             side_frags<G::TM, true>(s0, 1, am, l32, lhi, f.a[1]);
             side_frags<G::TN, true>(s0 + G::TA, 1, bn, l32, lhi, f.b[1]);
-            for (; t + 4 <= T; t += 4) {
-                lin_step8<G>(ld, kt(t + 4), s0, s1, f, g, acc, am, bn, l32, lhi);
-                lin_step8<G>(ld, kt(t + 5), s1, s2, g, f, acc, am, bn, l32, lhi);
-                lin_step8<G>(ld, kt(t + 6), s2, s3, f, g, acc, am, bn, l32, lhi);
-                lin_step8<G>(ld, kt(t + 7), s3, s0, g, f, acc, am, bn, l32, lhi);
+            for (; t + 4 <= all; t += 4) {
+                lin_step8<G, false>(ld, kt(t + 4), s0, s1, f, acc, am, bn, l32, lhi, true);
+                lin_step8<G, false>(ld, kt(t + 5), s1, s2, f, acc, am, bn, l32, lhi, true);
+                lin_step8<G, false>(ld, kt(t + 6), s2, s3, f, acc, am, bn, l32, lhi, true);
+                lin_step8<G, false>(ld, kt(t + 7), s3, s0, f, acc, am, bn, l32, lhi, true);
             }
-            if (t < T) lin_step8<G>(ld, kt(t + 4), s0, s1, f, g, acc, am, bn, l32, lhi);
-            if (t + 1 < T) lin_step8<G>(ld, kt(t + 5), s1, s2, g, f, acc, am, bn, l32, lhi);
-            if (t + 2 < T) lin_step8<G>(ld, kt(t + 6), s2, s3, f, g, acc, am, bn, l32, lhi);
+            if (t < steps) lin_step8<G, true>(ld, kt(t + 4), s0, s1, f, acc, am, bn, l32, lhi, G::KG == 1 || t < mine);
+            if (t + 1 < steps) lin_step8<G, true>(ld, kt(t + 5), s1, s2, f, acc, am, bn, l32, lhi, G::KG == 1 || t + 1 < mine);
+            if (t + 2 < steps) lin_step8<G, true>(ld, kt(t + 6), s2, s3, f, acc, am, bn, l32, lhi, G::KG == 1 || t + 2 < mine);
+            if (G::KG > 1 && t + 3 < steps) lin_step8<G, true>(ld, kt(t + 7), s3, s0, f, acc, am, bn, l32, lhi, t + 3 < mine);
         } else {
-            for (; t + 4 <= T; t += 4) {
-                lin_step16<DT, G, KA, KB>(ld, kt(t + 4), s0, s1, f, acc, am, bn, l32, lhi);
-                lin_step16<DT, G, KA, KB>(ld, kt(t + 5), s1, s2, f, acc, am, bn, l32, lhi);
-                lin_step16<DT, G, KA, KB>(ld, kt(t + 6), s2, s3, f, acc, am, bn, l32, lhi);
-                lin_step16<DT, G, KA, KB>(ld, kt(t + 7), s3, s0, f, acc, am, bn, l32, lhi);
+            for (; t + 4 <= all; t += 4) {
+                lin_step16<DT, G, KA, KB, false>(ld, kt(t + 4), s0, s1, f, acc, am, bn, l32, lhi, true);
+                lin_step16<DT, G, KA, KB, false>(ld, kt(t + 5), s1, s2, f, acc, am, bn, l32, lhi, true);
+                lin_step16<DT, G, KA, KB, false>(ld, kt(t + 6), s2, s3, f, acc, am, bn, l32, lhi, true);
+                lin_step16<DT, G, KA, KB, false>(ld, kt(t + 7), s3, s0, f, acc, am, bn, l32, lhi, true);
             }
-            if (t < T) lin_step16<DT, G, KA, KB>(ld, kt(t + 4), s0, s1, f, acc, am, bn, l32, lhi);
-            if (t + 1 < T) lin_step16<DT, G, KA, KB>(ld, kt(t + 5), s1, s2, f, acc, am, bn, l32, lhi);
-            if (t + 2 < T) lin_step16<DT, G, KA, KB>(ld, kt(t + 6), s2, s3, f, acc, am, bn, l32, lhi);
+            if (t < steps) lin_step16<DT, G, KA, KB, true>(ld, kt(t + 4), s0, s1, f, acc, am, bn, l32, lhi, G::KG == 1 || t < mine);
+            if (t + 1 < steps)
+                lin_step16<DT, G, KA, KB, true>(ld, kt(t + 5), s1, s2, f, acc, am, bn, l32, lhi, G::KG == 1 || t + 1 < mine);
+            if (t + 2 < steps)
+                lin_step16<DT, G, KA, KB, true>(ld, kt(t + 6), s2, s3, f, acc, am, bn, l32, lhi, G::KG == 1 || t + 2 < mine);
+            if (G::KG > 1 && t + 3 < steps)
+                lin_step16<DT, G, KA, KB, true>(ld, kt(t + 7), s3, s0, f, acc, am, bn, l32, lhi, t + 3 < mine);
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load into LDS is left
-
-    if (a.splits > 1) {
-        const unsigned ws = xcd_remap16(blockIdx.x, gridDim.x);
-        const unsigned ti = ws / a.splits, sp = ws - ti * a.splits;
-        float *base = a.part + static_cast<size_t>(ti) * a.splits * (G::TM * G::TN) + threadIdx.x;
-        float *my = base + static_cast<size_t>(sp) * (G::TM * G::TN);
+    __syncthreads();  // every wave's fragment reads are done: the rings become scratch
+    auto scratch = [&](int i) { return reinterpret_cast<float *>(i == 0 ? r0 : i == 1 ? r1 : i == 2 ? r2 : r3); };
+    if constexpr (G::KG > 1) {
+        // a group's sums of the row blocks that another one finishes, by the
+        // sender's rank among the others
+        auto slot = [&](int i, int sender, int owner) {
+            const int rank = sender < owner ? sender : sender - 1;
+            return scratch(rank) + (gw * G::MB + i) * (G::NB * 16 * kWave) + lane;
+        };
 #pragma unroll
-        for (int i = 0; i < G::MB; ++i)
+        for (int i = 0; i < G::MB; ++i) {
+            const int owner = i / G::OWN;
+            if (owner == group) continue;
+            float *p = slot(i, group, owner);
 #pragma unroll
             for (int j = 0; j < G::NB; ++j)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) st_dev(my + ((i * G::NB + j) * 16 + r) * G::NT, acc[i][j][r]);
+                for (int r = 0; r < 16; ++r) p[(j * 16 + r) * kWave] = acc[i][j][r];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < G::MB; ++i) {
+            constexpr int O = G::OWN;
+            const int owner = i / O;
+            if (owner != group) continue;
+#pragma unroll
+            for (int j = 0; j < G::NB; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float v = 0.0f;
+#pragma unroll
+                    for (int s = 0; s < G::KG; ++s) {
+                        const float u = s == i / O ? acc[i][j][r] : slot(i, s, i / O)[(j * 16 + r) * kWave];
+                        v = s == 0 ? u : v + u;
+                    }
+                    acc[i][j][r] = v;
+                }
+        }
+        __syncthreads();
+    }
+    if (a.splits > 1) {
+        const unsigned ws = xcd_remap16(blockIdx.x, gridDim.x);
+        const unsigned ti = ws / a.splits, sp = ws - ti * a.splits;
+        float *base = a.part + static_cast<size_t>(ti) * a.splits * (G::TM * G::TN) + gw * kWave + lane;
+        float *my = base + static_cast<size_t>(sp) * (G::TM * G::TN);
+#pragma unroll
+        for (int i = 0; i < G::MB; ++i) {
+            if (i / G::OWN != group) continue;
+#pragma unroll
+            for (int j = 0; j < G::NB; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) st_dev(my + ((i * G::NB + j) * 16 + r) * (G::GW * kWave), acc[i][j][r]);
+        }
         if (!last_block_ticket(ctr(a.counters, ti), a.splits, &flag)) return;
 #pragma unroll
-        for (int i = 0; i < G::MB; ++i)
+        for (int i = 0; i < G::MB; ++i) {
+            if (i / G::OWN != group) continue;
 #pragma unroll
             for (int j = 0; j < G::NB; ++j)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-        for (unsigned q = 0; q < a.splits; ++q) {
-            const float *p = base + static_cast<size_t>(q) * (G::TM * G::TN);
-#pragma unroll
-            for (int i = 0; i < G::MB; ++i)
+            for (unsigned q = 0; q < a.splits; ++q) {
+                const float *p = base + static_cast<size_t>(q) * (G::TM * G::TN);
 #pragma unroll
                 for (int j = 0; j < G::NB; ++j)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) acc[i][j][r] += ld_dev(p + ((i * G::NB + j) * 16 + r) * G::NT);
+                    for (int r = 0; r < 16; ++r) acc[i][j][r] += ld_dev(p + ((i * G::NB + j) * 16 + r) * (G::GW * kWave));
+            }
         }
     }
-    __syncthreads();  // every wave's fragment reads are done: the stages become the epilogue's
     // the tile origin again, from the workgroup index, so that it need not live across the K loop
     group_tile(xcd_remap16(blockIdx.x, gridDim.x) / a.splits, a.tiles_m, a.tiles_n, a.gm, &tm, &tn);
-    constexpr int SH = G::WAVES / 4;  // waves sharing a stage's array
-    static_assert(32 * (G::HN + 8) * 4 <= G::STAGE * 2 / SH, "a wave's 32 rows fit its part of a stage");
-    const int st = wave / SH;
-    uint16_t *mine = (st == 0 ? s0 : st == 1 ? s1 : st == 2 ? s2 : s3) + wave % SH * (G::STAGE / SH);
-    lin_epilogue<OT, G>(a.e, acc, reinterpret_cast<float *>(mine), static_cast<size_t>(tm) * G::TM + am,
-                        static_cast<size_t>(tn) * G::TN + bn, a.M, a.N, l32, lhi);
+    lin_epilogue<OT, G>(a.e, acc, scratch(wave / G::PER) + wave % G::PER * G::EPI, static_cast<size_t>(tm) * G::TM + am,
+                        static_cast<size_t>(tn) * G::TN + bn, a.M, a.N, l32, lhi, group);
 }
 
 template <int DT, int OT, class G>
@@ -411,16 +521,19 @@ int ring_layout(const RingArgs &a, unsigned wgs, bool ta, bool tb, hipStream_t s
     } else {
         if (!ta && !tb) hipLaunchKernelGGL((k_linear_ring<DT, OT, G, true, false>), grid, block, 0, s, a);
         else if (!ta) hipLaunchKernelGGL((k_linear_ring<DT, OT, G, true, true>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((k_linear_ring<DT, OT, G, false, false>), grid, block, 0, s, a);
+        else if constexpr (G::TM >= 64) hipLaunchKernelGGL((k_linear_ring<DT, OT, G, false, false>), grid, block, 0, s, a);
+        else return CXM_E_INVALID;  // (no plan: a stage's rows of 32 columns are too short for the chunk keys)
     }
     return launch_status();
 }
 
 template <int DT, int OT>
 int ring_tile(const RingArgs &a, unsigned wgs, int tm, bool ta, bool tb, hipStream_t s) {
-    if (tm == 256) return ring_layout<DT, OT, Geo<256, 256, 2, 4>>(a, wgs, ta, tb, s);
-    if (tm == 128) return ring_layout<DT, OT, Geo<128, 128, 2, 4>>(a, wgs, ta, tb, s);
-    return ring_layout<DT, OT, Geo<64, 64, 2, 2>>(a, wgs, ta, tb, s);
+    if (tm == 256) return ring_layout<DT, OT, Geo<256, 256, 2, 4, 1>>(a, wgs, ta, tb, s);
+    if (tm == 128) return ring_layout<DT, OT, Geo<128, 128, 2, 4, 1>>(a, wgs, ta, tb, s);
+    if (tm == 64) return ring_layout<DT, OT, Geo<64, 64, 2, 2, 1>>(a, wgs, ta, tb, s);
+    if (tm == 32) return ring_layout<DT, OT, Geo<32, 64, 1, 2, 4>>(a, wgs, ta, tb, s);
+    return CXM_E_INVALID;
 }
 
 }  // namespace

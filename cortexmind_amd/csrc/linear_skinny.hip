@@ -1,18 +1,17 @@
-// Layer products of few rows (M up to 64: new tokens), bound by the one read
-// of the weight.
-//
-// The weight goes straight from memory to the matrix cores' registers as the
-// MFMA's row operand (16 outputs n per 16x16 step) and the rows of x are its
-// columns, 16 at a time; the waves of a workgroup take K in turns, several
-// steps of 128-bit loads in flight, and meet in LDS in wave order; K is
-// split over workgroups too until the chip is full, the last workgroup of a
-// tile adding the splits in their order.
-//  * weight [N, K]: a lane reads 32 bytes of one row per step of 128 bytes
-//    along K: two 16x16x32 16-bit steps, or one 16x16x128 e4m3 step;
-//  * weight [K, N]: a lane reads 8 columns of 8 rows (16 bytes each), and
-//    32 byte permutes turn them into the operands of 8 tiles of 16 columns.
-// Rows past the end re-read the last one, a ragged row's last columns are
-// read from its end (chunk.hpp); what is not the tile's is not stored.
+// Layer products of one to a few rows with the weight stored [N, K], bound by
+// the one read of the weight.
+//  * one row (two of 16 bits): a wave reads whole rows of the weight, 1 KiB per
+//    load, and multiplies on the vector units (1x4096x8192 bf16 14.9 us; the
+//    form below 16.6, the ring 17.0);
+//  * up to 16 rows by a weight of up to 8 MiB: the weight goes straight from
+//    memory to the matrix cores' registers as the MFMA's row operand (16
+//    outputs n per 16x16 step) and the rows of x are its columns; the waves of
+//    a workgroup share K and meet in LDS in wave order; K is split over
+//    workgroups too, the last one of a tile adding the splits in their order
+//    (16x1024x4096 bf16 5.5 us, the ring 5.8; larger weights are the ring's:
+//    16x4096x4096 12.3 and 10.1, as every lane's row of x is read with each step).
+// Rows past the end re-read the last one; what is not the tile's is not
+// stored.  Non-temporal loads of the weight were slower (15.7 against 14.9 us).
 #include "gemm16.hpp"
 #include "linear.hpp"
 #include "linear_act.hpp"
@@ -29,7 +28,7 @@ constexpr int kSW = 8;  // waves per workgroup
 struct SkinnyArgs {
     const uint8_t *x, *w;
     unsigned M, N;
-    size_t kb;       // bytes of K (weight [N, K]) or K (weight [K, N])
+    size_t kb;       // bytes of a row of K
     unsigned tiles, splits;
     unsigned per;    // steps per split
     float *part;
@@ -116,52 +115,33 @@ __device__ __forceinline__ void skinny_join(const SkinnyArgs &a, unsigned tile, 
     }
 }
 
-// Weight [N, K], k along its rows: 16 NR columns n per workgroup.  The two
-// 16-byte loads of a step take the halves of its 128 bytes, so that the four
-// lanes of a row read 64 contiguous bytes.
-template <int DT, int OT, int MT, int NR>
+// 16 columns n per workgroup, a step of 128 bytes along K.  The two 16-byte
+// loads of a step take its halves, so that the four lanes of a row read 64
+// contiguous bytes.
+template <int DT, int OT>
 __global__ __launch_bounds__(kSW *kWave) void k_linear_rows(SkinnyArgs a) {
-    constexpr int D = MT == 4 ? 2 : 4;  // steps in flight
-    constexpr int NC = 16 * NR, E = MT * 16 * NC;
+    constexpr int D = 4;  // steps in flight
+    constexpr int E = 256;
     __shared__ float sums[kSW * E];
     __shared__ int flag;
     const unsigned tile = blockIdx.x / a.splits, split = blockIdx.x - tile * a.splits;
-    const unsigned n0 = tile * NC;
+    const unsigned n0 = tile * 16;
     const int lane = threadIdx.x & (kWave - 1), r16 = lane & 15, q = lane >> 4;
     const unsigned w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const uint8_t *wp[NR], *xp[MT];
-#pragma unroll
-    for (int j = 0; j < NR; ++j) {
-        const unsigned n = n0 + 16 * j + r16 < a.N ? n0 + 16 * j + r16 : a.N - 1;
-        wp[j] = a.w + static_cast<size_t>(n) * a.kb + 16 * q;
-    }
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const unsigned m = 16 * i + r16 < a.M ? 16 * i + r16 : a.M - 1;
-        xp[i] = a.x + static_cast<size_t>(m) * a.kb + 16 * q;
-    }
-    f32x4v acc[MT][NR];
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NR; ++j) acc[i][j] = f32x4v{0.f, 0.f, 0.f, 0.f};
-    auto mul = [&](const u32x4 (&u)[NR][2], const u32x4 (&v)[MT][2]) {
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < NR; ++j) {
-                if constexpr (DT == CXM_DT_E4M3) {
-                    acc[i][j] = mfma_16x16_8(u[j][0], u[j][1], v[i][0], v[i][1], acc[i][j]);
-                } else {
-                    acc[i][j] = mfma_16x16<DT>(u[j][0], v[i][0], acc[i][j]);
-                    acc[i][j] = mfma_16x16<DT>(u[j][1], v[i][1], acc[i][j]);
-                }
-            }
+    const uint8_t *wp = a.w + static_cast<size_t>(n0 + r16 < a.N ? n0 + r16 : a.N - 1) * a.kb + 16 * q;
+    const uint8_t *xp = a.x + static_cast<size_t>(static_cast<unsigned>(r16) < a.M ? r16 : a.M - 1) * a.kb + 16 * q;
+    f32x4v acc = {0.f, 0.f, 0.f, 0.f};
+    auto mul = [&](const u32x4 (&u)[2], const u32x4 (&v)[2]) {
+        if constexpr (DT == CXM_DT_E4M3) {
+            acc = mfma_16x16_8(u[0], u[1], v[0], v[1], acc);
+        } else {
+            acc = mfma_16x16<DT>(u[0], v[0], acc);
+            acc = mfma_16x16<DT>(u[1], v[1], acc);
+        }
     };
-    // whole steps of 128 bytes: wave w's share of this split's [s0, s1), one
-    // after the other from a place that moves with the tile: rows a power of
-    // two apart, read by every workgroup at the same k, meet in few of the
-    // memory channels
+    // wave w's share of this split's whole steps [s0, s1), one after the other
+    // from a place that moves with the tile: rows a power of two apart, read by
+    // every workgroup at the same k, meet in few of the memory channels
     const unsigned whole = static_cast<unsigned>(a.kb / 128);
     const unsigned s0 = split * a.per, s1 = s0 + a.per < whole ? s0 + a.per : whole;
     const unsigned all = s1 > s0 ? s1 - s0 : 0, each = (all + kSW - 1) / kSW;
@@ -171,18 +151,13 @@ __global__ __launch_bounds__(kSW *kWave) void k_linear_rows(SkinnyArgs a) {
         const unsigned u = (t < T ? t : T - 1) + turn;
         return static_cast<size_t>(s0 + w * each + (u < T ? u : u - T)) * 128;
     };
-    u32x4 fw[D][NR][2], fx[D][MT][2];
+    u32x4 fw[D][2], fx[D][2];
     auto load = [&](int d, unsigned t) {
         const size_t o = at(t);
 #pragma unroll
-        for (int j = 0; j < NR; ++j) {
-            fw[d][j][0] = ld16(wp[j] + o);
-            fw[d][j][1] = ld16(wp[j] + o + 64);
-        }
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            fx[d][i][0] = ld16(xp[i] + o);
-            fx[d][i][1] = ld16(xp[i] + o + 64);
+        for (int h = 0; h < 2; ++h) {
+            fw[d][h] = ld16(wp + o + 64 * h);
+            fx[d][h] = ld16(xp + o + 64 * h);
         }
     };
     if (T > 0) {
@@ -204,173 +179,142 @@ __global__ __launch_bounds__(kSW *kWave) void k_linear_rows(SkinnyArgs a) {
     const int rest = static_cast<int>(a.kb % 128);
     if (rest != 0 && split == a.splits - 1 && w == kSW - 1) {  // the last wave's share is the shortest
         const size_t o = static_cast<size_t>(whole) * 128;
-        u32x4 u[NR][2], v[MT][2];
+        u32x4 u[2], v[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int j = 0; j < NR; ++j) u[j][h] = ld16_part(wp[j] + o + 64 * h, rest - 16 * q - 64 * h);
-#pragma unroll
-            for (int i = 0; i < MT; ++i) v[i][h] = ld16_part(xp[i] + o + 64 * h, rest - 16 * q - 64 * h);
+            u[h] = ld16_part(wp + o + 64 * h, rest - 16 * q - 64 * h);
+            v[h] = ld16_part(xp + o + 64 * h, rest - 16 * q - 64 * h);
         }
         mul(u, v);
     }
     // accumulator register r of lane l: n = 4 (l / 16) + r, m = l % 16
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NR; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) sums[w * E + (16 * i + r16) * NC + 16 * j + 4 * q + r] = acc[i][j][r];
+    for (int r = 0; r < 4; ++r) sums[w * E + r16 * 16 + 4 * q + r] = acc[r];
     __syncthreads();
     skinny_join<E>(a, tile, split, sums, &flag, [&](int p, float v) {
-        const unsigned m = p / NC, c = n0 + p % NC;
+        const unsigned m = p / 16, c = n0 + p % 16;
         if (m < a.M && c < a.N) skinny_store<OT>(a.e, v, m, c, a.N);
     });
 }
 
-// Weight [K, N]: 128 columns per workgroup, N >= 8.
-template <int DT, int OT, int MT>
-__global__ __launch_bounds__(kSW *kWave) void k_linear_cols(SkinnyArgs a) {
-    constexpr int D = MT == 1 ? 2 : 1;
-    constexpr int E = 16 * 128;  // one 16-row tile of x at a time
-    __shared__ float sums[kSW * E / 2];
-    __shared__ int flag;
-    const unsigned tile = blockIdx.x / a.splits, split = blockIdx.x - tile * a.splits;
-    const int lane = threadIdx.x & (kWave - 1), r16 = lane & 15, q = lane >> 4;
-    const unsigned w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const Span sp = span_of<8>(tile * 16 + r16, a.N);
-    const uint16_t *W = reinterpret_cast<const uint16_t *>(a.w) + sp.off;
-    const uint16_t *X = reinterpret_cast<const uint16_t *>(a.x);
-    const size_t K = a.kb;
-    const uint16_t *xp[MT];
+// One or two rows: a wave takes kDotRows rows of the weight whole.
+constexpr int kDotRows = 2, kDotDepth = 4;
+// (two rows of e4m3 take the matrix cores: 8192x8192 20.3 us here, 17.7 there)
+inline bool dot_takes(size_t M, size_t kb, int dtype) {
+    return kb >= 16 && (M == 1 || (M == 2 && dtype != CXM_DT_E4M3));
+}
+
+template <int DT>
+struct DotElems {
+    static constexpr int kVec = DT == CXM_DT_E4M3 ? 16 : 8;
+    __device__ static void get(u32x4 r, float (&v)[kVec]) {
+        if constexpr (DT == CXM_DT_E4M3) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i) xp[i] = X + static_cast<size_t>(16 * i + r16 < a.M ? 16 * i + r16 : a.M - 1) * K + 8 * q;
-    f32x4v acc[MT][8];
+            for (int i = 0; i < 4; ++i) unpack_e4m3(r[i], v + 4 * i);
+        } else {
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int c = 0; c < 8; ++c) acc[i][c] = f32x4v{0.f, 0.f, 0.f, 0.f};
-    auto mul = [&](const u32x4 (&f)[8], const u32x4 (&x)[MT]) {
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            u32x4 v;
-#pragma unroll
-            for (int p = 0; p < 4; ++p)
-                v[p] = __builtin_amdgcn_perm(f[2 * p + 1][c / 2], f[2 * p][c / 2], (c & 1) ? 0x07060302u : 0x05040100u);
-#pragma unroll
-            for (int i = 0; i < MT; ++i) acc[i][c] = mfma_16x16<DT>(v, x[i], acc[i][c]);
+            for (int i = 0; i < 8; ++i) v[i] = H<DT>::load(static_cast<uint16_t>(r[i / 2] >> (16 * (i & 1))));
         }
+    }
+};
+
+template <int DT, int OT, int M>
+__global__ __launch_bounds__(kBlock) void k_linear_dot(SkinnyArgs a) {
+    constexpr int VE = DotElems<DT>::kVec, RW = kDotRows, D = kDotDepth;
+    const unsigned lane = threadIdx.x % kWave;
+    const unsigned n0 = (blockIdx.x * (kBlock / kWave) + threadIdx.x / kWave) * RW;
+    if (n0 >= a.N) return;  // whole waves
+    const uint8_t *wp[RW];
+#pragma unroll
+    for (int j = 0; j < RW; ++j) wp[j] = a.w + static_cast<size_t>(n0 + j < a.N ? n0 + j : a.N - 1) * a.kb;
+    const unsigned T = static_cast<unsigned>((a.kb + 1023) / 1024), bytes = static_cast<unsigned>(a.kb);
+    float acc[RW][M];
+#pragma unroll
+    for (int j = 0; j < RW; ++j)
+#pragma unroll
+        for (int i = 0; i < M; ++i) acc[j][i] = 0.0f;
+    u32x4 fw[D][RW], fx[D][M];
+    // piece t of a row: 16 bytes per lane, those past its end moved back to it
+    auto off = [&](unsigned t) {
+        const unsigned o = t * 1024 + lane * 16;
+        return o < bytes - 16 ? o : bytes - 16;
     };
-    const unsigned whole = static_cast<unsigned>(K / 32);
-    const unsigned s0 = split * a.per, s1 = s0 + a.per < whole ? s0 + a.per : whole;
-    const unsigned T = s1 > s0 + w ? (s1 - s0 - w + kSW - 1) / kSW : 0;
-    u32x4 fw[D][8], fx[D][MT];
     auto load = [&](int d, unsigned t) {
-        const size_t k = static_cast<size_t>(s0 + w + (t < T ? t : T - 1) * kSW) * 32;
+        const unsigned o = off(t < T ? t : T - 1);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const u32x4e v = *reinterpret_cast<const u32x4e *>(W + (k + 8 * q + e) * a.N);
-            fw[d][e] = u32x4{v.x, v.y, v.z, v.w};
-        }
+        for (int j = 0; j < RW; ++j) fw[d][j] = ld16(wp[j] + o);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            const u32x4e v = *reinterpret_cast<const u32x4e *>(xp[i] + k);
-            fx[d][i] = u32x4{v.x, v.y, v.z, v.w};
+        for (int i = 0; i < M; ++i) fx[d][i] = ld16(a.x + static_cast<size_t>(i) * a.kb + o);
+    };
+    auto mul = [&](int d, unsigned t) {
+        float w[RW][VE];
+#pragma unroll
+        for (int j = 0; j < RW; ++j) DotElems<DT>::get(fw[d][j], w[j]);
+        const bool last = t == T - 1;  // the only one with elements of another lane's
+        const int dup = static_cast<int>(t * 1024 + lane * 16 - off(t)) / (16 / VE);
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            float x[VE];
+            DotElems<DT>::get(fx[d][i], x);
+            if (last) {
+#pragma unroll
+                for (int e = 0; e < VE; ++e) {
+                    x[e] = e >= dup ? x[e] : 0.0f;
+#pragma unroll
+                    for (int j = 0; j < RW; ++j) w[j][e] = e >= dup ? w[j][e] : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < RW; ++j)
+#pragma unroll
+                for (int e = 0; e < VE; ++e) acc[j][i] = fmaf(w[j][e], x[e], acc[j][i]);
         }
     };
-    if (T > 0) {
 #pragma unroll
-        for (int d = 0; d < D; ++d) load(d, d);
-        unsigned t = 0;
-        for (; t + D <= T; t += D) {
+    for (int d = 0; d < D; ++d) load(d, d);
+    for (unsigned t = 0; t < T; t += D) {
 #pragma unroll
-            for (int d = 0; d < D; ++d) {
-                mul(fw[d], fx[d]);
-                load(d, t + d + D);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+        for (int d = 0; d < D; ++d) {
+            if (t + d < T) mul(d, t + d);
+            load(d, t + d + D);
+            __builtin_amdgcn_sched_barrier(0);
         }
-#pragma unroll
-        for (int d = 0; d < D; ++d)
-            if (t + d < T) mul(fw[d], fx[d]);
     }
-    const unsigned rest = static_cast<unsigned>(K % 32);
-    if (rest != 0 && split == a.splits - 1 && w == whole % kSW) {
-        const size_t k = static_cast<size_t>(whole) * 32;
-        u32x4 f[8], x[MT];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const unsigned kk = 8 * q + e;
-            const u32x4e v = *reinterpret_cast<const u32x4e *>(W + (k + (kk < rest ? kk : rest - 1)) * a.N);
-            f[e] = kk < rest ? u32x4{v.x, v.y, v.z, v.w} : u32x4{0u, 0u, 0u, 0u};
+    for (int j = 0; j < RW; ++j)
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            const float v = group_reduce<SumOp, kWave>(acc[j][i]);
+            if (lane == static_cast<unsigned>(j * M + i) && n0 + j < a.N) skinny_store<OT>(a.e, v, i, n0 + j, a.N);
         }
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-            x[i] = ld16_part(reinterpret_cast<const uint8_t *>(xp[i] + k), 2 * (static_cast<int>(rest) - 8 * q));
-        mul(f, x);
-    }
-    // Tile c's accumulator register r of lane l: column chunk 4 (l / 16) + r,
-    // element c of it, row l % 16.  Eight rows of 128 columns at a time.
-    constexpr int EH = E / 2;
-#pragma unroll
-    for (int h = 0; h < 2 * MT; ++h) {
-        if (h > 0) __syncthreads();
-        if (r16 / 8 == (h & 1)) {
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) sums[w * EH + (r16 % 8) * 128 + 8 * (4 * q + r) + c] = acc[h / 2][c][r];
-        }
-        __syncthreads();
-        SkinnyArgs b = a;
-        b.part = a.part ? a.part + static_cast<size_t>(h) * a.tiles * a.splits * EH : nullptr;
-        b.counters = a.counters ? ctr(a.counters, static_cast<size_t>(h) * a.tiles) : nullptr;
-        if (8u * h < a.M)
-            skinny_join<EH>(b, tile, split, sums, &flag, [&](int p, float v) {
-                const unsigned m = 8 * h + p / 128, chunk = tile * 16 + (p % 128) / 8, e = p % 8;
-                const Span s = span_of<8>(chunk, a.N);
-                if (m < a.M && e >= s.dup && s.dup < 8) skinny_store<OT>(a.e, v, m, s.off + e, a.N);
-            });
-    }
 }
 
 template <int DT, int OT>
-int skinny_launch(const SkinnyArgs &a, bool tb, int nr, hipStream_t s) {
-    const dim3 grid(a.tiles * a.splits), block(kSW * kWave);
-    if (tb) {
-        if (a.M <= 16 && nr == 1) hipLaunchKernelGGL((k_linear_rows<DT, OT, 1, 1>), grid, block, 0, s, a);
-        else if (a.M <= 16) hipLaunchKernelGGL((k_linear_rows<DT, OT, 1, 2>), grid, block, 0, s, a);
-        else if (a.M <= 32) hipLaunchKernelGGL((k_linear_rows<DT, OT, 2, 2>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((k_linear_rows<DT, OT, 4, 1>), grid, block, 0, s, a);
-    } else if constexpr (DT != CXM_DT_E4M3) {
-        if (a.M <= 16) hipLaunchKernelGGL((k_linear_cols<DT, OT, 1>), grid, block, 0, s, a);
-        else if (a.M <= 32) hipLaunchKernelGGL((k_linear_cols<DT, OT, 2>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((k_linear_cols<DT, OT, 4>), grid, block, 0, s, a);
+int skinny_launch(const SkinnyArgs &a, hipStream_t s) {
+    if (dot_takes(a.M, a.kb, DT)) {
+        constexpr unsigned R = kBlock / kWave * kDotRows;
+        const dim3 grid((a.N + R - 1) / R), block(kBlock);
+        if (a.M == 1) hipLaunchKernelGGL((k_linear_dot<DT, OT, 1>), grid, block, 0, s, a);
+        else if constexpr (DT != CXM_DT_E4M3) hipLaunchKernelGGL((k_linear_dot<DT, OT, 2>), grid, block, 0, s, a);
+        return launch_status();
     }
+    hipLaunchKernelGGL((k_linear_rows<DT, OT>), dim3(a.tiles * a.splits), dim3(kSW * kWave), 0, s, a);
     return launch_status();
-}
-
-// Tiles of 16 outputs per workgroup, weight [N, K].
-int rows_tiles(size_t M, size_t N) {
-    if (M > 32) return 1;
-    if (M > 16) return 2;
-    (void)N;
-    return 1;
 }
 
 }  // namespace
 
-// CXM_OK with plan->kernel = 0, or kDeclined.
-int linear_skinny_plan(const LinProduct &p, LinPlan *l) {
-    constexpr size_t kMax = size_t(1) << 28;
-    const size_t kb = p.tb ? p.K * dtype_bytes(p.dtype) : p.K;
-    if (p.M > 64 || p.ta || (!p.tb && p.N < 8) || kb >= (size_t(1) << 31) || p.N >= kMax) return kDeclined;
+// Whether these kernels take the product; fills in the plan (kernel 0).
+bool linear_skinny_plan(const LinProduct &p, LinPlan *l) {
+    const size_t kb = p.K * dtype_bytes(p.dtype);
+    if (p.ta || !p.tb || p.M > 16 || kb >= (size_t(1) << 31) || p.N >= (size_t(1) << 28)) return false;
+    const bool dot = dot_takes(p.M, kb, p.dtype);
+    if (!dot && kb * p.N > (size_t(8) << 20)) return false;
     *l = LinPlan{};
-    l->kernel = 0;
-    const size_t width = p.tb ? 16 * rows_tiles(p.M, p.N) : 128, step = p.tb ? 128 : 32;
-    l->tiles = (p.N + width - 1) / width;
-    const size_t whole = kb / step, target = 2 * device_cus();
-    l->splits = 1;
+    l->splits = l->per = 1;
+    l->tiles = (p.N + 15) / 16;
+    if (dot) return true;
+    const size_t whole = kb / 128, target = 2 * device_cus();
     if (l->tiles < target) {
         l->splits = target / l->tiles;
         const size_t most = whole / (2 * kSW);  // two steps per wave at least
@@ -379,13 +323,8 @@ int linear_skinny_plan(const LinProduct &p, LinPlan *l) {
     }
     l->per = whole ? (whole + l->splits - 1) / l->splits : 1;
     if (whole) l->splits = (whole + l->per - 1) / l->per;
-    if (l->tiles * l->splits > 0x7fffffu) return kDeclined;
-    const size_t mt = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
-    if (l->splits > 1)
-        l->bytes_part = (l->tiles * l->splits * mt * 16 * width * sizeof(float) + 255) / 256 * 256;
-    l->tiles_n = l->tiles;  // one ticket per tile (and per 8 rows, weight [K, N])
-    if (!p.tb) l->tiles *= 2 * mt;
-    return CXM_OK;
+    if (l->splits > 1) l->bytes_part = (l->tiles * l->splits * 256 * sizeof(float) + 255) / 256 * 256;
+    return true;
 }
 
 int linear_skinny_run(const LinProduct &p, const LinPlan &l, float *part, unsigned *counters, hipStream_t s) {
@@ -393,20 +332,19 @@ int linear_skinny_run(const LinProduct &p, const LinPlan &l, float *part, unsign
                        static_cast<const uint8_t *>(p.b),
                        static_cast<unsigned>(p.M),
                        static_cast<unsigned>(p.N),
-                       p.tb ? p.K * dtype_bytes(p.dtype) : p.K,
-                       static_cast<unsigned>(l.tiles_n),
+                       p.K * dtype_bytes(p.dtype),
+                       static_cast<unsigned>(l.tiles),
                        static_cast<unsigned>(l.splits),
                        static_cast<unsigned>(l.per),
                        part,
                        counters,
                        p.e};
-    const int nr = rows_tiles(p.M, p.N);
     if (p.dtype == CXM_DT_E4M3) {
-        if (p.out == CXM_DT_BF16) return skinny_launch<CXM_DT_E4M3, CXM_DT_BF16>(a, true, nr, s);
-        return skinny_launch<CXM_DT_E4M3, CXM_DT_F16>(a, true, nr, s);
+        if (p.out == CXM_DT_BF16) return skinny_launch<CXM_DT_E4M3, CXM_DT_BF16>(a, s);
+        return skinny_launch<CXM_DT_E4M3, CXM_DT_F16>(a, s);
     }
-    if (p.dtype == CXM_DT_BF16) return skinny_launch<CXM_DT_BF16, CXM_DT_BF16>(a, p.tb, nr, s);
-    return skinny_launch<CXM_DT_F16, CXM_DT_F16>(a, p.tb, nr, s);
+    if (p.dtype == CXM_DT_BF16) return skinny_launch<CXM_DT_BF16, CXM_DT_BF16>(a, s);
+    return skinny_launch<CXM_DT_F16, CXM_DT_F16>(a, s);
 }
 
 }  // namespace cxm

@@ -280,15 +280,14 @@ __device__ __forceinline__ void lin_epilogue(const LinEpi &e, const Acc<G> &acc,
     float bias[8], cs[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) bias[i] = 0.0f, cs[i] = 1.0f;
+    // columns past the end: the last one's values, whose results are not stored
     if (e.bias) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < own) bias[i] = H<OT>::load(static_cast<const uint16_t *>(e.bias)[col + i]);
+        for (int i = 0; i < 8; ++i) bias[i] = H<OT>::load(static_cast<const uint16_t *>(e.bias)[col + i < N ? col + i : N - 1]);
     }
     if (e.cs) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < own) cs[i] = e.cs[col + i];
+        for (int i = 0; i < 8; ++i) cs[i] = e.cs[col + i < N ? col + i : N - 1];
     }
 #pragma unroll
     for (int i = 0; i < G::MB; ++i) {
@@ -317,10 +316,9 @@ __device__ __forceinline__ void lin_epilogue(const LinEpi &e, const Acc<G> &acc,
                 if (own == 8) {
                     c.load(res + o);
                 } else {
-                    uint16_t t[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                    uint16_t t[8];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        if (k < own) t[k] = res[o + k];
+                    for (int k = 0; k < 8; ++k) t[k] = res[o + (k < own ? k : own - 1)];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) c.r[k] = t[2 * k] | static_cast<unsigned>(t[2 * k + 1]) << 16;
                 }

@@ -273,12 +273,20 @@ __device__ __forceinline__ void lds_load16(const void *gsrc, const void *lds) {
 // `base` and `lds` (the LDS byte address, lds_addr) are the same in every
 // lane; read from the first lane, they are scalar values for the
 // instruction's SGPR operands whatever registers the compiler held them in.
+// The base goes through a scalar move: a vector-memory instruction may read an
+// SGPR that a vector instruction wrote (v_readfirstlane) only five wait states
+// later, which the compiler sees to for its own loads but not inside asm, and
+// M0 one wait state after its write.  Without the move the load could use what
+// the registers held before.
 __device__ __forceinline__ void lds_load16_at(const void *base, unsigned off, unsigned lds) {
     const size_t b = reinterpret_cast<size_t>(base);
     const unsigned lo = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(b));
     const unsigned hi = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(b >> 32));
     const void *sb = reinterpret_cast<const void *>((static_cast<size_t>(hi) << 32) | lo);
-    asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(sb), "{m0}"(__builtin_amdgcn_readfirstlane(lds))
+    const void *at;
+    asm volatile("s_mov_b64 %0, %2\n\tglobal_load_lds_dwordx4 %1, %0"
+                 : "=&s"(at)
+                 : "v"(off), "s"(sb), "{m0}"(__builtin_amdgcn_readfirstlane(lds))
                  : "memory");
 }
 // LDS byte address of a __shared__ location, as a wave-uniform value.

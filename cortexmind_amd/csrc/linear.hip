@@ -18,9 +18,9 @@ inline size_t up(size_t v, size_t m) { return (v + m - 1) / m * m; }
 // ------------------------------------------------ operands for the ring
 //
 // The ring's direct-to-LDS loads take 16-byte aligned pieces and whole stages
-// of 64 bytes of k.  An operand that has other row lengths (or another base)
-// is copied once, its rows extended by zeros; one read and one write of it,
-// against the product's many.
+// of 64 bytes of k.  Where that fails and the staged form is the slower
+// (linear_plan), an operand is copied once, its rows extended by zeros; one
+// read and one write of it, against the product's many.
 typedef unsigned u32x4b1 __attribute__((ext_vector_type(4), aligned(1)));
 
 struct PadSide {
@@ -35,7 +35,7 @@ struct PadSide {
 // load stands in a branch, where the compiler would wait for it (2500x1003 and
 // 1003x1499 8.3 us so).  A row's last piece is read as its last 16 bytes and
 // shifted down; rows shorter than 16 bytes go byte by byte.
-constexpr int kPadRows = 16;
+constexpr int kPadRows = 8;
 __global__ __launch_bounds__(kBlock) void k_pad(PadSide a, PadSide b) {
     constexpr int R = kPadRows / (kBlock / kWave);
     const bool first = blockIdx.x < a.wgs;
@@ -279,8 +279,6 @@ int linear_plan(const LinProduct &p, LinPlan *l) {
     l->lda = p.ta ? up(p.M, 8) : kpad;
     l->ldb = p.tb ? kpad : up(p.N, 8);
     if (l->lda >= (size_t(1) << 23) || l->ldb >= (size_t(1) << 23)) return CXM_E_TOO_LARGE;
-    if (l->copy_a) l->bytes_a = up((p.ta ? kpad : p.M) * l->lda * unit, 256);
-    if (l->copy_b) l->bytes_b = up((p.tb ? p.N : kpad) * l->ldb * unit, 256);
     const size_t cus = device_cus();
     auto tiles = [&](size_t tm, size_t tn) { return ((p.M + tm - 1) / tm) * ((p.N + tn - 1) / tn); };
     // The tile, by what these cost at K = 1024 (us; CUs of 256):
@@ -309,6 +307,23 @@ int linear_plan(const LinProduct &p, LinPlan *l) {
     }
     l->per = (l->stages + l->splits - 1) / l->splits;
     l->splits = (l->stages + l->per - 1) / l->per;
+    // Operands that the direct loads cannot take go through registers as they
+    // are, or are copied first.  A copy costs about 6 us and its bytes at 3
+    // TB/s, a stage through registers 0.15 us more on tiles of 64 (301x4001x301
+    // 14.8 us / copied 18.8, 100x4001x4001 22.9 / 28.6, but 701x8001x1201 85 /
+    // 52) and, its waves reading each weight once, nothing on 32x64 (20x4001x4001
+    // 16.1 / 26.9, e4m3 20x8001x8001 17.9 / 37.6); larger tiles gain nothing
+    // (128: 2500x1003x1499 22.5 / 22.3; 256: 4001^3 204 / 146).
+    const size_t copy_a = (p.ta ? kpad : p.M) * l->lda * unit, copy_b = (p.tb ? p.N : kpad) * l->ldb * unit;
+    if ((l->copy_a || l->copy_b) && tm <= 64 && (p.ta ? p.M : p.K) * es >= 16 && (p.tb ? p.K : p.N) * es >= 16) {
+        const double rounds = static_cast<double>((l->tiles * l->splits + cus - 1) / cus);
+        const double staged = few ? 0.0 : 0.15 * static_cast<double>(l->per) * rounds;
+        const double copied = 6.0 + (static_cast<double>(l->copy_a ? copy_a : 0) + static_cast<double>(l->copy_b ? copy_b : 0)) / 3e6;
+        l->staged = staged < copied;
+        if (l->staged) l->copy_a = l->copy_b = false;
+    }
+    if (l->copy_a) l->bytes_a = up(copy_a, 256);
+    if (l->copy_b) l->bytes_b = up(copy_b, 256);
     if (l->splits > 1) l->bytes_part = up(l->tiles * l->splits * tm * tn * sizeof(float), 256);
     return CXM_OK;
 }

@@ -29,7 +29,7 @@ struct LinProduct {
 
 struct LinPlan {
     int kernel;       // 0 skinny, else the rows of the ring's tile
-    bool copy_a, copy_b;
+    bool copy_a, copy_b, staged;
     size_t lda, ldb;  // of what the ring reads, in its 16-bit units
     size_t stages;    // of 32 units along K
     size_t splits, per;

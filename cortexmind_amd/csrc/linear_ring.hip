@@ -27,6 +27,8 @@
 // 2^3 and loses 2^2; the 16-byte forms of the instruction do the same): 1e-5 of
 // the sum of magnitudes at K = 64 and 2e-6 at K = 1024, far below the
 // half step of the 16-bit result (4.9e-4 and 3.9e-3) and of the operands (6e-2).
+#include <type_traits>
+
 #include "gemm16_ring.hpp"
 #include "linear.hpp"
 #include "linear_act.hpp"
@@ -38,8 +40,8 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 struct RingArgs {
     const uint16_t *A, *B;
-    size_t lda, ldb;  // units
-    size_t M, N;
+    size_t lda, ldb;  // of a stored row: units, staged bytes
+    size_t M, N, K;
     unsigned tiles_m, tiles_n, splits, stages, per, gm;
     float *part;
     unsigned *counters;
@@ -149,6 +151,125 @@ struct RingLoads {
     }
 };
 
+// The same stages filled through registers, for operands whose rows the
+// direct loads cannot take (no multiple of 16 bytes, another base, or a K
+// that ends inside a stage): unaligned 128-bit loads, D stages before their
+// LDS writes.  What lies past K is zero; a piece across a row's end is read as
+// the row's last 16 bytes and shifted down (rows of 16 bytes at least).
+__device__ __forceinline__ u32x4 shift_down(u32x4 v, unsigned bytes) {
+    const unsigned b = bytes * 8;
+    const uint64_t x = static_cast<uint64_t>(v.y) << 32 | v.x, y = static_cast<uint64_t>(v.w) << 32 | v.z;
+    const uint64_t lo = b == 0 ? x : b < 64 ? x >> b | y << (64 - b) : b < 128 ? y >> (b - 64) : 0;
+    const uint64_t hi = b < 64 ? y >> b : 0;
+    return u32x4{static_cast<unsigned>(lo), static_cast<unsigned>(lo >> 32), static_cast<unsigned>(hi),
+                 static_cast<unsigned>(hi >> 32)};
+}
+typedef unsigned u32x4p __attribute__((ext_vector_type(4), aligned(1)));
+
+template <int T, int ISSUES, bool KC>
+struct SideStage {
+    const char *x;   // KC: the tile's first row; else the operand
+    size_t ld;       // bytes of a row
+    size_t end;      // KC: the same; else rows of k
+    unsigned o[ISSUES], row0, c, sh, to;
+    __device__ __forceinline__ void init(const void *X, size_t row_bytes, size_t k_rows, size_t r0, size_t left,
+                                         unsigned w) {
+        constexpr unsigned PARTS = T / (16 * ISSUES);
+        w %= PARTS;
+        const unsigned lane = threadIdx.x & (kWave - 1);
+        to = w * (ISSUES * kWave * 16) + lane * 16;
+        ld = row_bytes;
+        if constexpr (KC) {
+            x = static_cast<const char *>(X) + r0 * ld;
+            end = row_bytes;
+            row0 = w * ISSUES * 16 + (lane >> 2);
+            c = 16 * ((lane & 3) ^ rkey(static_cast<int>(row0)));  // 16 rows on, the key is the same
+            sh = 0;
+#pragma unroll
+            for (int s = 0; s < ISSUES; ++s) {
+                const size_t r = row0 + 16 * s;
+                o[s] = static_cast<unsigned>((r < left ? r : left - 1) * ld);
+            }
+        } else {
+            constexpr unsigned CPR = T / 8, RPI = kWave / CPR;
+            x = static_cast<const char *>(X);
+            end = k_rows;
+            row0 = w * ISSUES * RPI + lane / CPR;
+            sh = 0;
+            c = 0;
+#pragma unroll
+            for (int s = 0; s < ISSUES; ++s) {
+                // the chunk of a row differs with its key; its place in the row as well
+                const unsigned r = row0 + RPI * s;
+                const size_t at = r0 * 2 + 16 * ((lane % CPR) ^ nkey<T>(static_cast<int>(r)));
+                const size_t in = at < ld - 16 ? at : ld - 16;
+                o[s] = static_cast<unsigned>(in);
+                const unsigned d = at - in < 16 ? static_cast<unsigned>(at - in) : 16u;
+                sh |= d << (8 * s);  // up to four issues
+            }
+        }
+    }
+    __device__ __forceinline__ void load(size_t tile, u32x4 (&v)[ISSUES]) const {
+        if constexpr (KC) {
+            const size_t at = tile * 64 + c, in = at < end - 16 ? at : end - 16;
+#pragma unroll
+            for (int s = 0; s < ISSUES; ++s) {
+                const u32x4p t = *reinterpret_cast<const u32x4p *>(x + o[s] + in);
+                v[s] = u32x4{t.x, t.y, t.z, t.w};
+            }
+        } else {
+            constexpr unsigned RPI = kWave / (T / 8);
+#pragma unroll
+            for (int s = 0; s < ISSUES; ++s) {
+                const size_t k = tile * 32 + row0 + RPI * s;
+                const u32x4p t = *reinterpret_cast<const u32x4p *>(x + (k < end ? k : end - 1) * ld + o[s]);
+                v[s] = u32x4{t.x, t.y, t.z, t.w};
+            }
+        }
+    }
+    __device__ __forceinline__ void store(size_t tile, const u32x4 (&v)[ISSUES], uint16_t *stage) const {
+        char *p = reinterpret_cast<char *>(stage) + to;
+        if constexpr (KC) {
+            const size_t at = tile * 64 + c;
+            const bool cut = tile * 64 + 64 > end;  // the same in every lane
+            const unsigned d = at + 16 <= end ? 0u : at - (end - 16) < 16 ? static_cast<unsigned>(at - (end - 16)) : 16u;
+#pragma unroll
+            for (int s = 0; s < ISSUES; ++s)
+                *reinterpret_cast<u32x4 *>(p + s * kWave * 16) = cut ? shift_down(v[s], d) : v[s];
+        } else {
+            constexpr unsigned RPI = kWave / (T / 8);
+            const bool cut = tile * 32 + 32 > end;
+#pragma unroll
+            for (int s = 0; s < ISSUES; ++s) {
+                u32x4 u = v[s];
+                if (__builtin_expect(__any(sh != 0), 0)) u = shift_down(u, (sh >> (8 * s)) & 0xffu);
+                if (cut && tile * 32 + row0 + RPI * s >= end) u = u32x4{0u, 0u, 0u, 0u};
+                *reinterpret_cast<u32x4 *>(p + s * kWave * 16) = u;
+            }
+        }
+    }
+};
+
+// Both sides; D register sets (D divides the four steps of a turn).
+template <class G, bool KA, bool KB>
+struct StageLoads {
+    static constexpr int D = 2;
+    SideStage<G::TM, G::IA, KA> a;
+    SideStage<G::TN, G::IB, KB> b;
+    u32x4 va[D][G::IA], vb[D][G::IB];
+    __device__ __forceinline__ void load(int d, size_t tile) {
+        a.load(tile, va[d]);
+        b.load(tile, vb[d]);
+    }
+    __device__ __forceinline__ void store(int d, size_t tile, uint16_t *stage) const {
+        a.store(tile, va[d], stage);
+        b.store(tile, vb[d], stage + G::TA);
+    }
+};
+
+// The barrier of a staged ring: this wave's LDS reads and writes are done.
+__device__ __forceinline__ void stage_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 __device__ __forceinline__ f32x16 mfma8(u32x4 a0, u32x4 a1, u32x4 b0, u32x4 b1, f32x16 c) {
     const i32x8 a = {static_cast<int>(a0.x), static_cast<int>(a0.y), static_cast<int>(a0.z), static_cast<int>(a0.w),
                      static_cast<int>(a1.x), static_cast<int>(a1.y), static_cast<int>(a1.z), static_cast<int>(a1.w)};
@@ -188,9 +309,14 @@ __device__ __forceinline__ void lin_mfma(const u32x4 (&a)[G::MB], const u32x4 (&
 // 16-bit step on stage cur, as ring_step; f[0] holds block 0 of cur.  LAST:
 // one of the steps after the unrolled loop, where a group may have no stage
 // left (`live` false) and only keeps the barrier.
-template <int DT, class G, bool KA, bool KB, bool LAST>
-__device__ __forceinline__ void lin_step16(const RingLoads<G, KA, KB> &ld, size_t kf, uint16_t *cur, const uint16_t *nxt,
-                                           Frags<G> &f, Acc<G> &acc, int am, int bn, int l32, int lhi, bool live) {
+// `feed` fills a stage ahead, after the barrier (STG: through registers).
+template <int DT, class G, bool KA, bool KB, bool STG, bool LAST, class F>
+__device__ __forceinline__ void lin_step16(const F &feed, uint16_t *cur, const uint16_t *nxt, Frags<G> &f, Acc<G> &acc,
+                                           int am, int bn, int l32, int lhi, bool live) {
+    auto barrier = [] {
+        if constexpr (STG) stage_barrier();
+        else ring_barrier<2 * G::PS>();
+    };
     if constexpr (LAST) {
         side_frags<G::TM, KA>(cur, 1, am, l32, lhi, f.a[1]);
         side_frags<G::TN, KB>(cur + G::TA, 1, bn, l32, lhi, f.b[1]);
@@ -198,10 +324,10 @@ __device__ __forceinline__ void lin_step16(const RingLoads<G, KA, KB> &ld, size_
             lin_mfma<DT, G>(f.a[0], f.b[0], acc);
             lin_mfma<DT, G>(f.a[1], f.b[1], acc);
         }
-        ring_barrier<2 * G::PS>();
+        barrier();
         side_frags<G::TM, KA>(nxt, 0, am, l32, lhi, f.a[0]);
         side_frags<G::TN, KB>(nxt + G::TA, 0, bn, l32, lhi, f.b[0]);
-        ld.issue(kf, cur);
+        feed();
         return;
     }
     constexpr int NM = G::MB * G::NB, ND = G::MB * (KA ? 1 : 2) + G::NB * (KB ? 1 : 2);
@@ -209,23 +335,24 @@ __device__ __forceinline__ void lin_step16(const RingLoads<G, KA, KB> &ld, size_
     side_frags<G::TN, KB>(cur + G::TA, 1, bn, l32, lhi, f.b[1]);
     lin_mfma<DT, G>(f.a[0], f.b[0], acc);
     lin_interleave<NM, ND>();
-    ring_barrier<2 * G::PS>();
+    barrier();
     side_frags<G::TM, KA>(nxt, 0, am, l32, lhi, f.a[0]);
     side_frags<G::TN, KB>(nxt + G::TA, 0, bn, l32, lhi, f.b[0]);
-    ld.issue(kf, cur);
+    feed();
     lin_mfma<DT, G>(f.a[1], f.b[1], acc);
-    lin_interleave<NM, ND>();
-    __builtin_amdgcn_sched_group_barrier(0x020, G::PS, 0);
+    if constexpr (!STG) {
+        lin_interleave<NM, ND>();
+        __builtin_amdgcn_sched_group_barrier(0x020, G::PS, 0);
+    }
 }
 
 // e4m3 step: f holds all of cur's stage and is refilled from nxt as its parts
 // have had their last product, the columns before the last ones before the
 // barrier: one set of fragments, where a second one spilled (the same 66 us at
 // 4096^3).
-template <class G, bool LAST>
-__device__ __forceinline__ void lin_step8(const RingLoads<G, true, true> &ld, size_t kf, uint16_t *cur,
-                                          const uint16_t *nxt, Frags<G> &f, Acc<G> &acc, int am, int bn, int l32, int lhi,
-                                          bool live) {
+template <class G, bool STG, bool LAST, class F>
+__device__ __forceinline__ void lin_step8(const F &feed, const uint16_t *nxt, Frags<G> &f, Acc<G> &acc, int am, int bn,
+                                          int l32, int lhi, bool live) {
     constexpr int J = G::NB - 1;
     const uint16_t *nb = nxt + G::TA;
     auto mul = [&](int i, int j) { acc[i][j] = mfma8(f.a[0][i], f.a[1][i], f.b[0][j], f.b[1][j], acc[i][j]); };
@@ -236,8 +363,9 @@ __device__ __forceinline__ void lin_step8(const RingLoads<G, true, true> &ld, si
             for (int i = 0; i < G::MB; ++i) mul(i, j);
         if constexpr (!LAST) __builtin_amdgcn_sched_group_barrier(0x008, J * G::MB, 0);
     }
-    ring_barrier<2 * G::PS>();
-    ld.issue(kf, cur);
+    if constexpr (STG) stage_barrier();
+    else ring_barrier<2 * G::PS>();
+    feed();
     auto read_b = [&](int j) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -253,7 +381,7 @@ __device__ __forceinline__ void lin_step8(const RingLoads<G, true, true> &ld, si
             f.a[kb][i] = *reinterpret_cast<const u32x4 *>(nxt + roff(am + i * 32 + l32, 2 * kb + lhi));
     }
     read_b(J);
-    if constexpr (!LAST) {
+    if constexpr (!LAST && !STG) {
         __builtin_amdgcn_sched_group_barrier(0x100, 2 * J, 0);
 #pragma unroll
         for (int i = 0; i < G::MB; ++i) {
@@ -351,7 +479,7 @@ __device__ __forceinline__ void lin_epilogue(const LinEpi &e, const Acc<G> &acc,
     }
 }
 
-template <int DT, int OT, class G, bool KA, bool KB>
+template <int DT, int OT, class G, bool KA, bool KB, bool STG>
 __global__ __launch_bounds__(G::NT) void k_linear_ring(RingArgs a) {
     // an array per stage of the rings, each holding the groups'
     constexpr int RS = G::KG * G::STAGE;
@@ -381,57 +509,82 @@ __global__ __launch_bounds__(G::NT) void k_linear_ring(RingArgs a) {
         // group g takes stages g, g + KG, ...; all make the same number of steps
         const size_t all = T / G::KG, steps = G::KG > 1 ? (T + G::KG - 1) / G::KG : T;
         const size_t mine = G::KG > 1 ? (T + G::KG - 1 - group) / G::KG : T;
-        RingLoads<G, KA, KB> ld;
-        ld.A = a.A;
-        ld.B = a.B;
-        ld.lda = a.lda;
-        ld.ldb = a.ldb;
-        ld.m0 = static_cast<size_t>(tm) * G::TM;
-        ld.n0 = static_cast<size_t>(tn) * G::TN;
-        ld.oa.init(a.lda, a.M - ld.m0, gw);
-        ld.ob.init(a.ldb, a.N - ld.n0, gw);
         // stages past the last reload it into places whose fragments are not used
-        auto kt = [&](size_t t) {
+        auto tile_of = [&](size_t t) {
             const size_t u = t < mine ? t : mine - 1;
-            if constexpr (G::KG > 1) return (first + (mine ? group + u * G::KG : 0)) * kR_BK;
-            else return (first + u) * kR_BK;
+            if constexpr (G::KG > 1) return first + (mine ? group + u * G::KG : 0);
+            else return first + u;
         };
-        ld.issue(kt(0), s0);
-        ld.issue(kt(1), s1);
-        ld.issue(kt(2), s2);
-        ld.issue(kt(3), s3);
-        ring_barrier<3 * G::PS>();
+        const size_t m0 = static_cast<size_t>(tm) * G::TM, n0 = static_cast<size_t>(tn) * G::TN;
         Frags<G> f;
-        side_frags<G::TM, KA>(s0, 0, am, l32, lhi, f.a[0]);
-        side_frags<G::TN, KB>(s0 + G::TA, 0, bn, l32, lhi, f.b[0]);
         size_t t = 0;
-        if constexpr (DT == CXM_DT_E4M3) {
-            side_frags<G::TM, true>(s0, 1, am, l32, lhi, f.a[1]);
-            side_frags<G::TN, true>(s0 + G::TA, 1, bn, l32, lhi, f.b[1]);
-            for (; t + 4 <= all; t += 4) {
-                lin_step8<G, false>(ld, kt(t + 4), s0, s1, f, acc, am, bn, l32, lhi, true);
-                lin_step8<G, false>(ld, kt(t + 5), s1, s2, f, acc, am, bn, l32, lhi, true);
-                lin_step8<G, false>(ld, kt(t + 6), s2, s3, f, acc, am, bn, l32, lhi, true);
-                lin_step8<G, false>(ld, kt(t + 7), s3, s0, f, acc, am, bn, l32, lhi, true);
+        auto loop = [&](const auto &feed) {
+            // feed(i, stage cur of step t + i, the stage two on)
+            side_frags<G::TM, KA>(s0, 0, am, l32, lhi, f.a[0]);
+            side_frags<G::TN, KB>(s0 + G::TA, 0, bn, l32, lhi, f.b[0]);
+            if constexpr (DT == CXM_DT_E4M3) {
+                side_frags<G::TM, true>(s0, 1, am, l32, lhi, f.a[1]);
+                side_frags<G::TN, true>(s0 + G::TA, 1, bn, l32, lhi, f.b[1]);
             }
-            if (t < steps) lin_step8<G, true>(ld, kt(t + 4), s0, s1, f, acc, am, bn, l32, lhi, G::KG == 1 || t < mine);
-            if (t + 1 < steps) lin_step8<G, true>(ld, kt(t + 5), s1, s2, f, acc, am, bn, l32, lhi, G::KG == 1 || t + 1 < mine);
-            if (t + 2 < steps) lin_step8<G, true>(ld, kt(t + 6), s2, s3, f, acc, am, bn, l32, lhi, G::KG == 1 || t + 2 < mine);
-            if (G::KG > 1 && t + 3 < steps) lin_step8<G, true>(ld, kt(t + 7), s3, s0, f, acc, am, bn, l32, lhi, t + 3 < mine);
+            auto step = [&](auto last, auto index, uint16_t *cur, uint16_t *nxt, uint16_t *two, bool live) {
+                constexpr bool L = decltype(last)::value;
+                auto fill = [&] { feed(index, cur, two); };
+                if constexpr (DT == CXM_DT_E4M3) lin_step8<G, STG, L>(fill, nxt, f, acc, am, bn, l32, lhi, live);
+                else lin_step16<DT, G, KA, KB, STG, L>(fill, cur, nxt, f, acc, am, bn, l32, lhi, live);
+            };
+            using No = std::false_type;
+            using Yes = std::true_type;
+            const std::integral_constant<int, 0> i0{};
+            const std::integral_constant<int, 1> i1{};
+            const std::integral_constant<int, 2> i2{};
+            const std::integral_constant<int, 3> i3{};
+            for (; t + 4 <= all; t += 4) {
+                step(No{}, i0, s0, s1, s2, true);
+                step(No{}, i1, s1, s2, s3, true);
+                step(No{}, i2, s2, s3, s0, true);
+                step(No{}, i3, s3, s0, s1, true);
+            }
+            if (t < steps) step(Yes{}, i0, s0, s1, s2, G::KG == 1 || t < mine);
+            if (t + 1 < steps) step(Yes{}, i1, s1, s2, s3, G::KG == 1 || t + 1 < mine);
+            if (t + 2 < steps) step(Yes{}, i2, s2, s3, s0, G::KG == 1 || t + 2 < mine);
+            if (G::KG > 1 && t + 3 < steps) step(Yes{}, i3, s3, s0, s1, t + 3 < mine);
+        };
+        if constexpr (STG) {
+            StageLoads<G, KA, KB> ld;
+            constexpr int D = StageLoads<G, KA, KB>::D;
+            ld.a.init(a.A, a.lda, a.K, m0, a.M - m0, gw);
+            ld.b.init(a.B, a.ldb, a.K, n0, a.N - n0, gw);
+            for (int i = 0; i < 2; ++i) {
+                ld.load(0, tile_of(i));
+                ld.store(0, tile_of(i), i ? s1 : s0);
+            }
+#pragma unroll
+            for (int d = 0; d < D; ++d) ld.load(d, tile_of(2 + d));
+            stage_barrier();
+            loop([&](auto index, uint16_t *, uint16_t *two) {
+                constexpr int d = decltype(index)::value % D;
+                const size_t at = t + decltype(index)::value;
+                ld.store(d, tile_of(at + 2), two);
+                ld.load(d, tile_of(at + 2 + D));
+            });
         } else {
-            for (; t + 4 <= all; t += 4) {
-                lin_step16<DT, G, KA, KB, false>(ld, kt(t + 4), s0, s1, f, acc, am, bn, l32, lhi, true);
-                lin_step16<DT, G, KA, KB, false>(ld, kt(t + 5), s1, s2, f, acc, am, bn, l32, lhi, true);
-                lin_step16<DT, G, KA, KB, false>(ld, kt(t + 6), s2, s3, f, acc, am, bn, l32, lhi, true);
-                lin_step16<DT, G, KA, KB, false>(ld, kt(t + 7), s3, s0, f, acc, am, bn, l32, lhi, true);
-            }
-            if (t < steps) lin_step16<DT, G, KA, KB, true>(ld, kt(t + 4), s0, s1, f, acc, am, bn, l32, lhi, G::KG == 1 || t < mine);
-            if (t + 1 < steps)
-                lin_step16<DT, G, KA, KB, true>(ld, kt(t + 5), s1, s2, f, acc, am, bn, l32, lhi, G::KG == 1 || t + 1 < mine);
-            if (t + 2 < steps)
-                lin_step16<DT, G, KA, KB, true>(ld, kt(t + 6), s2, s3, f, acc, am, bn, l32, lhi, G::KG == 1 || t + 2 < mine);
-            if (G::KG > 1 && t + 3 < steps)
-                lin_step16<DT, G, KA, KB, true>(ld, kt(t + 7), s3, s0, f, acc, am, bn, l32, lhi, t + 3 < mine);
+            RingLoads<G, KA, KB> ld;
+            ld.A = a.A;
+            ld.B = a.B;
+            ld.lda = a.lda;
+            ld.ldb = a.ldb;
+            ld.m0 = m0;
+            ld.n0 = n0;
+            ld.oa.init(a.lda, a.M - m0, gw);
+            ld.ob.init(a.ldb, a.N - n0, gw);
+            ld.issue(tile_of(0) * kR_BK, s0);
+            ld.issue(tile_of(1) * kR_BK, s1);
+            ld.issue(tile_of(2) * kR_BK, s2);
+            ld.issue(tile_of(3) * kR_BK, s3);
+            ring_barrier<3 * G::PS>();
+            loop([&](auto index, uint16_t *cur, uint16_t *) {
+                ld.issue(tile_of(t + 4 + decltype(index)::value) * kR_BK, cur);
+            });
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load into LDS is left
@@ -511,27 +664,40 @@ __global__ __launch_bounds__(G::NT) void k_linear_ring(RingArgs a) {
                         static_cast<size_t>(tn) * G::TN + bn, a.M, a.N, l32, lhi, group);
 }
 
-template <int DT, int OT, class G>
+template <int DT, int OT, class G, bool STG>
 int ring_layout(const RingArgs &a, unsigned wgs, bool ta, bool tb, hipStream_t s) {
     const dim3 grid(wgs), block(G::NT);
     if constexpr (DT == CXM_DT_E4M3) {
-        hipLaunchKernelGGL((k_linear_ring<DT, OT, G, true, true>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((k_linear_ring<DT, OT, G, true, true, STG>), grid, block, 0, s, a);
     } else {
-        if (!ta && !tb) hipLaunchKernelGGL((k_linear_ring<DT, OT, G, true, false>), grid, block, 0, s, a);
-        else if (!ta) hipLaunchKernelGGL((k_linear_ring<DT, OT, G, true, true>), grid, block, 0, s, a);
-        else if constexpr (G::TM >= 64) hipLaunchKernelGGL((k_linear_ring<DT, OT, G, false, false>), grid, block, 0, s, a);
+        if (!ta && !tb) hipLaunchKernelGGL((k_linear_ring<DT, OT, G, true, false, STG>), grid, block, 0, s, a);
+        else if (!ta) hipLaunchKernelGGL((k_linear_ring<DT, OT, G, true, true, STG>), grid, block, 0, s, a);
+        else if constexpr (G::TM >= 64)
+            hipLaunchKernelGGL((k_linear_ring<DT, OT, G, false, false, STG>), grid, block, 0, s, a);
         else return CXM_E_INVALID;  // (no plan: a stage's rows of 32 columns are too short for the chunk keys)
     }
     return launch_status();
 }
 
-template <int DT, int OT>
+template <int DT, int OT, bool STG>
 int ring_tile(const RingArgs &a, unsigned wgs, int tm, bool ta, bool tb, hipStream_t s) {
-    if (tm == 256) return ring_layout<DT, OT, Geo<256, 256, 2, 4, 1>>(a, wgs, ta, tb, s);
-    if (tm == 128) return ring_layout<DT, OT, Geo<128, 128, 2, 4, 1>>(a, wgs, ta, tb, s);
-    if (tm == 64) return ring_layout<DT, OT, Geo<64, 64, 2, 2, 1>>(a, wgs, ta, tb, s);
-    if (tm == 32) return ring_layout<DT, OT, Geo<32, 64, 1, 2, 4>>(a, wgs, ta, tb, s);
+    if constexpr (!STG) {  // (staged: linear_plan)
+        if (tm == 256) return ring_layout<DT, OT, Geo<256, 256, 2, 4, 1>, STG>(a, wgs, ta, tb, s);
+        if (tm == 128) return ring_layout<DT, OT, Geo<128, 128, 2, 4, 1>, STG>(a, wgs, ta, tb, s);
+    }
+    if (tm == 64) return ring_layout<DT, OT, Geo<64, 64, 2, 2, 1>, STG>(a, wgs, ta, tb, s);
+    if (tm == 32) return ring_layout<DT, OT, Geo<32, 64, 1, 2, 4>, STG>(a, wgs, ta, tb, s);
     return CXM_E_INVALID;
+}
+
+template <bool STG>
+int ring_dtype(const LinProduct &p, const RingArgs &a, unsigned n, int tm, hipStream_t s) {
+    if (p.dtype == CXM_DT_E4M3) {
+        if (p.out == CXM_DT_BF16) return ring_tile<CXM_DT_E4M3, CXM_DT_BF16, STG>(a, n, tm, false, true, s);
+        return ring_tile<CXM_DT_E4M3, CXM_DT_F16, STG>(a, n, tm, false, true, s);
+    }
+    if (p.dtype == CXM_DT_BF16) return ring_tile<CXM_DT_BF16, CXM_DT_BF16, STG>(a, n, tm, p.ta, p.tb, s);
+    return ring_tile<CXM_DT_F16, CXM_DT_F16, STG>(a, n, tm, p.ta, p.tb, s);
 }
 
 }  // namespace
@@ -539,17 +705,23 @@ int ring_tile(const RingArgs &a, unsigned wgs, int tm, bool ta, bool tb, hipStre
 int linear_ring_run(const LinProduct &p, const LinPlan &l, const void *A, const void *B, float *part,
                     unsigned *counters, hipStream_t s) {
     const size_t wgs = l.tiles * l.splits;
-    // what the kernel assumes: 16-byte aligned rows, whole stages, lane offsets of a tile within 32 bits
-    if (!aligned16(A) || !aligned16(B) || l.lda % 8 != 0 || l.ldb % 8 != 0 || l.lda >= (size_t(1) << 23) ||
-        l.ldb >= (size_t(1) << 23) || l.stages == 0 || l.stages > 0x7fffffffu || l.per * (l.splits - 1) >= l.stages ||
-        l.per * l.splits < l.stages || wgs > 0x7fffffffu || (p.ta && p.tb))
+    const size_t row_a = (p.ta ? p.M : p.K) * dtype_bytes(p.dtype), row_b = (p.tb ? p.K : p.N) * dtype_bytes(p.dtype);
+    if (l.stages == 0 || l.stages > 0x7fffffffu || l.per * (l.splits - 1) >= l.stages || l.per * l.splits < l.stages ||
+        wgs > 0x7fffffffu || (p.ta && p.tb))
+        return CXM_E_TOO_LARGE;
+    // what the kernels assume: direct loads, 16-byte aligned rows and whole stages;
+    // staged ones, rows of 16 bytes at least; both, a tile's lane offsets within 32 bits
+    if (l.staged ? row_a < 16 || row_b < 16 || row_a >= (size_t(1) << 24) || row_b >= (size_t(1) << 24)
+                 : !aligned16(A) || !aligned16(B) || l.lda % 8 != 0 || l.ldb % 8 != 0 || l.lda >= (size_t(1) << 23) ||
+                       l.ldb >= (size_t(1) << 23))
         return CXM_E_TOO_LARGE;
     const RingArgs a{static_cast<const uint16_t *>(A),
                      static_cast<const uint16_t *>(B),
-                     l.lda,
-                     l.ldb,
+                     l.staged ? row_a : l.lda,
+                     l.staged ? row_b : l.ldb,
                      p.M,
                      p.N,
+                     p.K,
                      static_cast<unsigned>(l.tiles_m),
                      static_cast<unsigned>(l.tiles_n),
                      static_cast<unsigned>(l.splits),
@@ -560,12 +732,7 @@ int linear_ring_run(const LinProduct &p, const LinPlan &l, const void *A, const 
                      counters,
                      p.e};
     const unsigned n = static_cast<unsigned>(wgs);
-    if (p.dtype == CXM_DT_E4M3) {
-        if (p.out == CXM_DT_BF16) return ring_tile<CXM_DT_E4M3, CXM_DT_BF16>(a, n, l.kernel, false, true, s);
-        return ring_tile<CXM_DT_E4M3, CXM_DT_F16>(a, n, l.kernel, false, true, s);
-    }
-    if (p.dtype == CXM_DT_BF16) return ring_tile<CXM_DT_BF16, CXM_DT_BF16>(a, n, l.kernel, p.ta, p.tb, s);
-    return ring_tile<CXM_DT_F16, CXM_DT_F16>(a, n, l.kernel, p.ta, p.tb, s);
+    return l.staged ? ring_dtype<true>(p, a, n, l.kernel, s) : ring_dtype<false>(p, a, n, l.kernel, s);
 }
 
 }  // namespace cxm

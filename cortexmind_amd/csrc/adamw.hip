@@ -329,7 +329,7 @@ int adam_create(cxm_adamw **out, const cxm_adamw_tensor_t *tensors, size_t count
         master = t.master != nullptr;
         if (master && p_dtype == CXM_DT_F32) return CXM_E_INVALID;
         const size_t blocks = (t.n + kBlock8 - 1) / kBlock8, pieces = (t.n + kPiece - 1) / kPiece;
-        if (owner.size() + pieces > 0x7fffffu * size_t(16)) return CXM_E_TOO_LARGE;
+        if (owner.size() + pieces > most_wgs(kBlock)) return CXM_E_TOO_LARGE;
         AdamTensor d{};
         d.p = t.p;
         d.g = t.g;

@@ -176,6 +176,10 @@ __device__ __forceinline__ Scale8 scale_e4m3(float amax) {
 
 // ---------------------------------------------------------- host
 
+// Workgroups of `threads` that one launch can have: fewer than 2^32 threads.
+constexpr size_t most_wgs(size_t threads) { return 0xffffffffu / threads; }
+
+
 // out[j] = sum of part[i][j] over i < n (rows `ld` floats apart), rounded to
 // `dtype`; the order is fixed (colsum.hip).
 int col_sum(const float *part, size_t n, size_t cols, size_t ld, void *out, int dtype, hipStream_t s);

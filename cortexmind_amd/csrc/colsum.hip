@@ -40,7 +40,7 @@ void launch(const float *part, unsigned n, unsigned cols, size_t ld, void *out, 
 }  // namespace
 
 int col_sum(const float *part, size_t n, size_t cols, size_t ld, void *out, int dtype, hipStream_t s) {
-    if (n > 0x7fffffffu || cols > 0x7fffffffu) return CXM_E_TOO_LARGE;
+    if (n > 0x7fffffffu || cols > 0x7fffffffu || (cols + kSumCols - 1) / kSumCols > most_wgs(kSumThreads)) return CXM_E_TOO_LARGE;
     const unsigned nn = static_cast<unsigned>(n), nc = static_cast<unsigned>(cols);
     if (dtype == CXM_DT_F32) launch<CXM_DT_F32>(part, nn, nc, ld, out, s);
     else if (dtype == CXM_DT_BF16) launch<CXM_DT_BF16>(part, nn, nc, ld, out, s);

@@ -85,7 +85,7 @@ __global__ __launch_bounds__(kBlock) void k_pad(PadSide a, PadSide b) {
 bool pad_side(PadSide *p, const void *x, void *y, size_t rows, size_t bytes, size_t out_rows, size_t out_bytes) {
     const size_t pieces = out_bytes / 16, tiles = (pieces + kWave - 1) / kWave;
     const size_t wgs = (out_rows + kPadRows - 1) / kPadRows * tiles;
-    if (wgs > 0x3fffffffu || pieces > 0x7fffffffu) return false;
+    if (wgs > most_wgs(kBlock) / 2 || pieces > 0x7fffffffu) return false;  // (two sides in a launch)
     *p = PadSide{static_cast<const uint8_t *>(x), static_cast<uint8_t *>(y), rows, bytes, out_rows,
                  static_cast<unsigned>(pieces), static_cast<unsigned>(tiles), static_cast<unsigned>(wgs)};
     return true;
@@ -138,11 +138,11 @@ int linear_f32(const float *x, const float *w, const float *bias, const float *r
     // without z, y holds x W + bias for a moment (so a residual in y itself is refused)
     const bool fused = !z && !res && (act == CXM_ACT_NONE || act == CXM_ACT_RELU);
     float *to = z ? z : y;
+    const size_t wgs = (m * n + 4 * kBlock - 1) / (4 * kBlock);
+    if (wgs > most_wgs(kBlock)) return CXM_E_TOO_LARGE;
     const Epilogue e{bias, nullptr, fused ? act : CXM_ACT_NONE, 0, 0.0f};
     const int rc = gemm_ex(x, w, to, m, k, n, 0, tw, e, st);
     if (rc || fused || (to == y && !res && act == CXM_ACT_NONE)) return rc;
-    const size_t wgs = (m * n + 4 * kBlock - 1) / (4 * kBlock);
-    if (wgs > 0x7fffffffu) return CXM_E_TOO_LARGE;
     hipLaunchKernelGGL(k_linear_f32, dim3(static_cast<unsigned>(wgs)), dim3(kBlock), 0, hs(st), to, res, y, m * n, act);
     return launch_status();
 }
@@ -307,6 +307,7 @@ int linear_plan(const LinProduct &p, LinPlan *l) {
     }
     l->per = (l->stages + l->splits - 1) / l->splits;
     l->splits = (l->stages + l->per - 1) / l->per;
+    if (l->tiles > most_wgs(1024) / l->splits) return CXM_E_TOO_LARGE;
     // Operands that the direct loads cannot take go through registers as they
     // are, or are copied first.  A copy costs about 6 us and its bytes at 3
     // TB/s, a stage through registers 0.15 us more on tiles of 64 (301x4001x301

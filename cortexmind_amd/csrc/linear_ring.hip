@@ -707,7 +707,7 @@ int linear_ring_run(const LinProduct &p, const LinPlan &l, const void *A, const 
     const size_t wgs = l.tiles * l.splits;
     const size_t row_a = (p.ta ? p.M : p.K) * dtype_bytes(p.dtype), row_b = (p.tb ? p.K : p.N) * dtype_bytes(p.dtype);
     if (l.stages == 0 || l.stages > 0x7fffffffu || l.per * (l.splits - 1) >= l.stages || l.per * l.splits < l.stages ||
-        wgs > 0x7fffffffu || (p.ta && p.tb))
+        wgs > most_wgs(1024) || (p.ta && p.tb))
         return CXM_E_TOO_LARGE;
     // what the kernels assume: direct loads, 16-byte aligned rows and whole stages;
     // staged ones, rows of 16 bytes at least; both, a tile's lane offsets within 32 bits

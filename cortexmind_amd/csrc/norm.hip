@@ -462,7 +462,7 @@ template <int DT, int VE, int G, int C, int NT>
 int fwd_launch(const RmsFwd &a, hipStream_t s) {
     constexpr int R = G <= kWave ? NT / G : 1;
     const size_t wgs = (a.rows + R - 1) / R;
-    if (wgs > 0x7fffffffu) return CXM_E_TOO_LARGE;
+    if (wgs > most_wgs(NT)) return CXM_E_TOO_LARGE;
     const dim3 grid(static_cast<unsigned>(wgs));
     if (whole_lines(a.x, a.cols, sizeof(typename Elem<DT>::S)) && whole_lines(a.res, a.cols, sizeof(typename Elem<DT>::S)))
         hipLaunchKernelGGL((k_rms_fwd<DT, VE, G, C, NT, true>), grid, dim3(NT), 0, s, a);
@@ -485,7 +485,7 @@ int fwd_dispatch(const RmsFwd &a, hipStream_t s) {
     if (chunks <= 1024) return few ? fwd_launch<DT, VE, 1024, 1, 1024>(a, s) : fwd_launch<DT, VE, 256, 4, 256>(a, s);
     if (chunks <= 2048) return fwd_launch<DT, VE, 1024, 2, 1024>(a, s);
     if (chunks <= 4096) return fwd_launch<DT, VE, 1024, 4, 1024>(a, s);
-    if (a.rows > 0x7fffffffu) return CXM_E_TOO_LARGE;
+    if (a.rows > most_wgs(1024)) return CXM_E_TOO_LARGE;
     hipLaunchKernelGGL((k_rms_fwd_long<DT, 1024>), dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, s, a);
     return launch_status();
 }
@@ -542,7 +542,7 @@ int bwd_dispatch(RmsBwd a, void *dw, cxm_stream_t st) {
     if (chunks <= 512) return bwd_launch<DT, VE, 256, 2, 256>(a, dw, st);
     if (chunks <= 1024) return bwd_launch<DT, VE, 512, 2, 512>(a, dw, st);
     if (chunks <= 2048) return bwd_launch<DT, VE, 1024, 2, 1024>(a, dw, st);
-    if (a.rows > 0x7fffffffu) return CXM_E_TOO_LARGE;
+    if (a.rows > most_wgs(1024)) return CXM_E_TOO_LARGE;
     const size_t tiles = (chunks + kBlock - 1) / kBlock;
     size_t parts = 4 * device_cus() / tiles;
     parts = parts < 1 ? 1 : parts > a.rows ? a.rows : parts;
@@ -559,7 +559,7 @@ int bwd_dispatch(RmsBwd a, void *dw, cxm_stream_t st) {
 
 // Row lengths stay below 2^31, so that an element's place in its row is 32 bits.
 bool row_shape_ok(size_t rows, size_t cols) {
-    return cols < (size_t(1) << 31) && rows <= (size_t(1) << 40) && rows * cols <= (size_t(1) << 46);
+    return cols < (size_t(1) << 31) && (rows == 0 || cols == 0 || rows <= (size_t(1) << 46) / cols);
 }
 
 }  // namespace
@@ -613,7 +613,7 @@ int cxm_rmsnorm_bwd_t(const void *h, const float *rstd, const void *w, const voi
     using cxm::overlap;
     using cxm::overlap_not_same;
     if (!cxm::is_float_dtype(dtype) || !dw || cols == 0) return CXM_E_INVALID;
-    if (!cxm::row_shape_ok(rows, cols)) return CXM_E_TOO_LARGE;
+    if (!cxm::row_shape_ok(rows, cols) || cols >= (size_t(1) << 26)) return CXM_E_TOO_LARGE;  // (col_sum's grid)
     const size_t e = cxm::dtype_bytes(dtype), n = rows * cols * e;
     cxm::RmsBwd a{h, w, dy, dh, rstd, dx, nullptr, rows, static_cast<unsigned>(cols), 0};
     if (rows == 0) return cxm::col_sum(nullptr, 0, cols, cols, dw, dtype, cxm::hs(s));  // an empty sum

@@ -10,9 +10,10 @@
 // backward(const Tensor&), ToString()) and adds flows for every operator on
 // the path -- MatMul, AddBias, Add, MulRow (Broadcast::row::mul), MulScalar
 // (ScalarOp::mul), ReLU / Sigmoid / Tanh, the fused AffineAct, Softmax and
-// LogSoftmax, Sum and Mean over an axis, SoftmaxCrossEntropy -- each
+// LogSoftmax, Sum and Mean over an axis, SoftmaxCrossEntropy, RmsNorm and
+// Linear (a dense layer with bias, activation and residual) -- each
 // running the library's kernels through the C ABI on hip::stream(), plus
-// backward(root[, seed]) and sgd().  Tensors are shared handles (TensorPtr)
+// backward(root[, seed]), sgd() and AdamW.  Tensors are shared handles (TensorPtr)
 // so that a flow can reach its inputs' gradients.
 //
 // Gradients accumulate: the first contribution to a tensor's gradient is
@@ -396,6 +397,91 @@ inline TensorPtr mean(const TensorPtr &x, std::size_t outer, std::size_t dim, st
     return reduce_axis(x, outer, dim, inner, 1);
 }
 
+// Y = X / rms(X) * w over the rows of X [rows, cols] (cxm_rmsnorm_fwd_t):
+// dX and dw from X and the saved 1 / rms (cxm_rmsnorm_bwd_t).
+struct RmsNormFlow : GradientFlow {
+    TensorPtr x, w;
+    Tensor rstd;
+    RmsNormFlow(TensorPtr x_, TensorPtr w_, Tensor rstd_)
+        : GradientFlow("RmsNorm"), x(std::move(x_)), w(std::move(w_)), rstd(std::move(rstd_)) {
+        inputs = {x, w};
+    }
+    void backward(const Tensor &dy) override {
+        Tensor tx, tw;
+        float *dx = grad_dst(x, tx), *dw = grad_dst(w, tw);
+        check(cxm_rmsnorm_bwd_t(x->data(), rstd.data(), w->data(), dy.data(), nullptr, dx, dw, rows_of(*x), cols_of(*x),
+                                CXM_DT_F32, stream()),
+              "RmsNormFlow");
+        grad_done(x, tx);
+        grad_done(w, tw);
+    }
+};
+inline TensorPtr rms_norm(const TensorPtr &x, const TensorPtr &w, float eps = 1e-5f) {
+    on_device({x.get(), w.get()}, "rms_norm");
+    if (w->len() != cols_of(*x)) check(CXM_E_INVALID, "rms_norm: one weight per column");
+    auto y = make_tensor(x->shape());
+    Tensor rstd = device_tensor({x->dim(0)});
+    check(cxm_rmsnorm_fwd_t(x->data(), nullptr, w->data(), eps, nullptr, y->data(), nullptr, nullptr, rstd.data(),
+                            rows_of(*x), cols_of(*x), CXM_DT_F32, stream()),
+          "rms_norm");
+    if (needs_grad(x) || needs_grad(w)) link(y, std::make_shared<RmsNormFlow>(x, w, std::move(rstd)));
+    return y;
+}
+
+// Y = act(X W + bias) + residual (cxm_linear_fwd_t), bias and residual
+// optional: the gradients of X, W and the bias from the saved X W + bias
+// (cxm_linear_bwd_t); the residual's is dY.
+struct LinearFlow : GradientFlow {
+    TensorPtr x, w, bias, res;
+    Tensor z;
+    int act;
+    LinearFlow(TensorPtr x_, TensorPtr w_, TensorPtr b_, TensorPtr r_, Tensor z_, int act_)
+        : GradientFlow("Linear"), x(std::move(x_)), w(std::move(w_)), bias(std::move(b_)), res(std::move(r_)),
+          z(std::move(z_)), act(act_) {
+        inputs = {x, w};
+        if (bias) inputs.push_back(bias);
+        if (res) inputs.push_back(res);
+    }
+    void backward(const Tensor &dy) override {
+        const std::size_t M = rows_of(*x), K = cols_of(*x), N = cols_of(*w);
+        Tensor tx, tw, tb, dz;
+        if (act != CXM_ACT_NONE) dz = device_tensor(dy.shape());
+        float *dx = needs_grad(x) ? grad_dst(x, tx) : nullptr;
+        // a tensor that is an input twice already has its first contribution when the second is made
+        float *dw = needs_grad(w) ? grad_dst(w, tw) : nullptr;
+        float *db = bias && needs_grad(bias) ? grad_dst(bias, tb) : nullptr;
+        check(cxm_linear_bwd_t(x->data(), w->data(), z.empty() ? nullptr : z.data(), dy.data(),
+                               dz.empty() ? nullptr : dz.data(), dx, dw, db, M, K, N, 0, act, CXM_DT_F32, stream()),
+              "LinearFlow");
+        grad_done(x, tx);
+        grad_done(w, tw);
+        if (db) grad_done(bias, tb);
+        if (res && needs_grad(res))
+            accumulate(res, [&](float *d) {
+                check(cxm_memcpy_d2d(d, dy.data(), dy.len() * sizeof(float), stream()), "LinearFlow: residual");
+            });
+    }
+};
+// act: CXM_ACT_NONE, RELU, SIGMOID, TANH, GELU or SILU.
+inline TensorPtr linear(const TensorPtr &x, const TensorPtr &w, const TensorPtr &bias = nullptr, int act = CXM_ACT_NONE,
+                        const TensorPtr &res = nullptr) {
+    on_device({x.get(), w.get()}, "linear");
+    if (bias) on_device({bias.get()}, "linear");
+    if (res) on_device({res.get()}, "linear");
+    const std::size_t M = rows_of(*x), K = cols_of(*x), N = cols_of(*w);
+    if (rows_of(*w) != K || (bias && bias->len() != N) || (res && res->len() != M * N))
+        check(CXM_E_INVALID, "linear: sizes do not match");
+    auto y = make_tensor({x->dim(0), w->dim(1)});
+    Tensor z;
+    if (act != CXM_ACT_NONE) z = device_tensor(y->shape());
+    check(cxm_linear_fwd_t(x->data(), w->data(), bias ? bias->data() : nullptr, res ? res->data() : nullptr,
+                           z.empty() ? nullptr : z.data(), y->data(), M, K, N, 0, act, CXM_DT_F32, stream()),
+          "linear");
+    if (needs_grad(x) || needs_grad(w) || (bias && needs_grad(bias)) || (res && needs_grad(res)))
+        link(y, std::make_shared<LinearFlow>(x, w, bias, res, std::move(z), act));
+    return y;
+}
+
 // labels: device int32 [rows].
 inline TensorPtr softmax_cross_entropy(const TensorPtr &logits, const std::int32_t *labels) {
     on_device({logits.get()}, "softmax_cross_entropy");
@@ -451,6 +537,73 @@ inline void sgd(const std::vector<TensorPtr> &params, float lr) {
         p->grad_ptr().reset();
     }
 }
+
+// AdamW over the parameters that have a gradient, in one launch
+// (cxm_adamw_step), after which the gradients are dropped, as by sgd().  Owns
+// the fp32 moments.  The list of pointers is kept on the device and made
+// again only when a parameter's or gradient's storage has moved.
+class AdamW {
+public:
+    explicit AdamW(std::vector<TensorPtr> params, float decay = 0.0f) : params_(std::move(params)) {
+        for (const auto &p : params_) {
+            on_device({p.get()}, "AdamW");
+            m_.push_back(zeros(p->shape()));
+            v_.push_back(zeros(p->shape()));
+            decay_.push_back(decay);
+        }
+    }
+    AdamW(const AdamW &) = delete;
+    AdamW &operator=(const AdamW &) = delete;
+    ~AdamW() { drop(); }
+    // Weight decay of parameter i alone.
+    void set_decay(std::size_t i, float decay) {
+        decay_.at(i) = decay;
+        drop();
+    }
+    void step(double lr, double beta1 = 0.9, double beta2 = 0.999, double eps = 1e-8) {
+        std::vector<cxm_adamw_tensor_t> list;
+        for (std::size_t i = 0; i < params_.size(); ++i) {
+            if (!params_[i]->has_grad()) continue;
+            on_device({params_[i].get(), &params_[i]->grad()}, "AdamW");
+            cxm_adamw_tensor_t t{};
+            t.p = params_[i]->data();
+            t.g = params_[i]->grad().data();
+            t.m = m_[i].data();
+            t.v = v_[i].data();
+            t.n = params_[i]->len();
+            t.decay = decay_[i];
+            list.push_back(t);
+        }
+        bool same = handle_ && list.size() == list_.size();
+        for (std::size_t i = 0; same && i < list.size(); ++i)
+            same = list[i].p == list_[i].p && list[i].g == list_[i].g && list[i].m == list_[i].m;
+        if (!same) {
+            drop();
+            check(cxm_adamw_create(&handle_, list.data(), list.size(), CXM_DT_F32, CXM_DT_F32, CXM_DT_F32), "AdamW");
+            list_ = std::move(list);
+        }
+        check(cxm_adamw_step(handle_, lr, beta1, beta2, eps, ++t_, nullptr, 0, stream()), "AdamW");
+        for (const auto &p : params_) p->grad_ptr().reset();
+    }
+
+private:
+    static Tensor zeros(const std::vector<std::int64_t> &shape) {
+        Tensor t = device_tensor(shape);
+        check(cxm_memset(t.data(), 0, t.len() * sizeof(float), stream()), "AdamW");
+        return t;
+    }
+    void drop() {
+        if (handle_) (void)cxm_adamw_destroy(handle_);
+        handle_ = nullptr;
+        list_.clear();
+    }
+    std::vector<TensorPtr> params_;
+    std::vector<Tensor> m_, v_;
+    std::vector<float> decay_;
+    std::vector<cxm_adamw_tensor_t> list_;
+    cxm_adamw *handle_ = nullptr;
+    std::size_t t_ = 0;
+};
 
 }  // namespace cortex::_fw::hip
 

@@ -454,8 +454,8 @@ int cxm_rmsnorm_fwd_t(const void *x, const void *res, const void *w, float eps, 
  * dx = rstd * (g - n * mean(g * n)) + dh, where dh (or NULL) is the gradient
  * that reaches h past the norm; dx is the gradient of x and of res.
  * dw[j] = sum over rows of dy * n, summed in fp32 in a fixed order.  dx may be
- * h, dy or dh itself.  rows == 0 gives dw = 0.  Needs scratch (see
- * CXM_E_CAPTURE). */
+ * h, dy or dh itself.  rows == 0 gives dw = 0.  cols < 2^26.  Needs scratch
+ * (see CXM_E_CAPTURE). */
 int cxm_rmsnorm_bwd_t(const void *h, const float *rstd, const void *w, const void *dy, const void *dh, void *dx,
                       void *dw, size_t rows, size_t cols, int dtype, cxm_stream_t s);
 /* The rows of x in 8 bits with a scale each, as above: for a weight [n, k]
@@ -481,7 +481,9 @@ int cxm_linear_fwd_t(const void *x, const void *w, const void *bias, const void 
  * which the products read), db = column sums of the unrounded dz, dx = dz w^T,
  * dw = x^T dz (stored as w).  The residual's gradient is dy.  dx, dw and db
  * may be NULL; with act NONE also z, and dz (the products then read dy).  dz
- * may be z or dy itself; no other overlap.  m, k, n > 0, m < 2^23. */
+ * may be z or dy itself; no other overlap.  m, k, n > 0, m < 2^23.  Needs
+ * scratch (in fp32 that of cxm_gemm_f32 too: captured without it, dz and db may
+ * have been recorded before the products are refused). */
 int cxm_linear_bwd_t(const void *x, const void *w, const void *z, const void *dy, void *dz, void *dx, void *dw, void *db,
                      size_t m, size_t k, size_t n, int trans_w, int act, int dtype, cxm_stream_t s);
 /* The same layer from 8-bit operands (E4M3): z[i, j] = x_scale[i] *
@@ -518,7 +520,7 @@ int cxm_linear_q8_fwd(const uint8_t *x, const float *x_scale, const uint8_t *w, 
  * not the tensors; they are on the device that was current then, where step
  * has to be called too (else CXM_E_INVALID).  Nothing that a step writes may
  * overlap anything else in the list (else CXM_E_INVALID); empty tensors are
- * skipped. */
+ * skipped.  The handle outlives every graph that captured a step of it. */
 typedef struct cxm_adamw_tensor_t {
     void *p;         /* parameters (p_dtype) */
     const void *g;   /* gradients (g_dtype: p_dtype or CXM_DT_F32) */

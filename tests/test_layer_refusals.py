@@ -35,6 +35,10 @@ def test_norm_sizes(lib):
     assert fwd(lib, rows=0, x=None) == OK
     assert fwd(lib, cols=1 << 31) == E_TOO_LARGE
     assert fwd(lib, rows=1 << 41) == E_TOO_LARGE
+    assert fwd(lib, rows=1 << 40, cols=1 << 30) == E_TOO_LARGE  # a product past 64 bits
+    # grids of 2^32 threads and more
+    assert fwd(lib, x=1 << 44, res=None, w=A[2], h=None, y=1 << 45, rstd=None, rows=1 << 32, cols=8) == E_TOO_LARGE
+    assert bwd(lib, h=1 << 44, dy=1 << 45, dh=None, dx=1 << 46, cols=1 << 26) == E_TOO_LARGE
 
 
 def bwd(lib, h=A[0], rstd=A[1], w=A[2], dy=A[3], dh=A[4], dx=A[5], dw=A[6], rows=4, cols=64, dt=DT_F16):
@@ -75,6 +79,10 @@ def test_linear_sizes(lib):
     assert lin(lib, m=0, x=None) == OK and lin(lib, n=0, y=None) == OK
     for kw in (dict(k=1 << 23), dict(n=1 << 23), dict(m=1 << 31)):
         assert lin(lib, **kw) == E_TOO_LARGE
+    # more tiles, and more elements of the fp32 epilogue, than a grid has
+    big = dict(x=1 << 44, w=1 << 45, bias=None, res=None, z=None, y=1 << 47, m=(1 << 31) - 1, k=64, n=(1 << 23) - 1)
+    for dt in (DT_BF16, DT_F32):
+        assert lin(lib, dt=dt, **big) == E_TOO_LARGE
 
 
 def q8(lib, x=A[0], xs=A[1], w=A[2], ws=A[3], bias=A[4], res=A[5], z=A[6], y=A[7], m=4, k=64, n=32, act=ACT_RELU,
@@ -142,6 +150,8 @@ def test_adamw_types(lib):
     assert lib.cxm_adamw_create(ctypes.byref(h), None, 1, DT_F32, DT_F32, DT_F32) == E_INVALID
     assert lib.cxm_adamw_create(None, t, 1, DT_F32, DT_F32, DT_F32) == E_INVALID
     assert lib.cxm_adamw_create(ctypes.byref(h), tensors(dict(master=A[6])), 1, DT_F32, DT_F32, DT_F32) == E_INVALID
+    far = dict(n=1 << 40, g=1 << 44, m=1 << 45, v=1 << 46, p=1 << 47)
+    assert lib.cxm_adamw_create(ctypes.byref(h), tensors(far), 1, DT_F32, DT_F32, DT_F32) == E_TOO_LARGE
     assert lib.cxm_adamw_create(ctypes.byref(h), tensors(dict(n=1 << 50)), 1, DT_F32, DT_F32, DT_F32) == E_TOO_LARGE
 
 

@@ -202,3 +202,29 @@ def test_capture_without_scratch_is_refused(hip):
         h.hipGraphExecDestroy(exe)
         h.hipGraphDestroy(graph)
         s.close()
+
+
+def test_two_streams_at_once(hip):
+    """The same work queued on two streams without waiting in between (split
+    products, column sums and their scratch among it) gives each its own result."""
+    a, b = Block(130, 512, 300, DT_BF16, 13), Block(130, 512, 300, DT_BF16, 14)
+    wa, wb = Block(130, 512, 300, DT_BF16, 13), Block(130, 512, 300, DT_BF16, 14)
+    s, u = Stream(), Stream()
+    for blk, st in ((a, s), (b, u)):  # each stream's scratch
+        Block(130, 512, 300, DT_BF16, 15).step(1, st)
+    s.sync()
+    u.sync()
+    for t in range(1, 6):
+        a.step(t, s)
+        b.step(t, u)
+    for t in range(1, 6):
+        wa.step(t)
+        wb.step(t)
+    for x in (s, u):
+        x.sync()
+    for got, want in ((a, wa), (b, wb)):
+        for k in NAMES:
+            assert np.array_equal(got.p[k].numpy(), want.p[k].numpy()), k
+            assert np.array_equal(got.grad[k].numpy(), want.grad[k].numpy()), k
+    s.close()
+    u.close()

@@ -151,7 +151,12 @@ int linear_f32(const float *x, const float *w, const float *bias, const float *r
 //
 // dz = dy act'(z) and the column sums of dz (unrounded, fp32): each of a
 // workgroup's waves takes rows of one tile of 64 chunks; the waves meet in
-// LDS, the workgroups' shares in k_col_sum, both in a fixed order.
+// LDS, the workgroups' shares in k_col_sum, both in a fixed order.  bf16
+// 4096x4096 with GELU: 19.6 us, 5.1 TB/s; its slope is 18 vector operations an
+// element, two of them at a quarter of the rate, about 13 us of the vector
+// units beside 14.6 us of memory, and the two overlap only across waves.  Two
+// and four rows in flight per wave (20.0, 21.9 us) and the next row loaded
+// ahead of the slope (20.5, 19.6 with half the workgroups) gain nothing.
 struct ActBwd {
     const void *z, *dy;
     void *dz;
@@ -165,7 +170,7 @@ template <int DT, int VE>
 __global__ __launch_bounds__(kBlock) void k_act_bwd(ActBwd a) {
     using S = typename Elem<DT>::S;
     constexpr bool FINE = DT == CXM_DT_F32;
-    constexpr int W = kBlock / kWave, U = 2;
+    constexpr int W = kBlock / kWave;
     __shared__ float lds[W][kWave * VE];
     const unsigned lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
     const unsigned c = blockIdx.x * kWave + lane;
@@ -173,35 +178,26 @@ __global__ __launch_bounds__(kBlock) void k_act_bwd(ActBwd a) {
     float acc[VE];
 #pragma unroll
     for (int e = 0; e < VE; ++e) acc[e] = 0.0f;
-    // U rows of loads in flight (one row at a time: 4096x4096 bf16 18.9 us)
     const size_t step = static_cast<size_t>(gridDim.y) * W;
-    for (size_t r0 = static_cast<size_t>(blockIdx.y) * W + w; r0 < a.rows; r0 += U * step) {
-        Chunk<DT, VE> cz[U], cd[U];
+    for (size_t r = static_cast<size_t>(blockIdx.y) * W + w; r < a.rows; r += step) {
+        const size_t o = r * a.cols;
+        Chunk<DT, VE> cz, cd;
+        float z[VE], d[VE];
+        cd.load_nt(static_cast<const S *>(a.dy) + o + s.off);
+        if (a.act != CXM_ACT_NONE) {
+            cz.load_nt(static_cast<const S *>(a.z) + o + s.off);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const size_t r = r0 + u * step, o = (r < a.rows ? r : r0) * a.cols;
-            cd[u].load_nt(static_cast<const S *>(a.dy) + o + s.off);
-            if (a.act != CXM_ACT_NONE) cz[u].load_nt(static_cast<const S *>(a.z) + o + s.off);
+            for (int e = 0; e < VE; ++e) z[e] = cz.get(e);
         }
+        act_slope<FINE, VE>(a.act, z, d);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const size_t r = r0 + u * step;
-            if (r >= a.rows) break;
-            float z[VE], d[VE];
-            if (a.act != CXM_ACT_NONE) {
-#pragma unroll
-                for (int e = 0; e < VE; ++e) z[e] = cz[u].get(e);
-            }
-            act_slope<FINE, VE>(a.act, z, d);
-#pragma unroll
-            for (int e = 0; e < VE; ++e) {
-                d[e] *= cd[u].get(e);
-                acc[e] += d[e];
-            }
-            if (a.dz) {
-                cd[u].set(d);
-                store_span<DT, VE>(static_cast<S *>(a.dz) + r * a.cols, s, cd[u]);
-            }
+        for (int e = 0; e < VE; ++e) {
+            d[e] *= cd.get(e);
+            acc[e] += d[e];
+        }
+        if (a.dz) {
+            cd.set(d);
+            store_span<DT, VE>(static_cast<S *>(a.dz) + o, s, cd);
         }
     }
     if (!a.part) return;

@@ -12,8 +12,8 @@ namespace {
 // (iteratively reweighted least squares toward minimax in the relative error)
 // over all a >= 0; Phi(a) = 1 - Phi(-a).  Relative error of t p(t): 7.5e-6
 // with degree 6 (FINE = false, for 16-bit results, whose half step is 4.9e-4),
-// 2.4e-7 with degree 9.  A third of erff's instructions, no branch, and
-// the negative tail keeps its digits where 1 + erf loses them.
+// 2.4e-7 with degree 9.  No branch, and the negative tail keeps its digits
+// where 1 + erf loses them.
 template <bool FINE>
 __device__ __forceinline__ float normal_cdf(float z, float *bell) {
     const float a = fabsf(z);

@@ -33,8 +33,6 @@ namespace {
 
 typedef unsigned u32x2a __attribute__((ext_vector_type(2)));
 
-typedef unsigned u32x2a __attribute__((ext_vector_type(2)));
-
 constexpr unsigned kBlock8 = 256;                   // values per scale: 64 lanes of 4
 constexpr unsigned kLane = 4, kUnits = 2;           // values of a thread: kUnits times kLane, a wave's lanes side by side
 constexpr unsigned kPiece = kBlock * kLane * kUnits;  // values per workgroup
@@ -76,7 +74,9 @@ __device__ __forceinline__ unsigned noise32(unsigned long long c, unsigned key) 
 // Byte SEL of `w` becomes v (|v| up to 448) as e4m3, its magnitude rounded to
 // the neighbour above with the probability of the distance to the one below:
 // v_cvt_sr_fp8_f32 adds the upper 20 bits of `rnd` below the 3 kept mantissa
-// bits and cuts the rest off (below 2^-6 below the even steps of 2^-9).
+// bits and cuts the rest off (below 2^-6 below the even steps of 2^-9).  Its
+// last 4 bits are zero, so a block's largest value, 448 but for an fp32
+// rounding of the scale or two, never carries past 448 into the NaN.
 template <int SEL>
 __device__ __forceinline__ unsigned round_e4m3(float v, unsigned rnd, unsigned w) {
     return static_cast<unsigned>(__builtin_amdgcn_cvt_sr_fp8_f32(v, static_cast<int>(rnd), static_cast<int>(w), SEL));

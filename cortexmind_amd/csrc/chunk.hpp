@@ -41,8 +41,8 @@ __device__ __forceinline__ unsigned pack2(float a, float b) {
     else return __builtin_bit_cast(unsigned, f16x2{static_cast<_Float16>(a), static_cast<_Float16>(b)});
 }
 
-// load_nt and store_nt set the non-temporal hint, for what is touched once.
 // VE consecutive elements in registers: kVec (one 128-bit access) or 1.
+// load_nt sets the non-temporal hint, for what is touched once.
 template <int DT, int VE>
 struct Chunk;
 template <int VE>
@@ -71,10 +71,6 @@ struct Chunk<CXM_DT_F32, VE> {
     }
     __device__ __forceinline__ void store(float *p) const {
         if constexpr (VE == 4) *reinterpret_cast<f32x4e *>(p) = f32x4e{r[0], r[1], r[2], r[3]};
-        else *p = r[0];
-    }
-    __device__ __forceinline__ void store_nt(float *p) const {
-        if constexpr (VE == 4) __builtin_nontemporal_store(f32x4e{r[0], r[1], r[2], r[3]}, reinterpret_cast<f32x4e *>(p));
         else *p = r[0];
     }
     __device__ __forceinline__ float raw(int e) const { return r[e]; }
@@ -110,10 +106,6 @@ struct Chunk {
     }
     __device__ __forceinline__ void store(uint16_t *p) const {
         if constexpr (VE == 8) *reinterpret_cast<u32x4e *>(p) = u32x4e{r[0], r[1], r[2], r[3]};
-        else *p = static_cast<uint16_t>(r[0]);
-    }
-    __device__ __forceinline__ void store_nt(uint16_t *p) const {
-        if constexpr (VE == 8) __builtin_nontemporal_store(u32x4e{r[0], r[1], r[2], r[3]}, reinterpret_cast<u32x4e *>(p));
         else *p = static_cast<uint16_t>(r[0]);
     }
 };
@@ -179,11 +171,9 @@ __device__ __forceinline__ Scale8 scale_e4m3(float amax) {
 // Workgroups of `threads` that one launch can have: fewer than 2^32 threads.
 constexpr size_t most_wgs(size_t threads) { return 0xffffffffu / threads; }
 
-
 // out[j] = sum of part[i][j] over i < n (rows `ld` floats apart), rounded to
 // `dtype`; the order is fixed (colsum.hip).
 int col_sum(const float *part, size_t n, size_t cols, size_t ld, void *out, int dtype, hipStream_t s);
-
 
 // Whether [a, a + an) and [b, b + bn) share a byte (null or empty: no).
 inline bool overlap(const void *a, size_t an, const void *b, size_t bn) {

@@ -151,7 +151,9 @@ int linear_f32(const float *x, const float *w, const float *bias, const float *r
 //
 // dz = dy act'(z) and the column sums of dz (unrounded, fp32): each of a
 // workgroup's waves takes rows of one tile of 64 chunks; the waves meet in
-// LDS, the workgroups' shares in k_col_sum, both in a fixed order.  bf16
+// LDS, the workgroups' shares in k_col_sum, both in a fixed order (for few rows
+// the last workgroup of a tile adding them costs what the launch does: 512x1024
+// 21.5 -> 23.8 us for the whole backward, 98x86 13.5 -> 12.3).  bf16
 // 4096x4096 with GELU: 19.6 us, 5.1 TB/s; its slope is 18 vector operations an
 // element, two of them at a quarter of the rate, about 13 us of the vector
 // units beside 14.6 us of memory, and the two overlap only across waves.  Two
@@ -318,6 +320,15 @@ int linear_plan(const LinProduct &p, LinPlan *l) {
         const double copied = 6.0 + (static_cast<double>(l->copy_a ? copy_a : 0) + static_cast<double>(l->copy_b ? copy_b : 0)) / 3e6;
         l->staged = staged < copied;
         if (l->staged) l->copy_a = l->copy_b = false;
+        // Staged 16-bit tiles wait for their own loads more than for the CU: two
+        // of them per CU from 40 stages each (100x4001x4001 [K,N] 26.8 -> 20.4 us,
+        // 127x5887x1818 [N,K] 19.6 -> 18.9, three 24.2; e4m3 200x8001x2001 22.7
+        // -> 23.2; direct loads 128x5888x1792 13.1 -> 14.8)
+        if (l->staged && !few && es == 2 && l->per >= 40 && l->tiles * l->splits <= cus) {
+            l->splits *= 2;
+            l->per = (l->stages + l->splits - 1) / l->splits;
+            l->splits = (l->stages + l->per - 1) / l->per;
+        }
     }
     if (l->copy_a) l->bytes_a = up(copy_a, 256);
     if (l->copy_b) l->bytes_b = up(copy_b, 256);

@@ -128,6 +128,18 @@ def test_forward_large(hip, shape, tw, dt):
     check(v, dt, "silu", *forward(v, dt, "silu", tw, True))
 
 
+# ragged rows, K split over two workgroups per CU (an odd count of stages, unequal splits) and over one
+@pytest.mark.parametrize("dt", H16, ids=NAMES.get)
+@pytest.mark.parametrize("tw", [False, True], ids=["w", "wT"])
+@pytest.mark.parametrize("shape", [(100, 2601, 4001), (250, 1301, 3901), (127, 5888, 1818)], ids=ids)
+def test_forward_ragged_splits(hip, shape, tw, dt):
+    v = layer(*shape, dt, tw, True, True, 70)
+    y, z = forward(v, dt, "silu", tw, True)
+    check(v, dt, "silu", y, z)
+    y2, z2 = forward(v, dt, "silu", tw, True)
+    assert np.array_equal(y, y2) and np.array_equal(z, z2)
+
+
 @pytest.mark.parametrize("dt", DTYPES, ids=NAMES.get)
 @pytest.mark.parametrize("shape", [(2, 64, 64), (40, 128, 200), (300, 128, 264)], ids=ids)
 def test_misaligned(hip, shape, dt):

@@ -366,7 +366,110 @@ __global__ __launch_bounds__(NT) void k_rms_bwd(RmsBwd a) {
     }
 }
 
-// Rows longer than k_rms_bwd holds: dx by a workgroup per row, which reads
+// The same for rows of 2048 chunks (C = 2; fp32 4096, C = 4), a workgroup of 1024
+// per row, whose registers are half as many: the chunks stay packed until the
+// output, the weights are read for each use (from L1 or L2), and with C = 4 the
+// next row is not loaded ahead.  fp16 4096x8448 61.5 us and bf16 2048x12288 with
+// dh 54.8 (held as k_rms_bwd does, spilling 31 registers, 141.6 and 104.3), fp32
+// 1024x16000 66.6 (k_rms_bwd_long 87.3); 16-bit C = 4 spills 40 registers
+// (448x30656 78.5 us; k_rms_bwd_long 45.6).
+template <int DT, int C, bool AL>
+__global__ __launch_bounds__(1024) void k_rms_bwd_wide(RmsBwd a) {
+    using S = typename Elem<DT>::S;
+    constexpr int VE = Elem<DT>::kVec, NT = 1024;
+    constexpr bool AHEAD = C <= 2;
+    __shared__ float lds[NT / kWave];
+    const S *w = static_cast<const S *>(a.w);
+    float acc[C][VE];
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) acc[i][e] = 0.0f;
+    auto span = [&](int i) {  // computed anew in each place: else 60 registers spill
+        unsigned c = i * NT + threadIdx.x;
+        asm volatile("" : "+v"(c));
+        return span_of<VE>(c, a.cols);
+    };
+    // the wave's first chunk of its i-th ones, and the chunks there are: past them there is nothing to do
+    const unsigned chunks = (a.cols + VE - 1) / VE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    auto first = [&](int i) { return i * NT + wave * kWave; };
+    struct Row {
+        Chunk<DT, VE> h[C], d[C], a[C];
+        float rs;
+    };
+    auto load = [&](Row &q, size_t row) {
+        const size_t base = row * a.cols;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const unsigned off = span(i).off;
+            load_once<AL>(q.h[i], static_cast<const S *>(a.h) + base + off);
+            load_once<AL>(q.d[i], static_cast<const S *>(a.dy) + base + off);
+            if (a.dh) load_once<AL>(q.a[i], static_cast<const S *>(a.dh) + base + off);
+        }
+        q.rs = a.rstd[row];
+    };
+    Row cur, next;
+    size_t row = blockIdx.x;
+    if constexpr (AHEAD) load(next, row);
+    for (; row < a.rows; row += gridDim.x) {
+        const size_t base = row * a.cols, then = row + gridDim.x;
+        if constexpr (AHEAD) {
+            cur = next;
+            if (then < a.rows) load(next, then);
+        } else {
+            load(cur, row);
+        }
+        auto &ch = cur.h, &cd = cur.d, &ca = cur.a;
+        const float rs = cur.rs;
+        float dot = 0.0f;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (first(i) >= chunks) break;
+            const Span s = span(i);
+            Chunk<DT, VE> cw;
+            cw.load(w + s.off);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+                const float n = ch[i].get(e) * rs, dy = e >= static_cast<int>(s.dup) ? cd[i].get(e) : 0.0f;
+                acc[i][e] = fmaf(dy, n, acc[i][e]);
+                dot = fmaf(dy * cw.get(e), n, dot);
+            }
+        }
+        const float mean = block_reduce<SumOp, NT>(dot, lds) / static_cast<float>(a.cols);
+        S *dx = static_cast<S *>(a.dx) + base;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            if (first(i) >= chunks) break;
+            // one chunk at a time, and what it unpacks to not kept from above: else 60 registers spill
+            __builtin_amdgcn_sched_barrier(0);
+            for (auto &r : ch[i].r) asm volatile("" : "+v"(r));
+            for (auto &r : cd[i].r) asm volatile("" : "+v"(r));
+            const Span s = span(i);
+            Chunk<DT, VE> cw;
+            cw.load(w + s.off);
+            float t[VE];
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+                const float n = ch[i].get(e) * rs, g = cd[i].get(e) * cw.get(e), u = n * mean;
+                const float r = rs * (g - u);
+                t[e] = a.dh ? r + ca[i].get(e) : r;
+            }
+            ch[i].set(t);
+            store_span<DT, VE>(dx, s, ch[i]);
+        }
+    }
+    float *part = a.part + static_cast<size_t>(blockIdx.x) * a.ld;
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+        const Span s = span(i);
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+            if (e >= static_cast<int>(s.dup)) part[s.off + e] = acc[i][e];
+    }
+}
+
+// Rows longer than these hold: dx by a workgroup per row, which reads
 // the row twice; dw by k_rms_dw_part, run before it (dx may be dy or h).
 template <int DT, int NT>
 __global__ __launch_bounds__(NT) void k_rms_bwd_long(RmsBwd a) {
@@ -530,6 +633,21 @@ int bwd_launch(RmsBwd a, void *dw, cxm_stream_t st) {
     return r ? r : col_sum(a.part, wgs, a.cols, a.ld, dw, DT, hs(st));
 }
 
+template <int DT, int C>
+int bwd_wide(RmsBwd a, void *dw, cxm_stream_t st) {
+    const size_t wgs = a.rows < device_cus() ? a.rows : device_cus();
+    const int rc = bwd_parts(&a, wgs, st);
+    if (rc) return rc;
+    const dim3 grid(static_cast<unsigned>(wgs));
+    constexpr size_t E = sizeof(typename Elem<DT>::S);
+    if (whole_lines(a.h, a.cols, E) && whole_lines(a.dy, a.cols, E) && whole_lines(a.dh, a.cols, E))
+        hipLaunchKernelGGL((k_rms_bwd_wide<DT, C, true>), grid, dim3(1024), 0, hs(st), a);
+    else
+        hipLaunchKernelGGL((k_rms_bwd_wide<DT, C, false>), grid, dim3(1024), 0, hs(st), a);
+    const int r = launch_status();
+    return r ? r : col_sum(a.part, wgs, a.cols, a.ld, dw, DT, hs(st));
+}
+
 template <int DT>
 int bwd_dispatch(RmsBwd a, void *dw, cxm_stream_t st) {
     constexpr int VE = Elem<DT>::kVec;
@@ -541,7 +659,10 @@ int bwd_dispatch(RmsBwd a, void *dw, cxm_stream_t st) {
     if (chunks <= 256) return bwd_launch<DT, VE, 64, 4, 256>(a, dw, st);
     if (chunks <= 512) return bwd_launch<DT, VE, 256, 2, 256>(a, dw, st);
     if (chunks <= 1024) return bwd_launch<DT, VE, 512, 2, 512>(a, dw, st);
-    if (chunks <= 2048) return bwd_launch<DT, VE, 1024, 2, 1024>(a, dw, st);
+    if (chunks <= 2048) return bwd_wide<DT, 2>(a, dw, st);
+    if constexpr (DT == CXM_DT_F32) {
+        if (chunks <= 4096) return bwd_wide<DT, 4>(a, dw, st);
+    }
     if (a.rows > most_wgs(1024)) return CXM_E_TOO_LARGE;
     const size_t tiles = (chunks + kBlock - 1) / kBlock;
     size_t parts = 4 * device_cus() / tiles;

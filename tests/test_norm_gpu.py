@@ -217,6 +217,20 @@ def test_backward_in_place_and_misaligned(hip, shape, dt):
         assert all(np.array_equal(a, b) for a, b in zip(got, want)), kw
 
 
+# several long rows for each workgroup, the last turn taken by some only
+@pytest.mark.parametrize("dt", DTYPES, ids=NAMES.get)
+@pytest.mark.parametrize("shape", [(600, 8200), (300, 12289), (513, 16384)], ids=ids)
+def test_backward_of_many_long_rows(hip, shape, dt):
+    h, rstd, w, dy, dh = bwd_data(*shape, dt)
+    dx, dw = backward(h, rstd, w, dy, dh, dt)
+    want, size, want_w, size_w = backward64(h, rstd.astype(np.float64), w, dy, dh)
+    close(dx, want, HALF[dt] * np.abs(want) + C * U32 * size + TINY[dt], "dx")
+    close(dw, want_w, HALF[dt] * np.abs(want_w) + C * U32 * size_w + TINY[dt], "dw")
+    for kw in ({"off": 1}, {"alias": "h"}, {"alias": "dy"}, {"alias": "dh"}):
+        got = backward(h, rstd, w, dy, dh, dt, **kw)
+        assert np.array_equal(got[0], dx) and np.array_equal(got[1], dw), kw
+
+
 def test_backward_of_no_rows(hip):
     dw = out(10, DT_F32)
     call("cxm_rmsnorm_bwd_t", None, None, None, None, None, None, dw.ptr, 0, 10, DT_F32, None)

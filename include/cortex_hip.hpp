@@ -532,6 +532,8 @@ public:
     bool has_grad() const noexcept { return grad_ != nullptr; }
     Tensor &grad() { return *grad_; }
     std::shared_ptr<Tensor> &grad_ptr() { return grad_; }
+    // The buffer of a gradient that was dropped, for the next one (AdamW).
+    std::shared_ptr<Tensor> &spare_grad_ptr() { return spare_grad_; }
     std::shared_ptr<GradientFlow> &flow() { return flow_; }
     // Same tensor (shared storage, gradient and flow), as a handle.
     std::shared_ptr<Storage> storage() const { return storage_; }
@@ -551,7 +553,7 @@ private:
     std::vector<std::int64_t> shape_;
     DType dtype_ = DType::Float32;
     std::shared_ptr<Storage> storage_;
-    std::shared_ptr<Tensor> grad_;
+    std::shared_ptr<Tensor> grad_, spare_grad_;
     std::shared_ptr<GradientFlow> flow_;
     bool requires_grad_ = false;
 };

@@ -67,18 +67,26 @@ private:
 // was produced by a flow.
 inline bool needs_grad(const TensorPtr &t) { return t->isRequired() || t->flow() != nullptr; }
 
+// Gives t a gradient that the caller then fills: in the buffer of its last one
+// where an optimizer left that and nobody else holds it, else in a new one.
+inline void new_grad(const TensorPtr &t) {
+    TensorPtr spare = std::move(t->spare_grad_ptr());
+    // (storage() is a handle of its own, beside the tensor's)
+    const bool free = spare && spare.use_count() == 1 && spare->storage().use_count() == 2 && spare->shape() == t->shape();
+    t->grad_ptr() = free ? std::move(spare) : make_tensor(t->shape());
+}
+
 // Adds a gradient contribution to t: `write(dst)` fills a buffer of t's
 // shape; the first contribution writes t's gradient directly.
 inline void accumulate(const TensorPtr &t, const std::function<void(float *)> &write) {
-    auto &g = t->grad_ptr();
-    if (!g) {
-        g = make_tensor(t->shape());
-        write(g->data());
+    if (!t->has_grad()) {
+        new_grad(t);
+        write(t->grad().data());
         return;
     }
     Tensor tmp = device_tensor(t->shape());
     write(tmp.data());
-    matrix_t::add(g->data(), tmp.data(), g->len());
+    matrix_t::add(t->grad().data(), tmp.data(), t->grad().len());
 }
 
 // Where a kernel that forms several gradients at once writes t's
@@ -86,7 +94,7 @@ inline void accumulate(const TensorPtr &t, const std::function<void(float *)> &w
 // grad_done then adds in; a scratch buffer when t takes no gradient.
 inline float *grad_dst(const TensorPtr &t, Tensor &tmp) {
     if (needs_grad(t) && !t->has_grad()) {
-        t->grad_ptr() = make_tensor(t->shape());
+        new_grad(t);
         return t->grad().data();
     }
     tmp = device_tensor(t->shape());
@@ -539,9 +547,12 @@ inline void sgd(const std::vector<TensorPtr> &params, float lr) {
 }
 
 // AdamW over the parameters that have a gradient, in one launch
-// (cxm_adamw_step), after which the gradients are dropped, as by sgd().  Owns
-// the fp32 moments.  The list of pointers is kept on the device and made
-// again only when a parameter's or gradient's storage has moved.
+// (cxm_adamw_step), after which the gradients are dropped, as by sgd(), but
+// their buffers stay with the parameters for the next backward pass: the pool
+// would hand them out in another order, and the list of pointers, which is
+// kept on the device (making it blocks), would not hold for the next step.  So
+// it is made again only when a parameter's storage or a gradient's has moved, or
+// another set of parameters has one.  Owns the fp32 moments.
 class AdamW {
 public:
     explicit AdamW(std::vector<TensorPtr> params, float decay = 0.0f) : params_(std::move(params)) {
@@ -554,7 +565,10 @@ public:
     }
     AdamW(const AdamW &) = delete;
     AdamW &operator=(const AdamW &) = delete;
-    ~AdamW() { drop(); }
+    ~AdamW() {
+        drop();
+        for (const auto &p : params_) p->spare_grad_ptr().reset();
+    }
     // Weight decay of parameter i alone.
     void set_decay(std::size_t i, float decay) {
         decay_.at(i) = decay;
@@ -583,7 +597,8 @@ public:
             list_ = std::move(list);
         }
         check(cxm_adamw_step(handle_, lr, beta1, beta2, eps, ++t_, nullptr, 0, stream()), "AdamW");
-        for (const auto &p : params_) p->grad_ptr().reset();
+        for (const auto &p : params_)
+            if (p->has_grad()) p->spare_grad_ptr() = std::move(p->grad_ptr());
     }
 
 private:

@@ -29,6 +29,7 @@
 #include <cstdlib>
 #include <functional>
 #include <initializer_list>
+#include <map>
 #include <memory>
 #include <string>
 #include <string_view>
@@ -546,13 +547,16 @@ inline void sgd(const std::vector<TensorPtr> &params, float lr) {
     }
 }
 
-// AdamW over the parameters that have a gradient, in one launch
-// (cxm_adamw_step), after which the gradients are dropped, as by sgd(), but
-// their buffers stay with the parameters for the next backward pass: the pool
-// would hand them out in another order, and the list of pointers, which is
-// kept on the device (making it blocks), would not hold for the next step.  So
-// it is made again only when a parameter's storage or a gradient's has moved, or
-// another set of parameters has one.  Owns the fp32 moments.
+// AdamW over the parameters that have a gradient (cxm_adamw_step), after which
+// the gradients are dropped, as by sgd(), but their buffers stay with the
+// parameters for the next backward pass: the pool would hand them out in another
+// order, and the list of pointers, which is kept on the device (making it
+// blocks), would not hold for the next step.  Owns the fp32 moments and counts
+// each parameter's own steps, which the bias corrections go by: a parameter
+// whose first gradient comes late begins at 1.  Parameters of one count are one
+// list and one launch, all of them where every step gives each a gradient; a list
+// is made again only when other parameters than before are at one count or a
+// storage has moved.
 class AdamW {
 public:
     explicit AdamW(std::vector<TensorPtr> params, float decay = 0.0f) : params_(std::move(params)) {
@@ -561,23 +565,24 @@ public:
             m_.push_back(zeros(p->shape()));
             v_.push_back(zeros(p->shape()));
             decay_.push_back(decay);
+            steps_.push_back(0);
         }
     }
     AdamW(const AdamW &) = delete;
     AdamW &operator=(const AdamW &) = delete;
     ~AdamW() {
-        drop();
+        drop([](const List &) { return true; });
         for (const auto &p : params_) p->spare_grad_ptr().reset();
     }
     // Weight decay of parameter i alone.
     void set_decay(std::size_t i, float decay) {
         decay_.at(i) = decay;
-        drop();
+        drop([&](const List &l) { return has(l, m_[i].data()); });
     }
     void step(double lr, double beta1 = 0.9, double beta2 = 0.999, double eps = 1e-8) {
-        std::vector<cxm_adamw_tensor_t> list;
+        std::map<std::size_t, std::vector<cxm_adamw_tensor_t>> by;  // step number -> its tensors
         for (std::size_t i = 0; i < params_.size(); ++i) {
-            if (!params_[i]->has_grad()) continue;
+            if (!params_[i]->has_grad() || params_[i]->len() == 0) continue;
             on_device({params_[i].get(), &params_[i]->grad()}, "AdamW");
             cxm_adamw_tensor_t t{};
             t.p = params_[i]->data();
@@ -586,38 +591,67 @@ public:
             t.v = v_[i].data();
             t.n = params_[i]->len();
             t.decay = decay_[i];
-            list.push_back(t);
+            by[steps_[i] + 1].push_back(t);
         }
-        bool same = handle_ && list.size() == list_.size();
-        for (std::size_t i = 0; same && i < list.size(); ++i)
-            same = list[i].p == list_[i].p && list[i].g == list_[i].g && list[i].m == list_[i].m;
-        if (!same) {
-            drop();
-            check(cxm_adamw_create(&handle_, list.data(), list.size(), CXM_DT_F32, CXM_DT_F32, CXM_DT_F32), "AdamW");
-            list_ = std::move(list);
+        for (const auto &[t, tensors] : by)
+            check(cxm_adamw_step(list_of(tensors), lr, beta1, beta2, eps, t, nullptr, 0, stream()), "AdamW");
+        for (std::size_t i = 0; i < params_.size(); ++i) {
+            if (!params_[i]->has_grad()) continue;
+            ++steps_[i];
+            params_[i]->spare_grad_ptr() = std::move(params_[i]->grad_ptr());
         }
-        check(cxm_adamw_step(handle_, lr, beta1, beta2, eps, ++t_, nullptr, 0, stream()), "AdamW");
-        for (const auto &p : params_)
-            if (p->has_grad()) p->spare_grad_ptr() = std::move(p->grad_ptr());
     }
 
 private:
+    struct List {
+        std::vector<cxm_adamw_tensor_t> tensors;
+        cxm_adamw *handle;
+    };
     static Tensor zeros(const std::vector<std::int64_t> &shape) {
         Tensor t = device_tensor(shape);
         check(cxm_memset(t.data(), 0, t.len() * sizeof(float), stream()), "AdamW");
         return t;
     }
-    void drop() {
-        if (handle_) (void)cxm_adamw_destroy(handle_);
-        handle_ = nullptr;
-        list_.clear();
+    static bool same(const List &l, const std::vector<cxm_adamw_tensor_t> &tensors) {
+        bool eq = l.tensors.size() == tensors.size();
+        for (std::size_t i = 0; eq && i < tensors.size(); ++i)
+            eq = l.tensors[i].p == tensors[i].p && l.tensors[i].g == tensors[i].g && l.tensors[i].m == tensors[i].m;
+        return eq;
+    }
+    // Whether the parameter of moments m is in the list.
+    static bool has(const List &l, const void *m) {
+        for (const auto &t : l.tensors)
+            if (t.m == m) return true;
+        return false;
+    }
+    // The handle for these tensors; lists that one of them was in before go.
+    cxm_adamw *list_of(const std::vector<cxm_adamw_tensor_t> &tensors) {
+        for (const List &l : lists_)
+            if (same(l, tensors)) return l.handle;
+        drop([&](const List &l) {
+            for (const auto &t : tensors)
+                if (has(l, t.m)) return true;
+            return false;
+        });
+        cxm_adamw *h = nullptr;
+        check(cxm_adamw_create(&h, tensors.data(), tensors.size(), CXM_DT_F32, CXM_DT_F32, CXM_DT_F32), "AdamW");
+        lists_.push_back({tensors, h});
+        return h;
+    }
+    template <class F>
+    void drop(const F &which) {
+        std::vector<List> keep;
+        for (List &l : lists_) {
+            if (which(l)) (void)cxm_adamw_destroy(l.handle);
+            else keep.push_back(std::move(l));
+        }
+        lists_ = std::move(keep);
     }
     std::vector<TensorPtr> params_;
     std::vector<Tensor> m_, v_;
     std::vector<float> decay_;
-    std::vector<cxm_adamw_tensor_t> list_;
-    cxm_adamw *handle_ = nullptr;
-    std::size_t t_ = 0;
+    std::vector<std::size_t> steps_;
+    std::vector<List> lists_;
 };
 
 }  // namespace cortex::_fw::hip

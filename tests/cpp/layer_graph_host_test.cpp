@@ -2,7 +2,7 @@
 // (include/cortex_hip_graph.hpp): the caching pool itself over host memory,
 // every kernel entry a stand-in that only notes what it was called with.
 // Checks what the graph asks the library for: how often AdamW makes its list
-// of tensors.  Prints ALL OK and returns 0 when every check passes.
+// of tensors, and which step number each parameter gets.  Prints ALL OK and returns 0 when every check passes.
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -26,6 +26,12 @@ cxm::CachingPool<HostBackend> &pool() {
 }
 
 int creates = 0, live = 0;
+std::vector<std::pair<const void *, size_t>> steps;  // (parameter, step number) of every step
+size_t step_of(const hip::TensorPtr &p) {            // the last one, 0 for none
+    for (auto it = steps.rbegin(); it != steps.rend(); ++it)
+        if (it->first == p->data()) return it->second;
+    return 0;
+}
 
 int failures = 0;
 #define EXPECT(c, ...)                          \
@@ -78,7 +84,8 @@ int cxm_adamw_create(cxm_adamw **h, const cxm_adamw_tensor_t *t, size_t n, int, 
     *h = new cxm_adamw{std::vector<cxm_adamw_tensor_t>(t, t + n)};
     return CXM_OK;
 }
-int cxm_adamw_step(cxm_adamw *, double, double, double, double, size_t, const float *, uint64_t, cxm_stream_t) {
+int cxm_adamw_step(cxm_adamw *h, double, double, double, double, size_t t, const float *, uint64_t, cxm_stream_t) {
+    for (const auto &e : h->list) steps.emplace_back(e.p, t);
     return CXM_OK;
 }
 int cxm_adamw_destroy(cxm_adamw *h) {
@@ -129,6 +136,35 @@ void kept_gradient() {
     EXPECT(w->grad().data() != copy.data(), "a gradient held by its storage is written again");
 }
 
+// A parameter's step number counts its own steps: one that joins late begins at
+// 1, one that misses steps does not count them, and a step without gradients is none.
+void own_step_numbers() {
+    auto x = hip::make_tensor({4, 6});
+    auto w = leaf(6, 8), late = leaf(8, 8), some = leaf(8, 5);
+    hip::AdamW opt({w, late, some});
+    steps.clear();
+    creates = 0;
+    opt.step(1e-3);
+    EXPECT(steps.empty() && creates == 0, "a step without gradients");
+    size_t nl = 0, ns = 0;
+    int made = 0;
+    for (size_t s = 1; s <= 12; ++s) {
+        auto y = hip::linear(x, w);
+        if (s >= 3) y = hip::linear(y, late), ++nl;
+        if (s % 2 == 0) y = hip::linear(y, some), ++ns;
+        const size_t before = steps.size();
+        hip::backward(y);
+        opt.step(1e-3);
+        opt.step(1e-3);  // none has a gradient now
+        EXPECT(step_of(w) == s && step_of(late) == nl && step_of(some) == ns, "step %zu: %zu %zu %zu for %zu %zu %zu", s,
+               step_of(w), step_of(late), step_of(some), s, nl, ns);
+        EXPECT(steps.size() - before == size_t(1) + (s >= 3) + (s % 2 == 0), "step %zu: %zu parameters", s, steps.size() - before);
+        if (s == 6) made = creates;
+    }
+    // {w}, {some} and {late} are of different numbers from step 5 on: their lists stay
+    EXPECT(made == creates, "%d lists were made after step 6", creates - made);
+}
+
 }  // namespace
 
 int main() {
@@ -137,6 +173,7 @@ int main() {
                                {64, 1024, 4096}, {1024, 1024, 1024}};
     for (const auto &s : sizes) lists_made(s[0], s[1], s[2]);
     kept_gradient();
+    own_step_numbers();
     EXPECT(live == 0, "%d lists are left", live);
     pool().release_cached();
     if (failures == 0) std::printf("ALL OK\n");

@@ -429,17 +429,21 @@ inline TensorPtr rms_norm(const TensorPtr &x, const TensorPtr &w, float eps = 1e
     on_device({x.get(), w.get()}, "rms_norm");
     if (w->len() != cols_of(*x)) check(CXM_E_INVALID, "rms_norm: one weight per column");
     auto y = make_tensor(x->shape());
-    Tensor rstd = device_tensor({x->dim(0)});
-    check(cxm_rmsnorm_fwd_t(x->data(), nullptr, w->data(), eps, nullptr, y->data(), nullptr, nullptr, rstd.data(),
-                            rows_of(*x), cols_of(*x), CXM_DT_F32, stream()),
+    const bool grad = needs_grad(x) || needs_grad(w);
+    Tensor rstd;
+    if (grad) rstd = device_tensor({x->dim(0)});
+    check(cxm_rmsnorm_fwd_t(x->data(), nullptr, w->data(), eps, nullptr, y->data(), nullptr, nullptr,
+                            grad ? rstd.data() : nullptr, rows_of(*x), cols_of(*x), CXM_DT_F32, stream()),
           "rms_norm");
-    if (needs_grad(x) || needs_grad(w)) link(y, std::make_shared<RmsNormFlow>(x, w, std::move(rstd)));
+    if (grad) link(y, std::make_shared<RmsNormFlow>(x, w, std::move(rstd)));
     return y;
 }
 
 // Y = act(X W + bias) + residual (cxm_linear_fwd_t), bias and residual
 // optional: the gradients of X, W and the bias from the saved X W + bias
-// (cxm_linear_bwd_t); the residual's is dY.
+// (cxm_linear_bwd_t); the residual's is dY.  X W + bias is saved only where one
+// of those three takes a gradient (without it the fp32 product applies a ReLU
+// itself).
 struct LinearFlow : GradientFlow {
     TensorPtr x, w, bias, res;
     Tensor z;
@@ -454,14 +458,16 @@ struct LinearFlow : GradientFlow {
     void backward(const Tensor &dy) override {
         const std::size_t M = rows_of(*x), K = cols_of(*x), N = cols_of(*w);
         Tensor tx, tw, tb, dz;
-        if (act != CXM_ACT_NONE) dz = device_tensor(dy.shape());
+        const bool products = needs_grad(x) || needs_grad(w) || (bias && needs_grad(bias));
+        if (products && act != CXM_ACT_NONE) dz = device_tensor(dy.shape());
         float *dx = needs_grad(x) ? grad_dst(x, tx) : nullptr;
         // a tensor that is an input twice already has its first contribution when the second is made
         float *dw = needs_grad(w) ? grad_dst(w, tw) : nullptr;
         float *db = bias && needs_grad(bias) ? grad_dst(bias, tb) : nullptr;
-        check(cxm_linear_bwd_t(x->data(), w->data(), z.empty() ? nullptr : z.data(), dy.data(),
-                               dz.empty() ? nullptr : dz.data(), dx, dw, db, M, K, N, 0, act, CXM_DT_F32, stream()),
-              "LinearFlow");
+        if (products)
+            check(cxm_linear_bwd_t(x->data(), w->data(), z.empty() ? nullptr : z.data(), dy.data(),
+                                   dz.empty() ? nullptr : dz.data(), dx, dw, db, M, K, N, 0, act, CXM_DT_F32, stream()),
+                  "LinearFlow");
         grad_done(x, tx);
         grad_done(w, tw);
         if (db) grad_done(bias, tb);
@@ -481,12 +487,13 @@ inline TensorPtr linear(const TensorPtr &x, const TensorPtr &w, const TensorPtr 
     if (rows_of(*w) != K || (bias && bias->len() != N) || (res && res->len() != M * N))
         check(CXM_E_INVALID, "linear: sizes do not match");
     auto y = make_tensor({x->dim(0), w->dim(1)});
+    const bool products = needs_grad(x) || needs_grad(w) || (bias && needs_grad(bias));
     Tensor z;
-    if (act != CXM_ACT_NONE) z = device_tensor(y->shape());
+    if (products && act != CXM_ACT_NONE) z = device_tensor(y->shape());
     check(cxm_linear_fwd_t(x->data(), w->data(), bias ? bias->data() : nullptr, res ? res->data() : nullptr,
                            z.empty() ? nullptr : z.data(), y->data(), M, K, N, 0, act, CXM_DT_F32, stream()),
           "linear");
-    if (needs_grad(x) || needs_grad(w) || (bias && needs_grad(bias)) || (res && needs_grad(res)))
+    if (products || (res && needs_grad(res)))
         link(y, std::make_shared<LinearFlow>(x, w, bias, res, std::move(z), act));
     return y;
 }

@@ -2,7 +2,8 @@
 // (include/cortex_hip_graph.hpp): the caching pool itself over host memory,
 // every kernel entry a stand-in that only notes what it was called with.
 // Checks what the graph asks the library for: how often AdamW makes its list
-// of tensors, and which step number each parameter gets.  Prints ALL OK and returns 0 when every check passes.
+// of tensors, which step number each parameter gets, and that layers keep nothing
+// for a backward pass that does not come.  Prints ALL OK and returns 0 when every check passes.
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -32,6 +33,10 @@ size_t step_of(const hip::TensorPtr &p) {            // the last one, 0 for none
         if (it->first == p->data()) return it->second;
     return 0;
 }
+
+// of the last forward call, and the backward calls
+const void *saved_z = nullptr, *saved_rstd = nullptr;
+int backwards = 0;
 
 int failures = 0;
 #define EXPECT(c, ...)                          \
@@ -63,20 +68,23 @@ int cxm_stream_sync(cxm_stream_t) { return CXM_OK; }
 int cxm_binary_f32(const float *, const float *, float *, size_t, int, cxm_stream_t) { return CXM_OK; }
 int cxm_bcast_col_f32(const float *, const float *, float *, size_t, size_t, int, cxm_stream_t) { return CXM_OK; }
 int cxm_softmax_xent_f32(const float *, const int32_t *, float *, float *, size_t, size_t, cxm_stream_t) { return CXM_OK; }
-int cxm_rmsnorm_fwd_t(const void *, const void *, const void *, float, void *, void *, uint8_t *, float *, float *, size_t,
-                      size_t, int, cxm_stream_t) {
+int cxm_rmsnorm_fwd_t(const void *, const void *, const void *, float, void *, void *, uint8_t *, float *, float *rstd,
+                      size_t, size_t, int, cxm_stream_t) {
+    saved_rstd = rstd;
     return CXM_OK;
 }
 int cxm_rmsnorm_bwd_t(const void *, const float *, const void *, const void *, const void *, void *, void *, size_t,
                       size_t, int, cxm_stream_t) {
     return CXM_OK;
 }
-int cxm_linear_fwd_t(const void *, const void *, const void *, const void *, void *, void *, size_t, size_t, size_t, int,
+int cxm_linear_fwd_t(const void *, const void *, const void *, const void *, void *z, void *, size_t, size_t, size_t, int,
                      int, int, cxm_stream_t) {
+    saved_z = z;
     return CXM_OK;
 }
 int cxm_linear_bwd_t(const void *, const void *, const void *, const void *, void *, void *, void *, void *, size_t,
                      size_t, size_t, int, int, int, cxm_stream_t) {
+    ++backwards;
     return CXM_OK;
 }
 int cxm_adamw_create(cxm_adamw **h, const cxm_adamw_tensor_t *t, size_t n, int, int, int) {
@@ -165,6 +173,28 @@ void own_step_numbers() {
     EXPECT(made == creates, "%d lists were made after step 6", creates - made);
 }
 
+// What the backward reads (z, 1 / rms) is asked for only where it will be read.
+void nothing_kept_without_gradients() {
+    auto x = hip::make_tensor({4, 6}), w = hip::make_tensor({6, 8}), b = hip::make_tensor({8}), g = hip::make_tensor({6}),
+         r = hip::make_tensor({4, 8});
+    auto wg = leaf(6, 8), bg = leaf(0, 8), gg = leaf(0, 6), rg = leaf(4, 8), xg = leaf(4, 6);
+    for (int act : {CXM_ACT_RELU, CXM_ACT_GELU}) {
+        EXPECT(!hip::linear(x, w, b, act, r)->flow() && !saved_z, "act %d: z without a gradient", act);
+        EXPECT(hip::linear(x, wg, b, act, r)->flow() && saved_z, "act %d: z for the weight", act);
+        EXPECT(hip::linear(xg, w, b, act, r)->flow() && saved_z, "act %d: z for x", act);
+        EXPECT(hip::linear(x, w, bg, act, r)->flow() && saved_z, "act %d: z for the bias", act);
+        auto y = hip::linear(x, w, b, act, rg);  // dY is the residual's gradient
+        EXPECT(y->flow() && !saved_z, "act %d: z for the residual alone", act);
+        backwards = 0;
+        hip::backward(y);
+        EXPECT(backwards == 0 && rg->has_grad(), "act %d: the residual's gradient alone", act);
+        rg->grad_ptr().reset();
+    }
+    EXPECT(!hip::rms_norm(x, g)->flow() && !saved_rstd, "1 / rms without a gradient");
+    EXPECT(hip::rms_norm(x, gg)->flow() && saved_rstd, "1 / rms for the gain");
+    EXPECT(hip::rms_norm(xg, g)->flow() && saved_rstd, "1 / rms for x");
+}
+
 }  // namespace
 
 int main() {
@@ -174,6 +204,7 @@ int main() {
     for (const auto &s : sizes) lists_made(s[0], s[1], s[2]);
     kept_gradient();
     own_step_numbers();
+    nothing_kept_without_gradients();
     EXPECT(live == 0, "%d lists are left", live);
     pool().release_cached();
     if (failures == 0) std::printf("ALL OK\n");

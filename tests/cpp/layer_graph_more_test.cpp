@@ -1,5 +1,6 @@
 // More of the autograd graph's layers and AdamW (cortex_hip_graph.hpp) on the GPU:
-// parameters that do not all have a gradient at every step.
+// parameters that do not all have a gradient at every step, and layers whose inputs
+// take none.
 #include <cmath>
 #include <cstdio>
 #include <vector>
@@ -85,8 +86,28 @@ static void own_step_numbers() {
     EXPECT(exact[0].t == 8 && exact[1].t == 6 && exact[2].t == 4, "steps");
 }
 
+// A layer gives the same bits whether or not its backward pass will come.
+static void without_gradients() {
+    for (int act : {CXM_ACT_NONE, CXM_ACT_RELU, CXM_ACT_SIGMOID, CXM_ACT_TANH, CXM_ACT_GELU, CXM_ACT_SILU})
+        for (int with : {0, 1, 2, 3}) {
+            std::vector<float> y[2];
+            for (int grad : {0, 1}) {
+                auto x = leaf({37, 20}, 5, grad), w = leaf({20, 53}, 6, grad), g = leaf({20}, 7, grad);
+                auto b = with & 1 ? leaf({53}, 8, grad) : nullptr, r = with & 2 ? leaf({37, 53}, 9, grad) : nullptr;
+                auto t = hip::linear(hip::rms_norm(x, g), w, b, act, r);
+                EXPECT((t->flow() != nullptr) == (grad != 0), "act %d: the flow", act);
+                y[grad] = t->host();
+            }
+            EXPECT(y[0] == y[1], "act %d, bias and residual %d: other bits without gradients", act, with);
+        }
+    auto x = leaf({37, 20}, 5, false), w = leaf({20, 53}, 6, false), r = leaf({37, 53}, 9, true);
+    hip::backward(hip::linear(x, w, nullptr, CXM_ACT_GELU, r));
+    EXPECT(r->grad().host() == std::vector<float>(37 * 53, 1.0f), "the gradient of the residual alone");
+}
+
 int main() {
     own_step_numbers();
+    without_gradients();
     hip::check(cxm_device_sync(), "sync");
     if (failures == 0) std::printf("ALL OK\n");
     return failures == 0 ? 0 : 1;

@@ -1,6 +1,6 @@
-"""Parameters without a gradient at every step in the C++ autograd graph's AdamW
-(include/cortex_hip_graph.hpp) on the GPU: tests/cpp/layer_graph_more_test, built
-by __graft_entry__.build()."""
+"""The C++ autograd graph (include/cortex_hip_graph.hpp) on the GPU where not all
+tensors take a gradient: AdamW's parameters without one at every step, layers
+without any (tests/cpp/layer_graph_more_test, built by __graft_entry__.build())."""
 import os
 import subprocess
 

@@ -27,6 +27,7 @@ struct PadSide {
     const uint8_t *x;
     uint8_t *y;
     size_t rows, bytes, out_rows;  // stored rows and their length; rows of the copy, zero past them
+    size_t row0;                   // the launch's first row
     unsigned pieces, tiles;        // 16-byte pieces of a row of the copy; workgroups per kPadRows rows
     unsigned wgs;
 };
@@ -43,7 +44,7 @@ __global__ __launch_bounds__(kBlock) void k_pad(PadSide a, PadSide b) {
     const unsigned id = first ? blockIdx.x : blockIdx.x - a.wgs;
     const unsigned lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
     const unsigned piece = id % p.tiles * kWave + lane;
-    const size_t r0 = static_cast<size_t>(id / p.tiles) * kPadRows + w * R, at = static_cast<size_t>(piece) * 16;
+    const size_t r0 = p.row0 + static_cast<size_t>(id / p.tiles) * kPadRows + w * R, at = static_cast<size_t>(piece) * 16;
     if (piece >= p.pieces) return;
     uint64_t lo[R], hi[R];
     if (p.bytes >= 16) {
@@ -81,14 +82,32 @@ __global__ __launch_bounds__(kBlock) void k_pad(PadSide a, PadSide b) {
     }
 }
 
-// Fills in the launch of one side; false when beyond the grid.
-bool pad_side(PadSide *p, const void *x, void *y, size_t rows, size_t bytes, size_t out_rows, size_t out_bytes) {
-    const size_t pieces = out_bytes / 16, tiles = (pieces + kWave - 1) / kWave;
-    const size_t wgs = (out_rows + kPadRows - 1) / kPadRows * tiles;
-    if (wgs > most_wgs(kBlock) / 2 || pieces > 0x7fffffffu) return false;  // (two sides in a launch)
-    *p = PadSide{static_cast<const uint8_t *>(x), static_cast<uint8_t *>(y), rows, bytes, out_rows,
-                 static_cast<unsigned>(pieces), static_cast<unsigned>(tiles), static_cast<unsigned>(wgs)};
-    return true;
+PadSide pad_side(const void *x, void *y, size_t rows, size_t bytes, size_t out_rows, size_t out_bytes) {
+    const size_t pieces = out_bytes / 16;
+    return PadSide{static_cast<const uint8_t *>(x), static_cast<uint8_t *>(y), rows, bytes, out_rows, 0,
+                   static_cast<unsigned>(pieces), static_cast<unsigned>((pieces + kWave - 1) / kWave), 0};
+}
+
+// Both sides in one launch (out_rows 0: no such side); rows past what a grid holds,
+// 2^23 workgroups a side, in launches of their own.
+int pad_launch(PadSide a, PadSide b, hipStream_t s) {
+    size_t next[2] = {0, 0};
+    while (next[0] < a.out_rows || next[1] < b.out_rows) {
+        for (int i = 0; i < 2; ++i) {
+            PadSide &p = i ? b : a;
+            p.row0 = next[i];
+            p.wgs = 0;
+            if (next[i] >= p.out_rows) continue;
+            const size_t need = (p.out_rows - next[i] + kPadRows - 1) / kPadRows, most = most_wgs(kBlock) / 2 / p.tiles;
+            const size_t groups = need < most ? need : most;
+            p.wgs = static_cast<unsigned>(groups * p.tiles);
+            next[i] += groups * kPadRows;
+        }
+        hipLaunchKernelGGL(k_pad, dim3(a.wgs + b.wgs), dim3(kBlock), 0, s, a, b);
+        const int r = launch_status();
+        if (r) return r;
+    }
+    return CXM_OK;
 }
 
 // ------------------------------------------------------------ fp32 layer
@@ -346,21 +365,16 @@ int linear_run(const LinProduct &p, const LinPlan &l, char *scratch, unsigned *c
     PadSide pa{}, pb{};
     if (l.copy_a) {
         a = scratch;
-        if (!(p.ta ? pad_side(&pa, p.a, scratch, p.K, p.M * es, krows, l.lda * 2)
-                   : pad_side(&pa, p.a, scratch, p.M, p.K * es, p.M, l.lda * 2)))
-            return CXM_E_TOO_LARGE;
+        pa = p.ta ? pad_side(p.a, scratch, p.K, p.M * es, krows, l.lda * 2)
+                  : pad_side(p.a, scratch, p.M, p.K * es, p.M, l.lda * 2);
     }
     if (l.copy_b) {
         b = scratch + l.bytes_a;
-        if (!(p.tb ? pad_side(&pb, p.b, scratch + l.bytes_a, p.N, p.K * es, p.N, l.ldb * 2)
-                   : pad_side(&pb, p.b, scratch + l.bytes_a, p.K, p.N * es, krows, l.ldb * 2)))
-            return CXM_E_TOO_LARGE;
+        pb = p.tb ? pad_side(p.b, scratch + l.bytes_a, p.N, p.K * es, p.N, l.ldb * 2)
+                  : pad_side(p.b, scratch + l.bytes_a, p.K, p.N * es, krows, l.ldb * 2);
     }
-    if (l.copy_a || l.copy_b) {
-        hipLaunchKernelGGL(k_pad, dim3(pa.wgs + pb.wgs), dim3(kBlock), 0, s, pa, pb);
-        const int r = launch_status();
-        if (r) return r;
-    }
+    const int rc = pad_launch(pa, pb, s);
+    if (rc) return rc;
     return linear_ring_run(p, l, a, b, reinterpret_cast<float *>(scratch + l.bytes_a + l.bytes_b), counters, s);
 }
 

@@ -471,8 +471,9 @@ int cxm_quant_rows_t(const void *x, uint8_t *q, float *scale, size_t rows, size_
  * distribution function), SILU.  bias, res and z may be NULL; z, what the
  * backward reads, is rounded, y comes from the unrounded one.  y may be
  * res itself (in fp32 only with z given); any other overlap of an output is
- * CXM_E_INVALID.  k, n < 2^23, else CXM_E_TOO_LARGE.  m == 0 or n == 0 does
- * nothing; k == 0 is CXM_E_INVALID.  Rows whose length is no multiple of 64
+ * CXM_E_INVALID.  m < 2^31, k and n < 2^23 and at most 2^22 - 1 tiles of the
+ * result (of 32x64 to 256x256), else CXM_E_TOO_LARGE, before any launch.  m == 0
+ * or n == 0 does nothing; k == 0 is CXM_E_INVALID.  Rows whose length is no multiple of 64
  * bytes, and few tiles, need scratch (see CXM_E_CAPTURE).  Beside
  * cxm_gemm_f32 and cxm_matmul_t; no reference counterpart. */
 int cxm_linear_fwd_t(const void *x, const void *w, const void *bias, const void *res, void *z, void *y, size_t m,

@@ -295,7 +295,7 @@ int linear_plan(const LinProduct &p, LinPlan *l) {
     l->copy_b = !aligned16(p.b) || (p.tb ? kb % 64 != 0 : p.N % 8 != 0 || p.K % 32 != 0);
     l->lda = p.ta ? up(p.M, 8) : kpad;
     l->ldb = p.tb ? kpad : up(p.N, 8);
-    if (l->lda >= (size_t(1) << 23) || l->ldb >= (size_t(1) << 23)) return CXM_E_TOO_LARGE;
+    if (l->lda > (size_t(1) << 23) || l->ldb > (size_t(1) << 23)) return CXM_E_TOO_LARGE;  // (never, by dims_ok)
     const size_t cus = device_cus();
     auto tiles = [&](size_t tm, size_t tn) { return ((p.M + tm - 1) / tm) * ((p.N + tn - 1) / tn); };
     // The tile, by what these cost at K = 1024 (us; CUs of 256):

@@ -711,9 +711,10 @@ int linear_ring_run(const LinProduct &p, const LinPlan &l, const void *A, const 
         return CXM_E_TOO_LARGE;
     // what the kernels assume: direct loads, 16-byte aligned rows and whole stages;
     // staged ones, rows of 16 bytes at least; both, a tile's lane offsets within 32 bits
+    // (255 rows of 2^24 bytes)
     if (l.staged ? row_a < 16 || row_b < 16 || row_a >= (size_t(1) << 24) || row_b >= (size_t(1) << 24)
-                 : !aligned16(A) || !aligned16(B) || l.lda % 8 != 0 || l.ldb % 8 != 0 || l.lda >= (size_t(1) << 23) ||
-                       l.ldb >= (size_t(1) << 23))
+                 : !aligned16(A) || !aligned16(B) || l.lda % 8 != 0 || l.ldb % 8 != 0 || l.lda > (size_t(1) << 23) ||
+                       l.ldb > (size_t(1) << 23))
         return CXM_E_TOO_LARGE;
     const RingArgs a{static_cast<const uint16_t *>(A),
                      static_cast<const uint16_t *>(B),

@@ -39,13 +39,23 @@ void launch(const float *part, unsigned n, unsigned cols, size_t ld, void *out, 
 
 }  // namespace
 
+// (Columns past what a grid holds, 2^26 - 16 of them, in a launch of their own:
+// the callers have launched their first half and must not be refused here.)
 int col_sum(const float *part, size_t n, size_t cols, size_t ld, void *out, int dtype, hipStream_t s) {
-    if (n > 0x7fffffffu || cols > 0x7fffffffu || (cols + kSumCols - 1) / kSumCols > most_wgs(kSumThreads)) return CXM_E_TOO_LARGE;
-    const unsigned nn = static_cast<unsigned>(n), nc = static_cast<unsigned>(cols);
-    if (dtype == CXM_DT_F32) launch<CXM_DT_F32>(part, nn, nc, ld, out, s);
-    else if (dtype == CXM_DT_BF16) launch<CXM_DT_BF16>(part, nn, nc, ld, out, s);
-    else launch<CXM_DT_F16>(part, nn, nc, ld, out, s);
-    return launch_status();
+    if (n > 0x7fffffffu || cols > 0x7fffffffu) return CXM_E_TOO_LARGE;
+    constexpr size_t kMost = most_wgs(kSumThreads) * kSumCols;
+    const unsigned nn = static_cast<unsigned>(n);
+    for (size_t j = 0; j < cols; j += kMost) {
+        const unsigned nc = static_cast<unsigned>(cols - j < kMost ? cols - j : kMost);
+        const float *p = part ? part + j : nullptr;
+        char *o = static_cast<char *>(out) + j * dtype_bytes(dtype);
+        if (dtype == CXM_DT_F32) launch<CXM_DT_F32>(p, nn, nc, ld, o, s);
+        else if (dtype == CXM_DT_BF16) launch<CXM_DT_BF16>(p, nn, nc, ld, o, s);
+        else launch<CXM_DT_F16>(p, nn, nc, ld, o, s);
+        const int r = launch_status();
+        if (r) return r;
+    }
+    return CXM_OK;
 }
 
 }  // namespace cxm

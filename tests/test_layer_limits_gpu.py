@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from cortexmind_amd._lib import DT_BF16, DT_F16, call
+from cortexmind_amd._lib import DT_BF16, DT_F16, DT_F32, call
 from cortexmind_amd.data import SplitMix64
 from cortexmind_amd.device import DeviceArray
 from layer_util import HALF, TINY, U32, close, from_bits, get, rounded, to_bits, up
@@ -81,3 +81,39 @@ def test_longest_rows_backward(hip):
     want, size = x.T @ dy, np.abs(x).T @ np.abs(dy)
     close(from_bits(gw[:PERIOD], dt), want, HALF[dt] * np.abs(want) + m * U32 * size + TINY[dt])
     assert np.array_equal(gw, np.resize(gw[:PERIOD], (LAST, n)))
+
+
+@pytest.mark.parametrize("dt", [DT_F32, DT_BF16], ids=["f32", "bf16"])
+def test_longest_rows_of_the_norm_backward(hip, dt):
+    """2^26 - 1 columns: the sums of dw of the last ones are past one launch's grid."""
+    rows, cols, period = 2, (1 << 26) - 1, 4093
+    g = SplitMix64(95)
+    h, dy = rounded(g.normal((rows, period)), dt), rounded(g.normal((rows, period)), dt)
+    w = rounded(g.normal((1, period), 1.0, 0.2), dt)
+
+    def long(a):
+        return DeviceArray.from_numpy(np.concatenate([np.resize(r, (1, cols)) for r in to_bits(a, dt)]))
+
+    rstd = np.array([0.75, 1.25], np.float32)
+    bh, bdy, bw, br = long(h), long(dy), long(w), DeviceArray.from_numpy(rstd)
+    store = np.float32 if dt == DT_F32 else np.uint16
+    dx, dw = DeviceArray((rows, cols), store), DeviceArray((cols,), store)
+    call("cxm_rmsnorm_bwd_t", bh.ptr, br.ptr, bw.ptr, bdy.ptr, None, dx.ptr, dw.ptr, rows, cols, dt, None)
+    n, gr = h * rstd[:, None].astype(np.float64), dy * w
+    turns, rest = divmod(cols, period)
+    dot = (gr * n).sum(axis=1) * turns + (gr * n)[:, :rest].sum(axis=1)
+    mag = np.abs(gr * n).sum(axis=1) * (turns + 1)
+    got = dw.numpy()
+    want, size = (dy * n).sum(axis=0), np.abs(dy * n).sum(axis=0)
+    close(from_bits(got[:period], dt), want, HALF[dt] * np.abs(want) + 4 * U32 * size + TINY[dt], "dw")
+    assert np.array_equal(got, np.resize(got[:period], cols))
+    # a thread's sum has 8 columns of every 8192, of four-column chunks 4 of every 4096: 2^16 terms in turn
+    mean, off = dot / cols, (2 ** 16 + 32) * U32 * mag / cols
+    r = rstd[:, None].astype(np.float64)
+    want = r * (gr - n * mean[:, None])
+    size = r * (np.abs(gr) + np.abs(n) * np.abs(mean)[:, None])
+    gx = dx.numpy()
+    close(from_bits(gx[:, :period], dt), want,
+          HALF[dt] * np.abs(want) + 4 * U32 * size + r * np.abs(n) * off[:, None] + TINY[dt], "dx")
+    for i in range(rows):
+        assert np.array_equal(gx[i], np.resize(gx[i, :period], cols)), i

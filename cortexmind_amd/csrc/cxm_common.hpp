@@ -253,26 +253,18 @@ __device__ __forceinline__ void tail_store(float *p, float4 v, int i, int off) {
 }
 
 // Direct global-to-LDS load of 16 bytes per lane (global_load_lds_dwordx4):
-// lane L's 16 bytes at gsrc land at LDS byte lds + 16 L (lds wave-uniform,
-// placed in M0).  Issued through inline asm so that the compiler's wait
+// lane L's 16 bytes at base + off, a 32-bit byte offset of its own, land at LDS
+// byte lds + 16 L.  Issued through inline asm so that the compiler's wait
 // insertion does not see an LDS write in flight: it cannot always tell which
 // LDS array such a load fills and then waits for every outstanding load
 // (vmcnt(0)) before unrelated LDS reads.  The caller orders the load against
 // LDS reads and writes itself (s_waitcnt vmcnt plus a barrier before the
 // data is read; no read of the destination in flight when it is issued) and
 // waits for it before the workgroup ends.
-__device__ __forceinline__ void lds_load16(const void *gsrc, const void *lds) {
-    const unsigned a = __builtin_amdgcn_readfirstlane(
-        static_cast<unsigned>(reinterpret_cast<size_t>((const __attribute__((address_space(3))) void *)lds)));
-    asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(gsrc), "{m0}"(a) : "memory");
-}
-
-// The same load from a wave-uniform base (an SGPR pair) plus a 32-bit
-// per-lane byte offset (the saddr form): the lane's address costs no 64-bit
-// vector arithmetic.
-// `base` and `lds` (the LDS byte address, lds_addr) are the same in every
+// `base` (an SGPR pair: the saddr form, no 64-bit vector arithmetic per load)
+// and `lds` (the LDS byte address, lds_addr; in M0) are the same in every
 // lane; read from the first lane, they are scalar values for the
-// instruction's SGPR operands whatever registers the compiler held them in.
+// instruction's operands whatever registers the compiler held them in.
 // The base goes through a scalar move: a vector-memory instruction may read an
 // SGPR that a vector instruction wrote (v_readfirstlane) only five wait states
 // later, which the compiler sees to for its own loads but not inside asm, and
@@ -295,7 +287,7 @@ __device__ __forceinline__ unsigned lds_addr(const void *p) {
         static_cast<unsigned>(reinterpret_cast<size_t>((const __attribute__((address_space(3))) void *)p)));
 }
 
-// Barrier of an LDS ring filled by lds_load16: this wave waits until at
+// Barrier of an LDS ring filled by lds_load16_at: this wave waits until at
 // most PENDING of its global loads are outstanding (loads retire in order,
 // so every older fill has landed in LDS) and for its own LDS reads, then
 // joins the workgroup barrier; after it, every wave's older fills are

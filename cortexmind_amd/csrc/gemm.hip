@@ -717,7 +717,7 @@ __global__ __launch_bounds__(kW4Threads) void k_gemm_w4(const float *__restrict_
 // ------------------------------------------------ direct-to-LDS ring
 // A 256-thread workgroup (four waves of 64x64, 2x2 MFMA blocks each) per
 // 128x128 tile; K runs over a ring of four LDS stages of 32 k (16 KiB per
-// operand), filled by direct global-to-LDS loads (lds_load16) four steps
+// operand), filled by direct global-to-LDS loads (lds_load16_at) four steps
 // ahead, so three tiles are in flight while one is multiplied.  The
 // stage of step t is refilled with tile t+4 right after the ring barrier
 // that follows its last fragment read.  K a multiple of 8 (a split's range
@@ -736,7 +736,7 @@ __global__ __launch_bounds__(kW4Threads) void k_gemm_w4(const float *__restrict_
 constexpr int kRingThreads = 256;
 constexpr int kRBK = 32;                    // k per stage
 constexpr int kRST = BM * kRBK;             // floats per operand stage
-constexpr int kRPS = 2 * (kRST / 4 / kRingThreads);  // lds_load16 per wave per stage (A and B)
+constexpr int kRPS = 2 * (kRST / 4 / kRingThreads);  // lds_load16_at per wave per stage (A and B)
 
 // Shapes the ring takes: whole 8-k blocks; a partial last M or N tile is
 // clamped, which needs the [K, M] / [K, N] storage's row length a multiple

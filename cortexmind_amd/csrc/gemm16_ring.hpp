@@ -21,7 +21,7 @@ __device__ __forceinline__ unsigned xcd_remap16(unsigned b, unsigned g) {
 // (NB x NB MFMA blocks of 32x32, NB = TM/64), interior tiles only (M, N
 // multiples of TM, K a multiple of 128).  The k loop runs over a ring of
 // four LDS stages of 32 k, filled by direct global-to-LDS loads
-// (lds_load16) four steps ahead (three tiles in flight); the loop is
+// (lds_load16_at) four steps ahead (three tiles in flight); the loop is
 // unrolled over the ring so that stage addresses are constants.
 // A step on stage t: MFMAs of k block 0 with block 1's fragments read
 // between them; the ring barrier (this wave's loads of stage t+1 landed,

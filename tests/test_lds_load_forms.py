@@ -16,8 +16,8 @@ def sources():
 
 
 def test_asm_loads_begin_with_the_scalar_move():
-    asm = [(n, m.group(1)) for n, text in sources() for m in re.finditer(r"asm\s+volatile\s*\(\s*\"([^\"]*)\"", text)
-           if "load_lds" in m.group(1)]
+    asm = [(n, "".join(re.findall(r"\"([^\"]*)\"", m.group(1)))) for n, text in sources()
+           for m in re.finditer(r"asm\s+(?:volatile\s*)?\(((?:\s*\"[^\"]*\")+)", text) if "load_lds" in m.group(1)]
     assert asm
     for name, code in asm:
         steps = [c.strip() for c in code.replace("\\t", " ").split("\\n")]

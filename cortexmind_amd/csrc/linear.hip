@@ -173,9 +173,9 @@ int linear_f32(const float *x, const float *w, const float *bias, const float *r
 // LDS, the workgroups' shares in k_col_sum, both in a fixed order (for few rows
 // the last workgroup of a tile adding them costs what the launch does: 512x1024
 // 21.5 -> 23.8 us for the whole backward, 98x86 13.5 -> 12.3).  bf16
-// 4096x4096 with GELU: 19.6 us, 5.1 TB/s; its slope is 18 vector operations an
-// element, two of them at a quarter of the rate, about 13 us of the vector
-// units beside 14.6 us of memory, and the two overlap only across waves.  Two
+// 4096x4096 with GELU: 19.6 us, 5.1 TB/s; 26 vector instructions an element, by
+// the counters 12.5 us of the vector units beside 14.6 us of memory, and the
+// two overlap only across waves.  Two
 // and four rows in flight per wave (20.0, 21.9 us) and the next row loaded
 // ahead of the slope (20.5, 19.6 with half the workgroups) gain nothing.
 struct ActBwd {
@@ -302,7 +302,10 @@ int linear_plan(const LinProduct &p, LinPlan *l) {
     //  * 256: a round of up to one tile per CU about 37 (64 of them 27);
     //  * 128: 10 and 11 for each 256 of them (64 of them 9.8, 240 13.3, 1024 45);
     //  * 64, several on a CU: 3 and 3.9 for each 256 (256 of them 6.8, 960 19.2),
-    //    so 128 from half as many tiles as CUs;
+    //    so 128 from half as many tiles as CUs.  By tiles alone, this misses with
+    //    B [K, N], whose rows a 64 tile takes in 128-byte pieces: 225x1024x5000
+    //    18.0 us (on 128 10.2), 282x8256x4128 92.7 (74.8), at short K the other
+    //    way (3389x64x686 8.8, on 64 6.6); within 2% on average with B [N, K];
     //  * 32x64 up to 32 rows (16x4096x4096 10.1, on 64s 10.5; x8192 18.7 / 20.6).
     const size_t t256 = tiles(256, 256), t128 = tiles(128, 128);
     const double c256 = 3.4 * static_cast<double>((t256 + cus - 1) / cus), c128 = 1.0 + static_cast<double>(t128) / cus;

@@ -1,17 +1,17 @@
 // Layer products of one to a few rows with the weight stored [N, K], bound by
 // the one read of the weight.
 //  * one row (two of 16 bits): a wave reads whole rows of the weight, 1 KiB per
-//    load, and multiplies on the vector units (1x4096x8192 bf16 14.9 us; the
-//    form below 16.6, the ring 17.0);
+//    load, and multiplies on the vector units (1x4096x8192 bf16 13.2 us; the
+//    form below 15.3, the ring 14.2; two rows 14.5, 15.8 and 14.0);
 //  * up to 16 rows by a weight of up to 8 MiB: the weight goes straight from
 //    memory to the matrix cores' registers as the MFMA's row operand (16
 //    outputs n per 16x16 step) and the rows of x are its columns; the waves of
 //    a workgroup share K and meet in LDS in wave order; K is split over
 //    workgroups too, the last one of a tile adding the splits in their order
-//    (16x1024x4096 bf16 5.5 us, the ring 5.8; larger weights are the ring's:
-//    16x4096x4096 12.3 and 10.1, as every lane's row of x is read with each step).
+//    (16x1024x4096 bf16 5.1 us, the ring 5.6; larger weights are the ring's:
+//    16x4096x4096 17.4 and 10.4, as every lane's row of x is read with each step).
 // Rows past the end re-read the last one; what is not the tile's is not
-// stored.  Non-temporal loads of the weight were slower (15.7 against 14.9 us).
+// stored.  Non-temporal loads of the weight were slower (13.9 against 13.2 us).
 #include "gemm16.hpp"
 #include "linear.hpp"
 #include "linear_act.hpp"
@@ -199,7 +199,7 @@ __global__ __launch_bounds__(kSW *kWave) void k_linear_rows(SkinnyArgs a) {
 
 // One or two rows: a wave takes kDotRows rows of the weight whole.
 constexpr int kDotRows = 2, kDotDepth = 4;
-// (two rows of e4m3 take the matrix cores: 8192x8192 20.3 us here, 17.7 there)
+// (two rows of e4m3 take the ring: 8192x8192 17.9 us here, 14.3 there)
 inline bool dot_takes(size_t M, size_t kb, int dtype) {
     return kb >= 16 && (M == 1 || (M == 2 && dtype != CXM_DT_E4M3));
 }

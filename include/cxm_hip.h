@@ -15,7 +15,8 @@
  * Engine/CUDA/matrix.cuh:11-26: no op allocates its output).  Multi-pass
  * kernels take their scratch from a per-(device, stream) workspace that the
  * library allocates on first use and keeps until cxm_release_workspaces();
- * calls on distinct streams are independent, calls on one stream are ordered.
+ * calls on distinct streams are independent, calls on one stream are ordered
+ * and come from one host thread at a time.
  *
  * Reference paths below are relative to source/CortexMind/framework/.
  */

@@ -152,18 +152,14 @@ __device__ __forceinline__ void unpack_e4m3(unsigned w, float *v) {
 
 constexpr float kE4M3Max = 448.0f;
 
-// Scale of values whose largest magnitude is `amax`, amax / 448 rounded to
-// nearest, and its reciprocal; 0 and 0 where that is no normal float; NaN and
-// infinity stay.  The quotient is amax times the rounded 1 / 448 and one
-// correction by the exact remainder: equal to the division for every float, in
-// a third of its instructions (the product alone is one off for half of them).
+// Scale of values whose largest magnitude is `amax`, and its reciprocal:
+// amax times the rounded 1 / 448 (the largest is held as 448, within an fp32
+// rounding), or 0 and 0 where that is no normal float; NaN and infinity stay.
 struct Scale8 {
     float scale, inv;
 };
 __device__ __forceinline__ Scale8 scale_e4m3(float amax) {
-    constexpr float r = 1.0f / kE4M3Max;
-    const float q = amax * r;
-    const float s = q <= FLT_MAX ? fmaf(fmaf(-kE4M3Max, q, amax), r, q) : q;
+    const float s = amax * (1.0f / kE4M3Max);
     if (s < FLT_MIN) return {0.0f, 0.0f};
     return {s, 1.0f / s};
 }

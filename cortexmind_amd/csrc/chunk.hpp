@@ -154,7 +154,9 @@ constexpr float kE4M3Max = 448.0f;
 
 // Scale of values whose largest magnitude is `amax`, and its reciprocal:
 // amax times the rounded 1 / 448 (the largest is held as 448, within an fp32
-// rounding), or 0 and 0 where that is no normal float; NaN and infinity stay.
+// rounding; the correctly rounded amax / 448 is one away for half of all values,
+// an error of 2^-24 beside the codes' 2^-4), or 0 and 0 where that is no normal
+// float; NaN and infinity stay.
 struct Scale8 {
     float scale, inv;
 };

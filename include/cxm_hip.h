@@ -442,10 +442,11 @@ int cxm_sgd_f32(float *w, const float *g, float lr, size_t n, cxm_stream_t s);
  *   h = x + res, rounded to the type (res NULL: h = x),
  *   rstd = 1 / sqrt(mean(h*h) + eps), y = h * rstd * w.
  * Each output may be NULL, but y or q is given: h [rows, cols] (needs res);
- * y; q and scale, the rows of y in 8 bits (E4M3): scale[r] = max|y| / 448 and
- * q = y / scale rounded to nearest even (a row whose scale is no normal
- * float: scale 0 and zeros; a row with a NaN or an infinity has a NaN or
- * infinite scale); rstd [rows], for the backward.  w has the rows' type; sums
+ * y; q and scale, the rows of y in 8 bits (E4M3): scale[r] = max|y| * (1 / 448)
+ * and q = y * (1 / scale), every reciprocal and product rounded to fp32, q then
+ * to nearest even (a row whose scale is no normal float: scale 0 and zeros; a
+ * row with a NaN or an infinity has a NaN or infinite scale); rstd [rows], for
+ * the backward.  w has the rows' type; sums
  * are fp32.  h and y may each be x or res itself; any other overlap of an
  * output with an input or another output is CXM_E_INVALID.  rows == 0 does
  * nothing; cols == 0 is CXM_E_INVALID. */
@@ -508,8 +509,9 @@ int cxm_linear_q8_fwd(const uint8_t *x, const float *x_scale, const uint8_t *w, 
  * state_dtype CXM_DT_F32: m and v are fp32, zero before the first step.
  * state_dtype CXM_DT_E4M3: m and v hold m and sqrt(v) in 8 bits, value i
  * times m_scale[i / 256] (v_scale[i / 256]); all zero before the first step.
- * The scale is a block's largest finite magnitude / 448.  Rounding is to the
- * neighbour above with the probability of the distance to the one below
+ * The scale is a block's largest finite magnitude times 1 / 448, as a row's in
+ * cxm_rmsnorm_fwd_t.  Rounding (of the value times the scale's fp32 reciprocal)
+ * is to the neighbour above with the probability of the distance to the one below
  * (towards the larger magnitude; a root above zero never becomes zero),
  * decided by 16 of 32 random bits, the low ones for m: with c the value's
  * number (i plus 256 times the blocks of the tensors before it) and key =

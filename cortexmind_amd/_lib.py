@@ -130,6 +130,14 @@ SIGNATURES = {
     "cxm_rmsnorm_fwd_t": [_P, _P, _P, _F, _P, _P, _P, _P, _P, _SZ, _SZ, _I, _P],
     "cxm_rmsnorm_bwd_t": [_P, _P, _P, _P, _P, _P, _P, _SZ, _SZ, _I, _P],
     "cxm_quant_rows_t": [_P, _P, _P, _SZ, _SZ, _I, _P],
+    "cxm_layernorm_fwd_t": [_P, _P, _P, _P, _F, _P, _P, _P, _P, _P, _P, _SZ, _SZ, _I, _P],
+    "cxm_layernorm_bwd_t": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _SZ, _I, _P],
+    "cxm_embedding_fwd_t": [_P, _P, _F, _P, _SZ, _SZ, _SZ, _I, _P],
+    "cxm_embedding_bwd_t": [_P, _P, _F, _P, _I, _SZ, _SZ, _SZ, _I, _I, _P],
+    "cxm_logprob_fwd_t": [_P, _SZ, _P, _F, _P, _P, _P, _P, _P, _SZ, _SZ, _SZ, _I, _P],
+    "cxm_logprob_bwd_t": [_P, _SZ, _P, _F, _P, _P, _P, _P, _P, _SZ, _SZ, _SZ, _I, _P],
+    "cxm_distill_fwd_t": [_P, _SZ, _P, _P, _SZ, _F, _P, _P, _SZ, _SZ, _I, _P],
+    "cxm_distill_bwd_t": [_P, _SZ, _P, _P, _SZ, _F, _P, _P, _P, _SZ, _SZ, _SZ, _I, _P],
     "cxm_linear_fwd_t": [_P, _P, _P, _P, _P, _P, _SZ, _SZ, _SZ, _I, _I, _I, _P],
     "cxm_linear_bwd_t": [_P, _P, _P, _P, _P, _P, _P, _P, _SZ, _SZ, _SZ, _I, _I, _I, _P],
     "cxm_linear_q8_fwd": [_P, _P, _P, _P, _P, _P, _P, _P, _SZ, _SZ, _SZ, _I, _I, _P],

@@ -176,6 +176,9 @@ constexpr size_t most_wgs(size_t threads) { return 0xffffffffu / threads; }
 // out[j] = sum of part[i][j] over i < n (rows `ld` floats apart), rounded to
 // `dtype`; the order is fixed (colsum.hip).
 int col_sum(const float *part, size_t n, size_t cols, size_t ld, void *out, int dtype, hipStream_t s);
+// The same, and out2[j] (null: none) of the columns that lie `second` floats on.
+int col_sum2(const float *part, size_t n, size_t cols, size_t ld, void *out, size_t second, void *out2, int dtype,
+             hipStream_t s);
 
 // Whether [a, a + an) and [b, b + bn) share a byte (null or empty: no).
 inline bool overlap(const void *a, size_t an, const void *b, size_t bn) {

@@ -13,7 +13,7 @@
 // belongs to 16 or 64 lanes of a wave or to a whole workgroup, so that a
 // lane holds one to four chunks of 16 bytes; rows beyond that are read twice
 // (the second time mostly from L2).  All sums are fp32.
-#include "chunk.hpp"
+#include "norm.hpp"
 
 namespace cxm {
 namespace {
@@ -38,50 +38,8 @@ struct RmsBwd {
     unsigned cols, ld;
 };
 
-// Largest magnitude, NaN if any is NaN.
-struct AmaxOp : MaxOp {
-    __device__ static T identity() { return 0.0f; }
-};
-
-template <bool ONCE, int DT, int VE>
-__device__ __forceinline__ void load_once(Chunk<DT, VE> &c, const typename Elem<DT>::S *p) {
-    if constexpr (ONCE) c.load_nt(p);
-    else c.load(p);
-}
-
-template <class Op, int G, int NT>
-__device__ __forceinline__ float row_reduce(float v, float *lds) {
-    if constexpr (G <= kWave) return group_reduce<Op, G>(v);
-    else return block_reduce<Op, NT>(v, lds);
-}
-
 __device__ __forceinline__ float rms_rstd(float ss, unsigned cols, float eps) {
     return 1.0f / __builtin_sqrtf(ss / static_cast<float>(cols) + eps);
-}
-
-// Eight (four, one) e4m3 bytes of a chunk's own elements.
-template <int VE>
-__device__ __forceinline__ void store_q(uint8_t *row, Span s, const float (&v)[VE], float inv) {
-    float t[VE];
-#pragma unroll
-    for (int e = 0; e < VE; ++e) t[e] = v[e] * inv;
-    if constexpr (VE == 1) {
-        if (s.dup == 0) row[s.off] = static_cast<uint8_t>(pack_e4m3(t[0], 0.0f, 0.0f, 0.0f));
-    } else {
-        unsigned w[VE / 4];
-#pragma unroll
-        for (int i = 0; i < VE / 4; ++i) w[i] = pack_e4m3(t[4 * i], t[4 * i + 1], t[4 * i + 2], t[4 * i + 3]);
-        if (s.dup == 0) {
-            typedef unsigned u32b __attribute__((aligned(1)));
-            typedef unsigned u32x2b __attribute__((ext_vector_type(2), aligned(1)));
-            if constexpr (VE == 8) *reinterpret_cast<u32x2b *>(row + s.off) = u32x2b{w[0], w[1]};
-            else *reinterpret_cast<u32b *>(row + s.off) = w[0];
-        } else if (s.dup < VE) {
-#pragma unroll
-            for (int e = 1; e < VE; ++e)
-                if (e >= static_cast<int>(s.dup)) row[s.off + e] = static_cast<uint8_t>(w[e / 4] >> (8 * (e & 3)));
-        }
-    }
 }
 
 // G lanes per row, C chunks of VE elements per lane, NT threads.  AL: rows of
@@ -554,13 +512,6 @@ __global__ __launch_bounds__(kBlock) void k_rms_dw_part(RmsBwd a) {
 
 // ----------------------------------------------------------------- launch
 
-inline hipStream_t hs(cxm_stream_t s) { return reinterpret_cast<hipStream_t>(s); }
-
-// Rows of whole 128-byte lines (null: yes).
-inline bool whole_lines(const void *p, size_t cols, size_t bytes) {
-    return (reinterpret_cast<uintptr_t>(p) | cols * bytes) % 128 == 0;
-}
-
 template <int DT, int VE, int G, int C, int NT>
 int fwd_launch(const RmsFwd &a, hipStream_t s) {
     constexpr int R = G <= kWave ? NT / G : 1;
@@ -599,13 +550,6 @@ int fwd_any(const RmsFwd &a, int dtype, hipStream_t s) {
         case CXM_DT_BF16: return fwd_dispatch<CXM_DT_BF16>(a, s);
         default: return fwd_dispatch<CXM_DT_F16>(a, s);
     }
-}
-
-// Workgroups of the backward: enough to fill the chip, few enough that their
-// shares of dw are a small part of the traffic.
-size_t bwd_wgs(size_t rows, int per_wg) {
-    const size_t need = (rows + per_wg - 1) / per_wg, most = device_cus() * 2;
-    return need < most ? need : most;
 }
 
 int bwd_parts(RmsBwd *a, size_t parts, cxm_stream_t st) {
@@ -676,11 +620,6 @@ int bwd_dispatch(RmsBwd a, void *dw, cxm_stream_t st) {
     if (r) return r;
     hipLaunchKernelGGL((k_rms_bwd_long<DT, 1024>), dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, hs(st), a);
     return launch_status();
-}
-
-// Row lengths stay below 2^31, so that an element's place in its row is 32 bits.
-bool row_shape_ok(size_t rows, size_t cols) {
-    return cols < (size_t(1) << 31) && (rows == 0 || cols == 0 || rows <= (size_t(1) << 46) / cols);
 }
 
 }  // namespace

@@ -337,6 +337,82 @@ class rmsnorm:
         call("cxm_rmsnorm_bwd_t", _p(H), _p(rstd), _p(W), _p(dY), _p(dH), _p(dX), _p(dW), rows, cols, dtype, _s(stream))
 
 
+class layernorm:
+    """Layer norm of rows with the residual's addition, forward
+    (cxm_layernorm_fwd_t) and backward (cxm_layernorm_bwd_t), for a DT_* dtype."""
+
+    @staticmethod
+    def forward(X, W, Y, rows, cols, dtype, bias=None, eps=1e-5, residual=None, H=None, Q=None, scale=None, mean=None,
+                rstd=None, stream=None):
+        """H = X + residual, Y = norm(H) * W + bias; Q and scale: Y's rows in 8
+        bits (Y may then be None); mean and rstd are what the backward reads."""
+        call("cxm_layernorm_fwd_t", _p(X), _p(residual), _p(W), _p(bias), float(eps), _p(H), _p(Y), _p(Q), _p(scale),
+             _p(mean), _p(rstd), rows, cols, dtype, _s(stream))
+
+    @staticmethod
+    def backward(H, mean, rstd, W, dY, dX, dW, rows, cols, dtype, db=None, dH=None, stream=None):
+        """dX: the gradient of X and of the residual, dH (what reaches H past
+        the norm) included."""
+        call("cxm_layernorm_bwd_t", _p(H), _p(mean), _p(rstd), _p(W), _p(dY), _p(dH), _p(dX), _p(dW), _p(db), rows, cols,
+             dtype, _s(stream))
+
+
+class embedding:
+    """Rows of a table looked up by token (int32; negative: padding) and
+    scaled (cxm_embedding_fwd_t), and the table's gradient (cxm_embedding_bwd_t)."""
+
+    @staticmethod
+    def forward(table, ids, Y, tokens, vocab, cols, dtype, scale=1.0, stream=None):
+        call("cxm_embedding_fwd_t", _p(table), _p(ids), float(scale), _p(Y), tokens, vocab, cols, dtype, _s(stream))
+
+    @staticmethod
+    def backward(ids, dY, dW, tokens, vocab, cols, dtype, scale=1.0, g_dtype=None, accumulate=False, stream=None):
+        """dW, of g_dtype (default: dtype), is written whole, or with
+        accumulate added to where a token names its row."""
+        call("cxm_embedding_bwd_t", _p(ids), _p(dY), float(scale), _p(dW), int(bool(accumulate)), tokens, vocab, cols,
+             dtype, dtype if g_dtype is None else g_dtype, _s(stream))
+
+
+class logprob:
+    """Log probabilities of given tokens (int32; negative: padding) under
+    softmax(scale * logits), with the entropy and the top tokens
+    (cxm_logprob_fwd_t), and the logits' gradient (cxm_logprob_bwd_t).  Rows of
+    logits lie ld elements apart (default: vocab)."""
+
+    @staticmethod
+    def forward(logits, tokens, logp, rows, vocab, dtype, scale=1.0, ld=None, entropy=None, lse=None, top=0, top_logp=None,
+                top_ids=None, stream=None):
+        """lse is what the backward reads; top: how many alternatives."""
+        call("cxm_logprob_fwd_t", _p(logits), vocab if ld is None else ld, _p(tokens), float(scale), _p(logp), _p(entropy),
+             _p(lse), _p(top_logp), _p(top_ids), top, rows, vocab, dtype, _s(stream))
+
+    @staticmethod
+    def backward(logits, tokens, lse, dlogp, dlogits, rows, vocab, dtype, scale=1.0, ld=None, ld_d=None, entropy=None,
+                 dentropy=None, stream=None):
+        """dlogits: rows ld_d elements apart (default: vocab), or logits itself
+        (with ld_d = ld)."""
+        call("cxm_logprob_bwd_t", _p(logits), vocab if ld is None else ld, _p(tokens), float(scale), _p(lse), _p(entropy),
+             _p(dlogp), _p(dentropy), _p(dlogits), vocab if ld_d is None else ld_d, rows, vocab, dtype, _s(stream))
+
+
+class distill:
+    """Divergence of softmax(scale * logits) from a teacher's distribution
+    over its k top tokens, softmax(scale * teacher) (cxm_distill_fwd_t), and the
+    logits' gradient (cxm_distill_bwd_t).  ids: int32 [rows, k] (negative: no
+    entry), teacher: float32 [rows, k]."""
+
+    @staticmethod
+    def forward(logits, ids, teacher, loss, lse, rows, vocab, k, dtype, scale=1.0, ld=None, stream=None):
+        call("cxm_distill_fwd_t", _p(logits), vocab if ld is None else ld, _p(ids), _p(teacher), k, float(scale), _p(loss),
+             _p(lse), rows, vocab, dtype, _s(stream))
+
+    @staticmethod
+    def backward(logits, ids, teacher, lse, dloss, dlogits, rows, vocab, k, dtype, scale=1.0, ld=None, ld_d=None,
+                 stream=None):
+        call("cxm_distill_bwd_t", _p(logits), vocab if ld is None else ld, _p(ids), _p(teacher), k, float(scale), _p(lse),
+             _p(dloss), _p(dlogits), vocab if ld_d is None else ld_d, rows, vocab, dtype, _s(stream))
+
+
 class quant:
     """Rows in 8 bits (e4m3) with a scale each."""
 

@@ -465,6 +465,49 @@ int cxm_rmsnorm_bwd_t(const void *h, const float *rstd, const void *w, const voi
  * reach it without a norm. */
 int cxm_quant_rows_t(const void *x, uint8_t *q, float *scale, size_t rows, size_t cols, int dtype, cxm_stream_t s);
 
+/* ---------------------------------------------------------- layer norm
+ * The rows of [rows, cols] less their mean, by their deviation, with the
+ * residual's addition before it; beside cxm_rmsnorm_*, with its types, rules of
+ * overlap and 8-bit rows.  No reference counterpart; it is the composition
+ * matrix_t::add, reduce::mean, Broadcast::col::sub, reduce::var,
+ * Broadcast::col::mul and Broadcast::row::{mul,add}:
+ *   h = x + res, rounded to the type (res NULL: h = x),
+ *   rstd = 1 / sqrt(mean((h - mean)^2) + eps), y = (h - mean) * rstd * w + bias.
+ * bias may be NULL (none), and each output but one of y and q: h [rows, cols]
+ * (needs res); y; q and scale; mean and rstd [rows], for the backward. */
+int cxm_layernorm_fwd_t(const void *x, const void *res, const void *w, const void *bias, float eps, void *h, void *y,
+                        uint8_t *q, float *scale, float *mean, float *rstd, size_t rows, size_t cols, int dtype,
+                        cxm_stream_t s);
+/* Backward from h, mean and rstd of the forward: with n = (h - mean) * rstd and
+ * g = dy * w, dx = rstd * (g - mean(g) - n * mean(g * n)) + dh, where dh (or
+ * NULL) is the gradient that reaches h past the norm; dx is the gradient of x
+ * and of res.  dw[j] = sum over rows of dy * n and db[j] = sum over rows of dy (db
+ * may be NULL), summed in fp32 in a fixed order.  dx may be h, dy or dh itself.
+ * rows == 0 gives dw = db = 0.  cols < 2^26.  Needs scratch (see
+ * CXM_E_CAPTURE). */
+int cxm_layernorm_bwd_t(const void *h, const float *mean, const float *rstd, const void *w, const void *dy,
+                        const void *dh, void *dx, void *dw, void *db, size_t rows, size_t cols, int dtype,
+                        cxm_stream_t s);
+
+/* ----------------------------------------------------------- embedding
+ * Rows of a table [vocab, cols] looked up by token and scaled, beside
+ * cxm_gather_f32: y[t] = table[ids[t]] * scale, rounded once.  A negative id is
+ * padding, a row of zeros; an id of vocab or more gives a row of NaN.  y must
+ * not overlap the table or the ids; tokens, vocab and cols < 2^31; a scale that
+ * is not finite, vocab == 0 or cols == 0 is CXM_E_INVALID; tokens == 0 does
+ * nothing.  No reference counterpart (wise::gather and ScalarOp::mul). */
+int cxm_embedding_fwd_t(const void *table, const int32_t *ids, float scale, void *y, size_t tokens, size_t vocab,
+                        size_t cols, int dtype, cxm_stream_t s);
+/* The table's gradient: dw[v] = scale * sum over t with ids[t] == v of dy[t], in
+ * fp32 in a fixed order, rounded once; zeros where no token is v.  With
+ * `accumulate` (1) dw[v] is added to that before the rounding, and rows that no
+ * token has stay as they are (a table that is also a layer's weight).  Ids
+ * outside [0, vocab) take no part.  dy is of `dtype`, dw of `g_dtype`: `dtype`
+ * or CXM_DT_F32.  Needs scratch (see CXM_E_CAPTURE): 8 bytes a token, 4 an id,
+ * and sums of a share of the tokens. */
+int cxm_embedding_bwd_t(const int32_t *ids, const void *dy, float scale, void *dw, int accumulate, size_t tokens,
+                        size_t vocab, size_t cols, int dtype, int g_dtype, cxm_stream_t s);
+
 /* --------------------------------------------------------- dense layer
  * z = x w + bias, y = act(z) + res over x [m, k], w [k, n] ([n, k] with
  * trans_w), bias [n], res / z / y [m, n], all of `dtype` (CXM_DT_F32 / BF16 /
@@ -498,6 +541,60 @@ int cxm_linear_bwd_t(const void *x, const void *w, const void *z, const void *dy
 int cxm_linear_q8_fwd(const uint8_t *x, const float *x_scale, const uint8_t *w, const float *w_scale, const void *bias,
                       const void *res, void *z, void *y, size_t m, size_t k, size_t n, int act, int dtype,
                       cxm_stream_t s);
+
+/* --------------------------------------------- log probabilities of tokens
+ * What logits [rows, vocab] of `dtype`, rows ld >= vocab elements apart, say
+ * under softmax(scale * logits), scale > 0 and finite; beside cxm_softmax_* and
+ * cxm_softmax_xent_f32.  Logits are read once.  All results are fp32, and each
+ * may be NULL (but not all):
+ *   lse[r]     log of the sum of exp(scale * logits[r]), for the backward;
+ *   logp[r]    log probability of tokens[r]; 0 where that is negative
+ *              (padding), NaN where it is vocab or more;
+ *   entropy[r] of the row's distribution;
+ *   top_ids, top_logp [rows, top]: the `top` (0 to 64, at most vocab) largest
+ *              logits, largest first, of equal ones (+0 and -0 are) the lowest id,
+ *              and their log probabilities.
+ * A logit of -inf has probability 0.  A row of -inf alone has lse -inf and NaN
+ * elsewhere; a row with a NaN has NaN everywhere and top_ids of -1; +inf gives
+ * NaN.  A row of the type's lowest value alone is a row of equal logits.
+ * Outputs overlap nothing.  rows < 2^24, rows * segments (16384 16-bit or 8192
+ * fp32 elements each, fewer in few rows) too, else CXM_E_TOO_LARGE.  Rows cut
+ * into segments need scratch (see CXM_E_CAPTURE). */
+int cxm_logprob_fwd_t(const void *logits, size_t ld, const int32_t *tokens, float scale, float *logp, float *entropy,
+                      float *lse, float *top_logp, int32_t *top_ids, size_t top, size_t rows, size_t vocab, int dtype,
+                      cxm_stream_t s);
+/* The logits' gradient, [rows, vocab] with rows ldd >= vocab elements apart, of
+ * `dtype`, from those of logp and of the entropy (either may be NULL), with p =
+ * exp(scale * logits - lse):
+ *   dlogits[j] = scale * (dlogp ([j == token] - p[j])
+ *                         - dentropy p[j] (log p[j] + entropy)).
+ * entropy, the forward's, is read with dentropy only.  A negative token takes no
+ * part, one of vocab or more makes the row NaN.  Where dlogp (or the token's
+ * part in it) and dentropy are 0 the row is zeros whatever the logits and lse
+ * are.  dlogits may be logits itself (ldd == ld); any other overlap is
+ * CXM_E_INVALID.  What lies past vocab in a row stays as it is. */
+int cxm_logprob_bwd_t(const void *logits, size_t ld, const int32_t *tokens, float scale, const float *lse,
+                      const float *entropy, const float *dlogp, const float *dentropy, void *dlogits, size_t ldd,
+                      size_t rows, size_t vocab, int dtype, cxm_stream_t s);
+
+/* --------------------------------------------------------- distillation
+ * Divergence of a model's distribution from a teacher's over the teacher's top
+ * tokens.  ids and teacher [rows, k], k from 1 to 256: the tokens' ids and their
+ * logits or log probabilities (as top_ids and top_logp above give them with
+ * scale 1); a negative id is no entry.  With q = softmax(scale * teacher) over a
+ * row's entries and p = softmax(scale * logits) over the vocabulary:
+ *   loss[r] = sum over entries of q (log q - log p[id]), lse as above (or NULL).
+ * An entry of -inf has q = 0; a row without an entry of q > 0 has loss 0; an id
+ * of vocab or more makes the loss NaN.  Entries may share an id.  Logits, sizes
+ * and scratch as above. */
+int cxm_distill_fwd_t(const void *logits, size_t ld, const int32_t *ids, const float *teacher, size_t k, float scale,
+                      float *loss, float *lse, size_t rows, size_t vocab, int dtype, cxm_stream_t s);
+/* The logits' gradient: dlogits[j] = dloss[r] * scale * (p[j] - sum of q over
+ * the entries with id j); zeros where dloss is 0 or the row has no entry of q > 0,
+ * NaN where an id is vocab or more.  dlogits may be logits itself (ldd == ld). */
+int cxm_distill_bwd_t(const void *logits, size_t ld, const int32_t *ids, const float *teacher, size_t k, float scale,
+                      const float *lse, const float *dloss, void *dlogits, size_t ldd, size_t rows, size_t vocab,
+                      int dtype, cxm_stream_t s);
 
 /* --------------------------------------------------------------- AdamW
  * One step over all tensors of a model in one launch (beside cxm_sgd_f32):

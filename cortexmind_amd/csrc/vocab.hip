@@ -55,28 +55,89 @@ struct Logits {
     size_t ld, rows;
     unsigned vocab, nseg, seglen;  // seglen: a multiple of 64
     float scale, c;                // c = scale log2(e)
+    unsigned odd;                  // 1: some row's chunks begin an element earlier (shift_of)
 };
-// A segment's chunk that begins at column col: moved back to the segment's last
-// VE elements where it reaches past its end (which may lie before the segment:
-// never before the row).
+// A chunk's place in its row, and which of its elements are its own: lo <= e < hi.
+struct Own {
+    unsigned off;
+    int lo, hi;
+    __device__ bool has(int e) const { return e >= lo && e < hi; }
+};
+// The chunk at column col - shift of a row, in a segment that ends at column
+// end: moved back to the segment's last VE elements where it reaches past its
+// end (which may lie before the segment), and on to the row's first where it
+// begins before it.
 template <int VE>
-__device__ __forceinline__ Span seg_span(unsigned col, unsigned end) {
-    const unsigned last = end - VE, off = col < last ? col : last;
-    return {off, col - off};
+__device__ __forceinline__ Own own_of(unsigned col, unsigned shift, unsigned end) {
+    const int c = static_cast<int>(col - shift), last = static_cast<int>(end) - VE;
+    int off = c < last ? c : last;
+    off = off > 0 ? off : 0;
+    return {static_cast<unsigned>(off), c - off, c < 0 ? c + VE : VE};
 }
-// The first `dup` elements become -infinity.
+// 1 for 16-bit rows that begin between two dwords: their chunks then begin an
+// element earlier, at a dword (2500 fp16 rows of 50001 took 55 us at any element's
+// address, of 50002 45).
 template <int DT, int VE>
-__device__ __forceinline__ void drop_dup(Chunk<DT, VE> &c, unsigned dup) {
-    if (dup == 0) return;
+__device__ __forceinline__ unsigned shift_of(const void *row) {
+    return DT == CXM_DT_F32 || VE == 1 ? 0u : static_cast<unsigned>(reinterpret_cast<uintptr_t>(row) >> 1 & 1);
+}
+// The elements that are not the chunk's own become -infinity.
+template <int DT, int VE>
+__device__ __forceinline__ void drop_others(Chunk<DT, VE> &c, Own o) {
+    if (o.lo <= 0 && o.hi == VE) return;
     if constexpr (DT == CXM_DT_F32) {
 #pragma unroll
-        for (int e = 0; e < VE; ++e) c.r[e] = e < static_cast<int>(dup) ? -INFINITY : c.r[e];
+        for (int e = 0; e < VE; ++e) c.r[e] = o.has(e) ? c.r[e] : -INFINITY;
     } else {
         constexpr unsigned inf = DT == CXM_DT_BF16 ? 0xff80u : 0xfc00u;
 #pragma unroll
         for (int e = 0; e < VE; ++e)
-            if (e < static_cast<int>(dup)) c.r[e / 2] = e & 1 ? (c.r[e / 2] & 0xffffu) | inf << 16 : (c.r[e / 2] & 0xffff0000u) | inf;
+            if (!o.has(e)) c.r[e / 2] = e & 1 ? (c.r[e / 2] & 0xffffu) | inf << 16 : (c.r[e / 2] & 0xffff0000u) | inf;
     }
+}
+// Stores a chunk's own elements.
+template <int DT, int VE>
+__device__ __forceinline__ void store_own(typename Elem<DT>::S *row, Own o, const Chunk<DT, VE> &c) {
+    if (o.lo <= 0 && o.hi == VE) {
+        c.store(row + o.off);
+    } else {
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+            if (o.has(e)) row[o.off + e] = c.raw(e);
+    }
+}
+// A segment of a row: its chunks begin at columns s0 - shift, s0 - shift + VE, ...
+struct Seg {
+    unsigned s0, end, shift;
+    int its;  // chunks that some lane of this wave has, G lanes' VE elements apart
+    __device__ unsigned begin() const { return s0 < shift ? 0 : s0 - shift; }
+    template <int VE, int G>
+    __device__ Own own(int i, unsigned lane) const {
+        return own_of<VE>(s0 + (i * G + lane) * VE, shift, end);
+    }
+};
+template <int DT, int VE, int G>
+__device__ __forceinline__ Seg seg_of(const Logits &in, const void *row, unsigned number, unsigned lane) {
+    Seg s;
+    s.shift = shift_of<DT, VE>(row);
+    s.s0 = number * in.seglen;
+    const unsigned all = in.vocab + s.shift, to = all - s.s0 < in.seglen ? all : s.s0 + in.seglen;
+    s.end = to - s.shift;
+    const unsigned first = s.s0 + (__builtin_amdgcn_readfirstlane(lane / kWave) * kWave) * VE;
+    s.its = first >= to ? 0 : static_cast<int>((to - first + G * VE - 1) / (G * VE));
+    return s;
+}
+
+// The same value, which the compiler takes for a new one: what is computed from it
+// is computed anew and not kept in registers (64 unpacked values, 64 masks) from
+// one pass over a lane's chunks to the next.
+__device__ __forceinline__ unsigned again(unsigned v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+template <int DT, int VE>
+__device__ __forceinline__ void again(Chunk<DT, VE> &c) {
+    for (auto &r : c.r) asm volatile("" : "+v"(r));
 }
 
 // Barrier of G threads: a workgroup's, or a wave's own LDS accesses in order.
@@ -108,7 +169,9 @@ struct StatArgs {
     int kind;
     // segments
     Part *parts;      // [rows, nseg]
-    ArgPair *cands;   // [rows, nseg, top]
+    ArgPair *cands;   // [rows, nseg, keep]
+    float *bars;      // [rows, nseg, 2]: a value that `top` of the segment's tokens are not below, the largest
+    unsigned keep;    // tokens a segment hands on, its `top` among them
     unsigned *tickets;
 };
 
@@ -120,20 +183,98 @@ __device__ __forceinline__ float value_of(unsigned key) {
     return __builtin_bit_cast(float, key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
 
+// Bits of a 32-bit value that its type can have set: the others are all alike.
+template <int DT>
+constexpr int kLowBit = DT == CXM_DT_F32 ? 0 : DT == CXM_DT_BF16 ? 16 : 13;
+// A value's bits, ascending in the value's order; zeros alike.
+__device__ __forceinline__ unsigned key_of(float v) {
+    const unsigned u = __builtin_bit_cast(unsigned, v + 0.0f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// A value that at least `n` of a wave's 64 J values are not below: the n-th
+// largest, bit by bit, or less, where those not below it are at most `most`.
+template <int DT, int J>
+__device__ __forceinline__ float threshold(const float (&v)[J], unsigned n, unsigned most) {
+    unsigned k[J], key = 0;
+#pragma unroll
+    for (int j = 0; j < J; ++j) k[j] = key_of(v[j]);
+#pragma nounroll
+    for (int b = 31; b >= kLowBit<DT>; --b) {
+        const unsigned t = key | 1u << b;
+        unsigned c = 0;
+#pragma unroll
+        for (int j = 0; j < J; ++j) c += __popcll(__ballot(k[j] >= t));
+        if (c >= n) {
+            key = t;
+            if (c <= most) break;
+        }
+    }
+    // (a negative value whose last bits are open stands for the lowest that begins so: nothing is lost)
+    return key < 0x007fffffu ? -INFINITY : value_of(key);
+}
+
+// Chunk number i of a lane's, i known only when it runs: a few selections, where
+// an indexed register array would go through memory, and loops over i stay small
+// (the top tokens' code was 65 KB with all of them unrolled, past the instruction
+// cache).
+template <int DT, int VE, int C>
+__device__ __forceinline__ Chunk<DT, VE> pick(const Chunk<DT, VE> (&c)[C], int i) {
+    Chunk<DT, VE> r = c[0];
+#pragma unroll
+    for (int k = 1; k < C; ++k)
+#pragma unroll
+        for (int w = 0; w < static_cast<int>(sizeof(r.r) / sizeof(r.r[0])); ++w) r.r[w] = i == k ? c[k].r[w] : r.r[w];
+    return r;
+}
+
 // LDS of a group.
 struct Room {
-    ArgPair *list, *best;  // kList and kTopMost entries
+    ArgPair *list, *best;  // room for kCap<G> and kTopMost tokens
     int *count;
+    float *bar;
 };
-constexpr unsigned kList = 512;
-
-// Sorts list[0 .. n) (n <= kList) and keeps the first min(n, top) in it, in order.
 template <int G>
+constexpr unsigned kCap = G == kBlock ? 512 : 128;
+
+// Room for one more token in the list (the place may lie past it).  Each lane
+// for itself: few have any, and the compiler's joint form is long.
+__device__ __forceinline__ unsigned next_place(const Room &r) { return atomicAdd(r.count + again(0u), 1); }
+
+// Sorts list[0 .. n) and keeps the first min(n, top) in it, in order: each
+// token's place is the number of better ones.  Where there are many more than
+// `top`, those below a value that `top` are not below leave first (512 tokens
+// ranked among each other took 20 us).
+template <int DT, int G>
 __device__ __forceinline__ unsigned keep_top(const Room &r, unsigned n, unsigned top, unsigned lane) {
     group_sync<G>();
+    if (n > top + top / 4 + 8) {
+        constexpr int J = kCap<G> / kWave, E = kCap<G> / G;
+        if (G != kBlock || lane < kWave) {
+            float v[J];
+#pragma unroll
+            for (int j = 0; j < J; ++j) v[j] = j * kWave + lane < n ? r.list[j * kWave + lane].v : -INFINITY;
+            const float t = threshold<DT, J>(v, top, top + top / 8);
+            if (lane == 0) {
+                *r.bar = t;
+                *r.count = 0;
+            }
+        }
+        ArgPair mine[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) mine[e] = r.list[e * G + lane];  // (past n: not looked at)
+        group_sync<G>();
+        const float t = *r.bar;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (e * G + lane < n && mine[e].v >= t) r.list[next_place(r)] = mine[e];
+        group_sync<G>();
+        n = *r.count;
+    }
     for (unsigned i = lane; i < n; i += G) {
         const ArgPair mine = r.list[i];
         unsigned rank = 0;
+#pragma unroll 8
         for (unsigned j = 0; j < n; ++j) rank += better(r.list[j], mine);
         if (rank < top) r.best[rank] = mine;
     }
@@ -144,58 +285,234 @@ __device__ __forceinline__ unsigned keep_top(const Room &r, unsigned n, unsigned
     return kept;
 }
 
-// Log probabilities of a row whose sums are known, with its `n` top tokens in
-// r.list; or its divergence from the teacher.
-template <int DT, int G, bool ENT, bool TOP>
-__device__ __forceinline__ void finish_row(const StatArgs &a, size_t row, Part p, const Room &r, unsigned lane, float *lds) {
+// A teacher's row in a wave: entry j 64 + lane in place j, negative ids where there is none.
+struct Teacher {
+    static constexpr int E = kTeacherMost / kWave;
+    int id[E];
+    float v[E];
+    __device__ __forceinline__ void load(const int32_t *ids, const float *values, unsigned k, unsigned lane) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            const unsigned i = j * kWave + lane;
+            id[j] = -1;
+            if (i < k) {
+                id[j] = ids[i];
+                v[j] = values[i];
+            }
+        }
+    }
+};
+
+// Log probabilities of a row whose sums are known, with its top tokens in r.list;
+// or its divergence from the teacher.  By one wave.
+template <int DT, bool ENT, bool TOP>
+__device__ __forceinline__ void finish_row(const StatArgs &a, size_t row, Part p, const Room &r, const Teacher &t, unsigned lane) {
     using S = typename Elem<DT>::S;
     const S *x = static_cast<const S *>(a.in.x) + row * a.in.ld;
+    if (!TOP && a.kind == 1) {
+        // the teacher's tokens' logits, at once
+        float at[Teacher::E], tm = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < Teacher::E; ++j) {
+            at[j] = 0.0f;
+            if (t.id[j] < 0) continue;
+            if (static_cast<unsigned>(t.id[j]) < a.in.vocab) at[j] = Elem<DT>::load(x[t.id[j]]);
+            tm = fmax3(tm, static_cast<unsigned>(t.id[j]) < a.in.vocab ? t.v[j] : __builtin_nanf(""));
+        }
+        tm = wave_reduce<InfMaxOp>(tm);
+        const float log_s = logf(p.s);
+        float z = 0.0f, w = 0.0f;
+        if (tm != -INFINITY && !__builtin_isnan(tm)) {
+#pragma unroll
+            for (int j = 0; j < Teacher::E; ++j) {
+                if (t.id[j] < 0) continue;
+                const float l = (t.v[j] - tm) * a.in.scale, e = expf(l);
+                if (e == 0.0f) continue;
+                z += e;
+                w = fmaf(e, l - ((at[j] - p.m) * a.in.scale - log_s), w);
+            }
+        }
+        z = wave_reduce<SumOp>(z);
+        w = wave_reduce<SumOp>(w);
+        if (lane == 0) {
+            a.loss[row] = tm == -INFINITY ? 0.0f : __builtin_isnan(tm) ? tm : w / z - logf(z);
+            if (a.lse) a.lse[row] = fmaf(a.in.scale, p.m, log_s);
+        }
+        return;
+    }
     const float log_s = logf(p.s);
     auto logp = [&](float v) { return (v - p.m) * a.in.scale - log_s; };
+    if constexpr (TOP) {
+        const bool bad = __builtin_isnan(p.m);
+        if (lane < a.top) {
+            const ArgPair v = r.list[lane];
+            a.top_ids[row * a.top + lane] = bad ? -1 : v.i;
+            a.top_logp[row * a.top + lane] = bad ? __builtin_nanf("") : logp(v.v);
+        }
+    }
     if (lane == 0) {
         if (a.lse) a.lse[row] = fmaf(a.in.scale, p.m, log_s);
         if constexpr (ENT) {
             const float h = log_s - kLn2 * (p.t / p.s);
             a.entropy[row] = h < 0.0f ? 0.0f : h;
         }
-        if (a.kind == 0 && a.logp) {
+        if (a.logp) {
             const int tok = a.tokens[row];
             a.logp[row] = tok < 0                                       ? 0.0f
                           : static_cast<unsigned>(tok) < a.in.vocab ? logp(Elem<DT>::load(x[tok]))
                                                                         : __builtin_nanf("");
         }
     }
-    if constexpr (TOP) {
-        const bool bad = __builtin_isnan(p.m);
-        for (unsigned i = lane; i < a.top; i += G) {
-            const ArgPair v = r.list[i];
-            a.top_ids[row * a.top + i] = bad ? -1 : v.i;
-            a.top_logp[row * a.top + i] = bad ? __builtin_nanf("") : logp(v.v);
+}
+
+// m, S and T of what a wave holds, from its largest value.
+template <int DT, int VE, int C, bool ENT>
+__device__ __forceinline__ Part again_from_the_largest(Chunk<DT, VE> (&c)[C], int its, float scale) {
+    float m = -INFINITY, s = 0.0f, t = 0.0f;
+#pragma nounroll
+    for (int i = 0; i < its; ++i) {
+        const Chunk<DT, VE> v = pick(c, i);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) m = fmax3(m, v.get(e));
+    }
+    m = wave_reduce<InfMaxOp>(m);
+    const float base = m == -INFINITY ? 0.0f : m;
+#pragma nounroll
+    for (int i = 0; i < its; ++i) {
+        const Chunk<DT, VE> v = pick(c, i);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+            const float u = fmax3((v.get(e) - base) * scale, kLow), p = __builtin_amdgcn_exp2f(u);
+            s += p;
+            if constexpr (ENT) t = fmaf(u, p, t);
         }
     }
-    if (a.kind == 1) {
-        const int32_t *ids = a.ids + row * a.k;
-        const float *tv = a.teacher + row * a.k;
-        float tm = -INFINITY, bad = 0.0f;
-        for (unsigned i = lane; i < a.k; i += G) {
-            if (ids[i] < 0) continue;
-            if (static_cast<unsigned>(ids[i]) >= a.in.vocab) bad = __builtin_nanf("");
-            tm = fmax3(tm, tv[i]);
-        }
-        tm = group_all<InfMaxOp, G>(fmax3(tm, bad == 0.0f ? -INFINITY : bad), lds);
-        float z = 0.0f, w = 0.0f;
-        if (tm != -INFINITY && !__builtin_isnan(tm)) {
-            for (unsigned i = lane; i < a.k; i += G) {
-                if (ids[i] < 0) continue;
-                const float l = (tv[i] - tm) * a.in.scale, e = expf(l);
-                if (e == 0.0f) continue;
-                z += e;
-                w = fmaf(e, l - logp(Elem<DT>::load(x[ids[i]])), w);
+    return Part{m, wave_reduce<SumOp>(s), ENT ? wave_reduce<SumOp>(t) : 0.0f};
+}
+
+// The n best tokens of a segment whose lanes hold c exactly, where too many are
+// not below the bar because they are equal: the value of the n-th bit by bit,
+// then, of those equal to it, the last place that is taken.  Into the list.
+template <int DT, int VE, int G, int C>
+__device__ __forceinline__ void exact_top(const Chunk<DT, VE> (&c)[C], const Seg &seg, unsigned n, const Room &room,
+                                          unsigned lane, int *lds) {
+    // tokens above t, and those equal to it before place `to`: into the list with `keep`, else counted
+    auto count = [&](float t, unsigned to, bool keep) {
+        int k = 0;
+#pragma nounroll
+        for (int i = 0; i < seg.its; ++i) {
+            const Own own = seg.own<VE, G>(i, lane);
+            const Chunk<DT, VE> v = pick(c, i);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+                const float x = v.get(e);
+                const unsigned j = own.off + e;
+                const bool in = own.has(e) && (x > t || (x == t && j < to));
+                k += in;
+                if (in && keep) room.list[next_place(room)] = ArgPair{x, static_cast<int>(j)};
             }
         }
-        z = group_all<SumOp, G>(z, lds);
-        w = group_all<SumOp, G>(w, lds);
-        if (lane == 0) a.loss[row] = tm == -INFINITY ? 0.0f : __builtin_isnan(tm) ? tm : w / z - logf(z);
+        return static_cast<unsigned>(group_all<IntSumOp, G>(k, lds));
+    };
+    constexpr int places = 15;  // a segment has at most 2^14
+    unsigned key = 0, place = 0;
+    float t = 0.0f;
+#pragma nounroll
+    for (int step = 31; step >= kLowBit<DT> - places - 1; --step) {
+        const bool value = step >= kLowBit<DT>, last = step == kLowBit<DT> - places - 1;
+        const unsigned bit = value ? 1u << step : last ? 0u : 1u << (step - kLowBit<DT> + places);
+        if (!value && step == kLowBit<DT> - 1) {  // all bits of the value are known
+            if (!(key & 0x80000000u)) key |= (1u << kLowBit<DT>) - 1;  // a negative value's are counted from its other end
+            t = key < 0x007fffffu ? -INFINITY : value_of(key);
+        }
+        if (last && lane == 0) *room.count = 0;
+        if (last) group_sync<G>();
+        const unsigned got = count(value ? value_of(key | bit) : t, value ? ~0u : last ? seg.begin() + place + 1 : seg.begin() + (place | bit), last);
+        if (value && got >= n) key |= bit;
+        if (!value && got < n) place |= bit;  // (before the last place that is taken there are fewer)
+    }
+    group_sync<G>();
+}
+
+// A row's top tokens, in order, from its segments' lists: those below the
+// highest bar are left out as they are read.
+template <int DT, int G>
+__device__ __forceinline__ void join_top(const StatArgs &a, size_t row, const Room &room, unsigned lane, float *lds_f,
+                                         int *lds_i) {
+    constexpr int U = 4, J = 4;
+    const float *bars = a.bars + row * a.in.nseg * 2;
+    const size_t total = static_cast<size_t>(a.in.nseg) * a.keep;
+    const ArgPair *cands = a.cands + row * total;
+    ArgPair v[U];
+    auto load = [&](size_t b) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = b + u * G + lane < total ? ld_dev(cands + b + u * G + lane) : ArgPair{-INFINITY, 0x7fffffff};
+    };
+    load(0);
+    float low = -INFINITY;
+    for (unsigned i = lane; i < a.in.nseg; i += G) low = fmax3(low, ld_dev(bars + 2 * i));
+    low = group_all<InfMaxOp, G>(low, lds_f);
+    // of as many segments as tokens are wanted each has one not below its largest value
+    if (a.in.nseg >= a.top && a.in.nseg <= J * kWave) {
+        if (lane < kWave) {
+            float most[J];
+#pragma unroll
+            for (int j = 0; j < J; ++j) most[j] = j * kWave + lane < a.in.nseg ? ld_dev(bars + 2 * (j * kWave + lane) + 1) : -INFINITY;
+            const float t = threshold<DT, J>(most, a.top, 0);
+            if (lane == 0) *room.bar = t;
+        }
+        group_sync<G>();
+        low = fmax3(low, *room.bar);
+    }
+    unsigned have = 0;
+    if (lane == 0) *room.count = 0;
+    group_sync<G>();
+    auto counted = [&] {
+        group_sync<G>();
+        have = *room.count;
+        group_sync<G>();
+    };
+    bool fits = true;
+    size_t b = 0;
+    int u = 0;
+    for (;;) {
+        const bool done = b >= total;
+        if (u == 0 && !done) {
+            if (b) load(b);
+            auto passing = [&] {
+                int k = 0;
+#pragma unroll
+                for (int j = 0; j < U; ++j) k += v[j].v >= low && v[j].i != 0x7fffffff;
+                return static_cast<unsigned>(group_all<IntSumOp, G>(k, lds_i));
+            };
+            fits = have + passing() <= kCap<G>;
+            if (!fits) {  // without those that the wave's own best ones leave out
+                float w[U];
+#pragma unroll
+                for (int j = 0; j < U; ++j) w[j] = v[j].v;
+                low = fmax3(low, threshold<DT, U>(w, a.top, a.top + a.top / 8));
+                fits = have + passing() <= kCap<G>;
+            }
+        }
+        if (!fits && !done) counted();
+        if (done || (!fits && have + G > kCap<G>)) {  // (at most G more each time)
+            have = keep_top<DT, G>(room, have, a.top, lane);
+            if (done) break;
+            if (lane == 0) *room.count = static_cast<int>(have);
+            group_sync<G>();
+        }
+        ArgPair mine = v[0];
+#pragma unroll
+        for (int j = 1; j < U; ++j) {
+            mine.v = u == j ? v[j].v : mine.v;
+            mine.i = u == j ? v[j].i : mine.i;
+        }
+        if (mine.v >= low && mine.i != 0x7fffffff) room.list[next_place(room)] = mine;
+        if (++u == U || b + u * G >= total) {
+            counted();
+            b += U * G;
+            u = 0;
+        }
     }
 }
 
@@ -207,114 +524,155 @@ __global__ __launch_bounds__(kBlock) void k_vocab_stats(StatArgs a) {
     __shared__ float lds_f[kBlock / kWave];
     __shared__ int lds_i[kBlock / kWave];
     __shared__ Part lds_p[kBlock / kWave];
-    __shared__ ArgPair lists[TOP ? NG : 1][TOP ? (G == kBlock ? kList : kTopMost) : 1], bests[TOP ? NG : 1][TOP ? kTopMost : 1];
+    constexpr unsigned CAP = kCap<G>;
+    __shared__ ArgPair lists[TOP ? NG : 1][TOP ? CAP : 1], bests[TOP ? NG : 1][TOP ? kTopMost : 1];
+    __shared__ float peaks[TOP && G == kBlock ? kBlock : 1], bars[NG];  // peaks: each lane's largest value
     __shared__ int counts[NG], flag;
     const unsigned lane = threadIdx.x % G, grp = threadIdx.x / G;
-    const Room room{lists[TOP ? grp : 0], bests[TOP ? grp : 0], &counts[grp]};
+    const Room room{lists[TOP ? grp : 0], bests[TOP ? grp : 0], &counts[grp], &bars[grp]};
     const size_t row = G == kBlock ? blockIdx.x / a.in.nseg : static_cast<size_t>(blockIdx.x) * NG + grp;
     if (row >= a.in.rows) return;  // a whole wave of a workgroup whose waves have rows of their own
-    const unsigned seg = G == kBlock ? blockIdx.x % a.in.nseg : 0;
-    const unsigned s0 = seg * a.in.seglen, s1 = a.in.vocab - s0 < a.in.seglen ? a.in.vocab : s0 + a.in.seglen;
+    const unsigned number = G == kBlock ? blockIdx.x % a.in.nseg : 0;
     const S *x = static_cast<const S *>(a.in.x) + row * a.in.ld;
-    // chunks that some lane of this wave has
-    const unsigned first = s0 + (__builtin_amdgcn_readfirstlane(lane / kWave) * kWave) * VE;
-    const int its = first >= s1 ? 0 : static_cast<int>((s1 - first + G * VE - 1) / (G * VE));
+    const Seg seg = seg_of<DT, VE, G>(a.in, x, number, lane);
     Chunk<DT, VE> c[C];
-    Span sp[C];
+    Teacher teacher;
+    if (!TOP && a.kind == 1 && lane < kWave) teacher.load(a.ids + row * a.k, a.teacher + row * a.k, a.k, lane);
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-        sp[i] = seg_span<VE>(s0 + (i * G + lane) * VE, s1);
-        if (i < its) c[i].load_nt(x + sp[i].off);
-    }
-    float m = -INFINITY;
+    for (int i = 0; i < C; ++i)
+        if (i < seg.its) c[i].load_nt(x + seg.own<VE, G>(i, lane).off);
+    // Without the top tokens one pass, with the largest of the wave's first chunks as m, which the others need
+    // not be below: S then says whether they are by too much (or are NaN, or infinite), and the sums are taken
+    // again from the largest of all.  With them the largest values come first, and a wave finds the bar
+    // while the others go on.  z's product with c is not rounded on its own; what m c lost is made up for.
+    [[maybe_unused]] const unsigned held = seg.end - seg.begin(), n0 = held < a.top ? held : a.top;
+    [[maybe_unused]] float low = -INFINITY;  // the bar: at least `top` tokens are not below it, so none below it is wanted
+    float cm[C], from = -INFINITY;           // each chunk's largest, all of them's
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-        if (i >= its) break;
-        drop_dup<DT, VE>(c[i], sp[i].dup);
+    for (int i = 0; i < C; ++i) cm[i] = -INFINITY;
+    auto prepare = [&](int i) {
+        // (only a wave's first and last chunks are shared with another)
+        if (i == 0 || i + 1 >= seg.its) drop_others<DT, VE>(c[i], seg.own<VE, G>(i, again(lane)));
+        if (!TOP && i) return;
+        float a0 = -INFINITY, a1 = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < VE; ++e) m = fmax3(m, c[i].get(e));
-    }
-    m = wave_reduce<InfMaxOp>(m);
-    const float base = m == -INFINITY ? 0.0f : m;
-    float sum[2] = {0.0f, 0.0f}, ent[2] = {0.0f, 0.0f};
+        for (int e = 0; e < VE; ++e) (e & 1 ? a1 : a0) = fmax3(e & 1 ? a1 : a0, c[i].get(e));
+        cm[i] = fmax3(a0, a1);
+        from = fmax3(from, cm[i]);
+    };
+    if constexpr (TOP) {
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-        if (i >= its) break;
+        for (int i = 0; i < C; ++i) {
+            if (i >= seg.its) break;
+            prepare(i);
+        }
+        if (lane == 0) *room.count = 0;
+        // (where most of the lanes that hold anything are wanted, stopping early would tell nothing)
+        const unsigned near = 2 * n0 * VE <= held && 2 * n0 <= G ? n0 + n0 / 8 + 4 : 0;
+        if constexpr (G == kBlock) {
+            constexpr int NW = kBlock / kWave;
+            peaks[lane] = from;
+            __syncthreads();
+            if (lane / kWave == number % NW) {
+                float v[NW];
 #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-            float u = (c[i].get(e) - base) * a.in.c;
-            if constexpr (ENT) u = fmax3(u, kLow);
-            const float p = __builtin_amdgcn_exp2f(u);
-            sum[e & 1] += p;
-            if constexpr (ENT) ent[e & 1] = fmaf(u, p, ent[e & 1]);
+                for (int j = 0; j < NW; ++j) v[j] = peaks[j * kWave + lane % kWave];
+                const float t = threshold<DT, NW>(v, n0, near);
+                const float most = wave_reduce<InfMaxOp>(fmax3(fmax3(v[0], v[1]), fmax3(v[2], v[3])));
+                if (lane % kWave == 0) {
+                    bars[0] = t;
+                    if (a.in.nseg > 1) {
+                        st_dev(a.bars + 2 * (row * a.in.nseg + number), n0 < a.top ? -INFINITY : t);
+                        st_dev(a.bars + 2 * (row * a.in.nseg + number) + 1, most);
+                    }
+                }
+            }
+        } else {
+            const float v[1] = {from};
+            low = threshold<DT, 1>(v, n0, near);
         }
     }
-    Part p{m, wave_reduce<SumOp>(sum[0] + sum[1]), ENT ? wave_reduce<SumOp>(ent[0] + ent[1]) : 0.0f};
+    Part p{-INFINITY, 0.0f, 0.0f};
+    if (seg.its > 0) {
+        float mc = 0.0f;
+        float sum[2] = {0.0f, 0.0f}, ent[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            if (i >= seg.its) break;
+            if constexpr (TOP) again(c[i]);
+            else prepare(i);
+            if (i == 0) {
+                from = wave_reduce<InfMaxOp>(from);
+                mc = from * a.in.c;
+            }
+            float u[VE], q[VE];
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+                u[e] = fmaf(c[i].get(e), a.in.c, -mc);
+                if constexpr (ENT) u[e] = fmax3(u[e], kLow);
+            }
+#pragma unroll
+            for (int e = 0; e < VE; ++e) q[e] = __builtin_amdgcn_exp2f(u[e]);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+                sum[e & 1] += q[e];
+                if constexpr (ENT) ent[e & 1] = fmaf(u[e], q[e], ent[e & 1]);
+            }
+        }
+        p = Part{from, wave_reduce<SumOp>(sum[0] + sum[1]), ENT ? wave_reduce<SumOp>(ent[0] + ent[1]) : 0.0f};
+        if (fabsf(mc) < 1e37f && p.s < 0x1p20f) {
+            const float lost = -fmaf(from, a.in.c, -mc), f = __builtin_amdgcn_exp2f(lost);
+            p = Part{from, p.s * f, fmaf(lost, p.s, p.t) * f};
+        } else {
+            p = again_from_the_largest<DT, VE, C, ENT>(c, seg.its, a.in.c);
+        }
+    }
     if constexpr (G == kBlock) {
         constexpr int NW = kBlock / kWave;
         if (lane % kWave == 0) lds_p[lane / kWave] = p;
         __syncthreads();
-        float top = lds_p[0].m;
-#pragma unroll
-        for (int w = 1; w < NW; ++w) top = fmax3(top, lds_p[w].m);
-        Part q{top, 0.0f, 0.0f};
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const Part v = rebase(lds_p[w], top, a.in.c);
-            q.s += v.s;
-            q.t += v.t;
-        }
+        const Part one = lds_p[lane % NW];  // every four lanes for themselves
+        static_assert(NW == 4, "the sums below are over four lanes");
+        const float top = group_reduce<InfMaxOp, NW>(one.m);
+        const Part v = rebase(one, top, a.in.c);
+        const Part q{top, group_reduce<SumOp, NW>(v.s), ENT ? group_reduce<SumOp, NW>(v.t) : 0.0f};
         p = q;
     }
-    unsigned n = 0;  // tokens selected
+    unsigned n = 0;  // tokens in the list
     if constexpr (TOP) {
-        // The segment's top tokens exactly: the value of the last of them bit by bit, then, of those equal to
-        // it, the last place that is taken.
-        n = s1 - s0 < a.top ? s1 - s0 : a.top;
+        if constexpr (G == kBlock) low = bars[0];
         if (!__builtin_isnan(p.m)) {
-            auto count = [&](auto &&f) {
-                int k = 0;
+            if constexpr (G != kBlock) group_sync<G>();
+            // the chunks that have such tokens, one per lane at a time
+            unsigned hits = 0;
 #pragma unroll
-                for (int i = 0; i < C; ++i) {
-                    if (i >= its) break;
-#pragma unroll
-                    for (int e = 0; e < VE; ++e) k += f(c[i].get(e), sp[i].off + e, e >= static_cast<int>(sp[i].dup));
-                }
-                return static_cast<unsigned>(group_all<IntSumOp, G>(k, lds_i));
-            };
-            unsigned key = 0;
-            constexpr int low = DT == CXM_DT_F32 ? 0 : DT == CXM_DT_BF16 ? 16 : 13;  // bits below are all alike
-            for (int b = 31; b >= low; --b) {
-                const float t = value_of(key | 1u << b);
-                if (count([&](float v, unsigned, bool own) { return own && v >= t; }) >= n) key |= 1u << b;
-            }
-            if (!(key & 0x80000000u)) key |= (1u << low) - 1;  // a negative value's bits are counted from its other end
-            const float t = key < 0x007fffffu ? -INFINITY : value_of(key);
-            const unsigned above = count([&](float v, unsigned, bool own) { return own && v > t; }), ties = n - above;
-            unsigned place = 0;  // the ties below s0 + place are fewer than `ties`
-            for (unsigned b = 1u << 14; b; b >>= 1) {
-                const unsigned to = s0 + (place | b);
-                if (count([&](float v, unsigned j, bool own) { return own && v == t && j < to; }) < ties) place |= b;
-            }
-            if (lane == 0) *room.count = 0;
-            group_sync<G>();
-#pragma unroll
-            for (int i = 0; i < C; ++i) {
-                if (i >= its) break;
+            for (int i = 0; i < C; ++i) hits |= i < seg.its && cm[i] >= low ? 1u << i : 0u;
+#pragma nounroll
+            while (__any(hits != 0)) {
+                const int i = hits ? __builtin_ctz(hits) : 0;
+                const Own own = seg.own<VE, G>(i, lane);
+                const Chunk<DT, VE> v = pick(c, i);
 #pragma unroll
                 for (int e = 0; e < VE; ++e) {
-                    const float v = c[i].get(e);
-                    const unsigned j = sp[i].off + e;
-                    if (e >= static_cast<int>(sp[i].dup) && (v > t || (v == t && j <= s0 + place)))
-                        room.list[atomicAdd(room.count, 1)] = ArgPair{v, static_cast<int>(j)};
+                    if (hits && v.get(e) >= low && own.has(e)) {
+                        const unsigned at = next_place(room);
+                        if (at < CAP) room.list[at] = ArgPair{v.get(e), static_cast<int>(own.off + e)};
+                    }
                 }
+                hits &= hits - 1;
             }
             group_sync<G>();
+            n = *room.count;
+            if (n > CAP) {
+                exact_top<DT, VE, G, C>(c, seg, n0, room, lane, lds_i);
+                n = n0;
+            }
+            if (G != kBlock || a.in.nseg == 1 || n > a.keep) n = keep_top<DT, G>(room, n, n0, lane);
         }
     }
     if constexpr (G == kBlock) {
         if (a.in.nseg > 1) {
-            const size_t at = row * a.in.nseg + seg;
+            const size_t at = row * a.in.nseg + number;
             if (lane == 0) {
                 float *to = &a.parts[at].m;
                 st_dev(to, p.m);
@@ -322,43 +680,37 @@ __global__ __launch_bounds__(kBlock) void k_vocab_stats(StatArgs a) {
                 st_dev(to + 2, p.t);
             }
             if constexpr (TOP) {
-                // (a NaN segment's are not looked at)
-                for (unsigned i = lane; i < a.top; i += G)
-                    st_dev(a.cands + at * a.top + i, i < n && !__builtin_isnan(p.m) ? room.list[i] : ArgPair{-INFINITY, 0x7fffffff});
+                for (unsigned i = lane; i < a.keep; i += G)
+                    st_dev(a.cands + at * a.keep + i, i < n ? room.list[i] : ArgPair{-INFINITY, 0x7fffffff});
             }
             if (!last_block_ticket(a.tickets + row * kTicket, a.in.nseg, &flag)) return;
-            const float *from = &a.parts[row * a.in.nseg].m;
-            float top = -INFINITY;
-            for (unsigned i = lane; i < a.in.nseg; i += G) top = fmax3(top, ld_dev(from + 3 * i));
-            top = block_reduce<InfMaxOp, kBlock>(top, lds_f);
-            Part q{top, 0.0f, 0.0f};
-            for (unsigned i = lane; i < a.in.nseg; i += G) {
-                const Part v = rebase(Part{ld_dev(from + 3 * i), ld_dev(from + 3 * i + 1), ld_dev(from + 3 * i + 2)}, top, a.in.c);
+            if (!TOP && lane >= kWave) return;
+            // every wave for itself
+            const float *parts = &a.parts[row * a.in.nseg].m;
+            const unsigned l = lane % kWave;
+            const Part one = l < a.in.nseg ? Part{ld_dev(parts + 3 * l), ld_dev(parts + 3 * l + 1), ld_dev(parts + 3 * l + 2)}
+                                           : Part{-INFINITY, 0.0f, 0.0f};
+            float top = one.m;
+            for (unsigned i = l + kWave; i < a.in.nseg; i += kWave) top = fmax3(top, ld_dev(parts + 3 * i));
+            top = wave_reduce<InfMaxOp>(top);
+            Part q = rebase(one, top, a.in.c);
+            for (unsigned i = l + kWave; i < a.in.nseg; i += kWave) {
+                const Part v = rebase(Part{ld_dev(parts + 3 * i), ld_dev(parts + 3 * i + 1), ld_dev(parts + 3 * i + 2)}, top, a.in.c);
                 q.s += v.s;
                 q.t += v.t;
             }
-            q.s = block_reduce<SumOp, kBlock>(q.s, lds_f);
-            q.t = block_reduce<SumOp, kBlock>(q.t, lds_f);
-            p = q;
+            p = Part{top, wave_reduce<SumOp>(q.s), wave_reduce<SumOp>(q.t)};
             if constexpr (TOP) {
-                const size_t total = static_cast<size_t>(a.in.nseg) * a.top;
-                const ArgPair *cands = a.cands + row * total;
-                unsigned have = 0;
-                for (size_t b = 0; b < total;) {
-                    const unsigned take = total - b < kList - have ? static_cast<unsigned>(total - b) : kList - have;
-                    for (unsigned i = lane; i < take; i += G) room.list[have + i] = ld_dev(cands + b + i);
-                    b += take;
-                    have = keep_top<G>(room, have + take, a.top, lane);
+                if (a.in.nseg * a.keep <= 512) {  // few enough for one wave, without barriers
+                    if (lane >= kWave) return;
+                    if (!__builtin_isnan(p.m)) join_top<DT, kWave>(a, row, room, lane, lds_f, lds_i);
+                } else {
+                    if (!__builtin_isnan(p.m)) join_top<DT, G>(a, row, room, lane, lds_f, lds_i);
                 }
-                n = have;
             }
-        } else if constexpr (TOP) {
-            keep_top<G>(room, n, a.top, lane);
         }
-    } else if constexpr (TOP) {
-        keep_top<G>(room, n, a.top, lane);
     }
-    finish_row<DT, G, ENT, TOP>(a, row, p, room, lane, lds_f);
+    if (lane < kWave) finish_row<DT, ENT, TOP>(a, row, p, room, teacher, lane);
 }
 
 struct GradArgs {
@@ -375,77 +727,80 @@ struct GradArgs {
     unsigned k;
 };
 
+// A row per G lanes or a segment per workgroup, as above.  Each wave finds out by
+// itself whether the row has a gradient; the teacher's probabilities and the
+// gradients of its tokens in the segment are the first wave's, which stores them
+// over the others'.
 template <int DT, int VE, int G, int C, bool DISTILL, bool ENT>
 __global__ __launch_bounds__(kBlock) void k_vocab_grad(GradArgs a) {
     using S = typename Elem<DT>::S;
-    constexpr int NG = kBlock / G, KE = kTeacherMost / G;
-    __shared__ float lds_f[kBlock / kWave];
+    constexpr int NG = kBlock / G, E = Teacher::E;
     __shared__ float qs[DISTILL ? NG : 1][DISTILL ? kTeacherMost : 1];
-    __shared__ int qi[DISTILL ? NG : 1][DISTILL ? kTeacherMost : 1];
+    __shared__ alignas(16) int qi[DISTILL ? NG : 1][DISTILL ? kTeacherMost : 1];
     const unsigned lane = threadIdx.x % G, grp = threadIdx.x / G;
     const size_t row = G == kBlock ? blockIdx.x / a.in.nseg : static_cast<size_t>(blockIdx.x) * NG + grp;
     if (row >= a.in.rows) return;  // a whole wave of a workgroup whose waves have rows of their own
-    const unsigned seg = G == kBlock ? blockIdx.x % a.in.nseg : 0;
-    const unsigned s0 = seg * a.in.seglen, s1 = a.in.vocab - s0 < a.in.seglen ? a.in.vocab : s0 + a.in.seglen;
     const S *x = static_cast<const S *>(a.in.x) + row * a.in.ld;
     S *dx = static_cast<S *>(a.dx) + row * a.ldd;
-    const unsigned first = s0 + (__builtin_amdgcn_readfirstlane(lane / kWave) * kWave) * VE;
-    const int its = first >= s1 ? 0 : static_cast<int>((s1 - first + G * VE - 1) / (G * VE));
+    const Seg seg = seg_of<DT, VE, G>(a.in, x, G == kBlock ? blockIdx.x % a.in.nseg : 0, lane);
     Chunk<DT, VE> c[C];
-    Span sp[C];
+    Own own[C];
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-        sp[i] = seg_span<VE>(s0 + (i * G + lane) * VE, s1);
-        if (i < its) c[i].load_nt(x + sp[i].off);
+        own[i] = seg.own<VE, G>(i, lane);
+        if (i < seg.its) c[i].load_nt(x + own[i].off);
     }
     const float lse = a.lse[row];
     // d x = p (slope + bend (log p)) + what the tokens get
     float slope, bend = 0.0f, given = 0.0f;
     unsigned token = ~0u;
-    float late_v[KE];  // distillation: the gradient at the teacher's tokens of this segment
-    bool late[KE];
+    [[maybe_unused]] float late[E];  // the gradient at the teacher's tokens of this segment
+    [[maybe_unused]] Teacher t;
     if constexpr (DISTILL) {
-        const int32_t *ids = a.ids + row * a.k;
-        const float *tv = a.teacher + row * a.k;
-        int id[KE];
-        float t[KE], tm = -INFINITY;
+        t.load(a.ids + row * a.k, a.teacher + row * a.k, a.k, lane % kWave);
+        float tm = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < KE; ++j) {
-            const unsigned i = j * G + lane;
-            id[j] = i < a.k ? ids[i] : -1;
-            t[j] = i < a.k && id[j] >= 0 ? tv[i] : -INFINITY;
-            if (id[j] >= 0 && static_cast<unsigned>(id[j]) >= a.in.vocab) t[j] = __builtin_nanf("");
-            tm = fmax3(tm, t[j]);
-        }
-        tm = group_all<InfMaxOp, G>(tm, lds_f);
-        float z = 0.0f, q[KE];
-        const float from = tm == -INFINITY ? 0.0f : tm;
+        for (int j = 0; j < E; ++j)
+            if (t.id[j] >= 0) tm = fmax3(tm, static_cast<unsigned>(t.id[j]) < a.in.vocab ? t.v[j] : __builtin_nanf(""));
+        tm = wave_reduce<InfMaxOp>(tm);
+        slope = tm == -INFINITY ? 0.0f : __builtin_isnan(tm) ? tm : a.dloss[row] * a.in.scale;
+        if (lane < kWave) {
+            float at[E], q[E], z = 0.0f;
+            bool mine[E];
 #pragma unroll
-        for (int j = 0; j < KE; ++j) {
-            q[j] = expf((t[j] - from) * a.in.scale);
-            z += q[j];
-        }
-        z = group_all<SumOp, G>(z, lds_f);
-        slope = tm == -INFINITY ? 0.0f : a.dloss[row] * a.in.scale;
+            for (int j = 0; j < E; ++j) {  // what the dense gradient may be stored over
+                mine[j] = t.id[j] >= static_cast<int>(seg.begin()) && t.id[j] < static_cast<int>(seg.end);
+                at[j] = mine[j] ? Elem<DT>::load(x[t.id[j]]) : 0.0f;
+                q[j] = t.id[j] < 0 ? 0.0f : expf((t.v[j] - (tm == -INFINITY ? 0.0f : tm)) * a.in.scale);
+                z += q[j];
+            }
+            z = wave_reduce<SumOp>(z);
 #pragma unroll
-        for (int j = 0; j < KE; ++j) {
-            q[j] /= z;
-            qs[grp][j * G + lane] = q[j];
-            qi[grp][j * G + lane] = id[j];
-        }
-        group_sync<G>();
+            for (int j = 0; j < E; ++j) {
+                q[j] /= z;
+                qs[grp][j * kWave + lane] = q[j];
+                qi[grp][j * kWave + lane] = mine[j] ? t.id[j] : -1;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-        for (int j = 0; j < KE; ++j) {
-            late[j] = id[j] >= static_cast<int>(s0) && id[j] < static_cast<int>(s1);
-            late_v[j] = 0.0f;
-            if (late[j]) {
-                float all = 0.0f;  // a token may be there more than once
-                for (unsigned i = 0; i < a.k; ++i) all += qi[grp][i] == id[j] ? qs[grp][i] : 0.0f;
-                const float p = __builtin_amdgcn_exp2f(fmaf(a.in.scale, Elem<DT>::load(x[id[j]]), -lse) * kLog2e);
-                late_v[j] = slope == 0.0f ? 0.0f : slope * (p - all);
+            for (int j = 0; j < E; ++j) {
+                if (!__any(mine[j])) continue;
+                // a token may be there more than once
+                int times = 0;
+                for (unsigned i = 0; i < (a.k + 3) / 4; ++i) {
+                    const int4 v = reinterpret_cast<const int4 *>(qi[grp])[i];
+                    times += (v.x == t.id[j]) + (v.y == t.id[j]) + (v.z == t.id[j]) + (v.w == t.id[j]);
+                }
+                float all = q[j];
+                if (__any(mine[j] && times > 1)) {
+                    all = 0.0f;
+                    for (unsigned i = 0; i < a.k; ++i) all += qi[grp][i] == t.id[j] ? qs[grp][i] : 0.0f;
+                }
+                const float p = __builtin_amdgcn_exp2f(fmaf(a.in.scale, at[j], -lse) * kLog2e);
+                late[j] = slope == 0.0f ? 0.0f : slope * (p - all);
+                if (!mine[j]) t.id[j] = -1;
             }
         }
-        if (__builtin_isnan(tm)) slope = tm;
     } else {
         const int tok = a.tokens ? a.tokens[row] : -1;
         const float g = tok < 0 || !a.dlogp ? 0.0f : static_cast<unsigned>(tok) < a.in.vocab ? a.dlogp[row] : __builtin_nanf("");
@@ -460,34 +815,41 @@ __global__ __launch_bounds__(kBlock) void k_vocab_grad(GradArgs a) {
         }
     }
     const bool none = slope == 0.0f && bend == 0.0f && given == 0.0f;  // zeros, whatever the logits are
-    if constexpr (DISTILL) {  // every teacher's token has been read (dx may be x)
+    if (DISTILL && a.dx == a.in.x) {  // not before the teacher's tokens have been read
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         group_sync<G>();
     }
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-        if (i >= its) break;
-        float v[VE];
+        if (i >= seg.its) break;
+        float l[VE], p[VE], v[VE];
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
-            float l = fmaf(a.in.scale, c[i].get(e), -lse);
-            if constexpr (ENT) l = fmax3(l, kLow);
-            const float p = __builtin_amdgcn_exp2f(l * kLog2e);
-            if constexpr (ENT) v[e] = p * fmaf(bend, l, slope);
-            else v[e] = p * slope;
-            if constexpr (!DISTILL) v[e] += sp[i].off + e == token ? given : 0.0f;
+            l[e] = fmaf(a.in.scale, c[i].get(e), -lse);
+            if constexpr (ENT) l[e] = fmax3(l[e], kLow);
+        }
+#pragma unroll
+        for (int e = 0; e < VE; ++e) p[e] = __builtin_amdgcn_exp2f(l[e] * kLog2e);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+            if constexpr (ENT) v[e] = p[e] * fmaf(bend, l[e], slope);
+            else v[e] = p[e] * slope;
+            if constexpr (!DISTILL) v[e] += own[i].off + e == token ? given : 0.0f;
             v[e] = none ? 0.0f : v[e];
         }
         c[i].set(v);
-        store_span<DT, VE>(dx, sp[i], c[i]);
+        store_own<DT, VE>(dx, own[i], c[i]);
     }
     if constexpr (DISTILL) {
         // over what was stored above, by whichever lane
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         group_sync<G>();
+        if (lane < kWave) {
 #pragma unroll
-        for (int j = 0; j < KE; ++j)
-            if (late[j]) dx[qi[grp][j * G + lane]] = Elem<DT>::store(__builtin_isnan(slope) ? slope : late_v[j]);
+            for (int j = 0; j < E; ++j)
+                if (t.id[j] >= static_cast<int>(seg.begin()) && t.id[j] < static_cast<int>(seg.end))
+                    dx[t.id[j]] = Elem<DT>::store(__builtin_isnan(slope) ? slope : late[j]);
+        }
     }
 }
 
@@ -496,17 +858,18 @@ __global__ __launch_bounds__(kBlock) void k_vocab_grad(GradArgs a) {
 // Cuts rows into segments of at most `most` elements, and of fewer (but a chunk
 // for every lane) where there would be fewer workgroups than fill the chip.
 void cut(Logits *in, unsigned most, unsigned least) {
-    size_t nseg = (in->vocab + most - 1) / most;
-    const size_t want = (4 * device_cus() + in->rows - 1) / in->rows, can = (in->vocab + least - 1) / least;
+    const size_t all = static_cast<size_t>(in->vocab) + in->odd;
+    size_t nseg = (all + most - 1) / most;
+    const size_t want = (4 * device_cus() + in->rows - 1) / in->rows, can = (all + least - 1) / least;
     if (nseg < want) nseg = want < can ? want : can;
-    const size_t len = (in->vocab + nseg - 1) / nseg;
+    const size_t len = (all + nseg - 1) / nseg;
     in->seglen = static_cast<unsigned>((len + 63) / 64 * 64);
-    in->nseg = (in->vocab + in->seglen - 1) / in->seglen;
+    in->nseg = static_cast<unsigned>((all + in->seglen - 1) / in->seglen);
 }
 
 // Whether a wave holds a row of C chunks a lane, and there are rows enough to give each wave one.
 bool wave_rows(const Logits &in, unsigned chunk, unsigned chunks) {
-    return in.vocab <= 64 * chunk * chunks && (in.vocab <= 64 * chunk || in.rows >= 4 * device_cus());
+    return in.vocab + in.odd <= 64 * chunk * chunks && (in.vocab <= 64 * chunk || in.rows >= 4 * device_cus());
 }
 
 template <int DT, int VE, int G, bool ENT, bool TOP>
@@ -521,7 +884,7 @@ template <int DT, bool ENT, bool TOP>
 int stats(StatArgs a, cxm_stream_t st) {
     constexpr int VE = Elem<DT>::kVec;
     a.in.nseg = 1;
-    a.in.seglen = (a.in.vocab + 63) / 64 * 64;
+    a.in.seglen = (a.in.vocab + a.in.odd + 63) / 64 * 64;
     const bool wave = a.in.vocab < static_cast<unsigned>(VE) || wave_rows(a.in, VE, kStatChunks);
     if (!wave) cut(&a.in, kBlock * VE * kStatChunks, kBlock * VE);
     if (a.in.nseg > most_wgs(kBlock) / a.in.rows) return CXM_E_TOO_LARGE;
@@ -530,13 +893,16 @@ int stats(StatArgs a, cxm_stream_t st) {
                                                       : stats_launch<DT, VE, 64, ENT, TOP>(a, hs(st));
     }
     if (a.in.nseg > 1) {
-        const size_t segs = a.in.rows * a.in.nseg, o_cands = (segs * sizeof(Part) + 255) / 256 * 256;
+        const size_t segs = a.in.rows * a.in.nseg, o_bars = (segs * sizeof(Part) + 255) / 256 * 256;
+        const size_t o_cands = o_bars + (TOP ? (segs * 2 * sizeof(float) + 255) / 256 * 256 : 0);
+        a.keep = a.top + a.top / 4 + 12;
         Workspace ws;
         const int rc = get_workspace(st, (a.in.rows * kTicket + kCtr - 1) / kCtr,
-                                     o_cands + (TOP ? segs * a.top * sizeof(ArgPair) : 0), &ws);
+                                     o_cands + (TOP ? segs * a.keep * sizeof(ArgPair) : 0), &ws);
         if (rc) return rc;
         a.tickets = ws.counters;
         a.parts = static_cast<Part *>(ws.scratch);
+        a.bars = reinterpret_cast<float *>(static_cast<char *>(ws.scratch) + o_bars);
         a.cands = reinterpret_cast<ArgPair *>(static_cast<char *>(ws.scratch) + o_cands);
     }
     return stats_launch<DT, VE, kBlock, ENT, TOP>(a, hs(st));
@@ -567,7 +933,7 @@ template <int DT, bool DISTILL, bool ENT>
 int grad(GradArgs a, cxm_stream_t st) {
     constexpr int VE = Elem<DT>::kVec;
     a.in.nseg = 1;
-    a.in.seglen = (a.in.vocab + 63) / 64 * 64;
+    a.in.seglen = (a.in.vocab + a.in.odd + 63) / 64 * 64;
     const bool wave = a.in.vocab < static_cast<unsigned>(VE) || wave_rows(a.in, VE, kGradChunks);
     if (!wave) cut(&a.in, kBlock * VE * kGradChunks, kBlock * VE);
     if (a.in.nseg > most_wgs(kBlock) / a.in.rows) return CXM_E_TOO_LARGE;
@@ -612,8 +978,9 @@ bool any_overlap(const Region (&out)[NO], const Region (&in)[NI]) {
     return false;
 }
 
-Logits logits_of(const void *x, size_t ld, float scale, size_t rows, size_t vocab) {
-    return Logits{x, ld, rows, static_cast<unsigned>(vocab), 1, 0, scale, scale * kLog2e};
+Logits logits_of(const void *x, size_t ld, float scale, size_t rows, size_t vocab, int dtype) {
+    const unsigned odd = dtype != CXM_DT_F32 && ((reinterpret_cast<uintptr_t>(x) >> 1 | ld) & 1);
+    return Logits{x, ld, rows, static_cast<unsigned>(vocab), 1, 0, scale, scale * kLog2e, odd};
 }
 
 }  // namespace
@@ -636,7 +1003,7 @@ int cxm_logprob_fwd_t(const void *logits, size_t ld, const int32_t *tokens, floa
     const cxm::Region in[2] = {{logits, cxm::span_bytes(rows, ld, vocab, cxm::dtype_bytes(dtype))}, {tokens, r4}};
     if (cxm::any_overlap(out, in)) return CXM_E_INVALID;
     cxm::StatArgs a{};
-    a.in = cxm::logits_of(logits, ld, scale, rows, vocab);
+    a.in = cxm::logits_of(logits, ld, scale, rows, vocab, dtype);
     a.tokens = tokens;
     a.logp = logp;
     a.entropy = entropy;
@@ -659,7 +1026,7 @@ int cxm_distill_fwd_t(const void *logits, size_t ld, const int32_t *ids, const f
     const cxm::Region in[3] = {{logits, cxm::span_bytes(rows, ld, vocab, cxm::dtype_bytes(dtype))}, {ids, r4 * k}, {teacher, r4 * k}};
     if (cxm::any_overlap(out, in)) return CXM_E_INVALID;
     cxm::StatArgs a{};
-    a.in = cxm::logits_of(logits, ld, scale, rows, vocab);
+    a.in = cxm::logits_of(logits, ld, scale, rows, vocab, dtype);
     a.ids = ids;
     a.teacher = teacher;
     a.loss = loss;
@@ -684,7 +1051,7 @@ int cxm_logprob_bwd_t(const void *logits, size_t ld, const int32_t *tokens, floa
     const cxm::Region in[6] = {{in_place ? nullptr : logits, n}, {tokens, r4}, {lse, r4}, {entropy, r4}, {dlogp, r4}, {dentropy, r4}};
     if (cxm::any_overlap(out, in)) return CXM_E_INVALID;
     cxm::GradArgs a{};
-    a.in = cxm::logits_of(logits, ld, scale, rows, vocab);
+    a.in = cxm::logits_of(logits, ld, scale, rows, vocab, dtype);
     a.lse = lse;
     a.dx = dlogits;
     a.ldd = ldd;
@@ -710,7 +1077,7 @@ int cxm_distill_bwd_t(const void *logits, size_t ld, const int32_t *ids, const f
     const cxm::Region in[5] = {{in_place ? nullptr : logits, n}, {ids, r4 * k}, {teacher, r4 * k}, {lse, r4}, {dloss, r4}};
     if (cxm::any_overlap(out, in)) return CXM_E_INVALID;
     cxm::GradArgs a{};
-    a.in = cxm::logits_of(logits, ld, scale, rows, vocab);
+    a.in = cxm::logits_of(logits, ld, scale, rows, vocab, dtype);
     a.lse = lse;
     a.dx = dlogits;
     a.ldd = ldd;

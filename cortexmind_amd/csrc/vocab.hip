@@ -170,7 +170,8 @@ struct StatArgs {
     // segments
     Part *parts;      // [rows, nseg]
     ArgPair *cands;   // [rows, nseg, keep]
-    float *bars;      // [rows, nseg, 2]: a value that `top` of the segment's tokens are not below, the largest
+    float *bars;      // [rows, nseg, 2]: values that `top`, and `rth`, of the segment's tokens are not below
+    unsigned rth, need;  // need segments' rth tokens are at least `top`
     unsigned keep;    // tokens a segment hands on, its `top` among them
     unsigned *tickets;
 };
@@ -199,17 +200,17 @@ __device__ __forceinline__ float threshold(const float (&v)[J], unsigned n, unsi
     unsigned k[J], key = 0;
 #pragma unroll
     for (int j = 0; j < J; ++j) k[j] = key_of(v[j]);
-#pragma nounroll
-    for (int b = 31; b >= kLowBit<DT>; --b) {
+    auto step = [&](int b) {  // whether that is enough
         const unsigned t = key | 1u << b;
         unsigned c = 0;
 #pragma unroll
         for (int j = 0; j < J; ++j) c += __popcll(__ballot(k[j] >= t));
-        if (c >= n) {
-            key = t;
-            if (c <= most) break;
-        }
-    }
+        key = c >= n ? t : key;
+        return c >= n && c <= most;
+    };
+#pragma nounroll
+    for (int b = 31; b >= kLowBit<DT>; --b)
+        if (step(b)) break;
     // (a negative value whose last bits are open stands for the lowest that begins so: nothing is lost)
     return key < 0x007fffffu ? -INFINITY : value_of(key);
 }
@@ -234,6 +235,10 @@ struct Room {
     int *count;
     float *bar;
 };
+template <int J>
+struct Width {
+    static constexpr int value = J;
+};
 template <int G>
 constexpr unsigned kCap = G == kBlock ? 512 : 128;
 
@@ -245,16 +250,21 @@ __device__ __forceinline__ unsigned next_place(const Room &r) { return atomicAdd
 // token's place is the number of better ones.  Where there are many more than
 // `top`, those below a value that `top` are not below leave first (512 tokens
 // ranked among each other took 20 us).
-template <int DT, int G>
+template <int DT, int G, unsigned CAP>
 __device__ __forceinline__ unsigned keep_top(const Room &r, unsigned n, unsigned top, unsigned lane) {
     group_sync<G>();
     if (n > top + top / 4 + 8) {
-        constexpr int J = kCap<G> / kWave, E = kCap<G> / G;
+        constexpr int E = CAP / G;
         if (G != kBlock || lane < kWave) {
-            float v[J];
+            // (as few values a lane as hold the list)
+            auto bar = [&](auto width) {
+                constexpr int J = decltype(width)::value;
+                float v[J];
 #pragma unroll
-            for (int j = 0; j < J; ++j) v[j] = j * kWave + lane < n ? r.list[j * kWave + lane].v : -INFINITY;
-            const float t = threshold<DT, J>(v, top, top + top / 8);
+                for (int j = 0; j < J; ++j) v[j] = j * kWave + lane < n ? r.list[j * kWave + lane].v : -INFINITY;
+                return threshold<DT, J>(v, top, top + top / 8);
+            };
+            const float t = n <= kWave ? bar(Width<1>{}) : n <= 2 * kWave ? bar(Width<2>{}) : bar(Width<CAP / kWave>{});
             if (lane == 0) {
                 *r.bar = t;
                 *r.count = 0;
@@ -436,7 +446,7 @@ __device__ __forceinline__ void exact_top(const Chunk<DT, VE> (&c)[C], const Seg
 
 // A row's top tokens, in order, from its segments' lists: those below the
 // highest bar are left out as they are read.
-template <int DT, int G>
+template <int DT, int G, unsigned CAP>
 __device__ __forceinline__ void join_top(const StatArgs &a, size_t row, const Room &room, unsigned lane, float *lds_f,
                                          int *lds_i) {
     constexpr int U = 4, J = 4;
@@ -452,13 +462,13 @@ __device__ __forceinline__ void join_top(const StatArgs &a, size_t row, const Ro
     float low = -INFINITY;
     for (unsigned i = lane; i < a.in.nseg; i += G) low = fmax3(low, ld_dev(bars + 2 * i));
     low = group_all<InfMaxOp, G>(low, lds_f);
-    // of as many segments as tokens are wanted each has one not below its largest value
-    if (a.in.nseg >= a.top && a.in.nseg <= J * kWave) {
+    // each of `need` segments has `rth` tokens not below its second bar
+    if (a.in.nseg >= 16 && a.in.nseg <= J * kWave) {
+        float second[J];
         if (lane < kWave) {
-            float most[J];
 #pragma unroll
-            for (int j = 0; j < J; ++j) most[j] = j * kWave + lane < a.in.nseg ? ld_dev(bars + 2 * (j * kWave + lane) + 1) : -INFINITY;
-            const float t = threshold<DT, J>(most, a.top, 0);
+            for (int j = 0; j < J; ++j) second[j] = j * kWave + lane < a.in.nseg ? ld_dev(bars + 2 * (j * kWave + lane) + 1) : -INFINITY;
+            const float t = threshold<DT, J>(second, a.need, 0);
             if (lane == 0) *room.bar = t;
         }
         group_sync<G>();
@@ -485,18 +495,18 @@ __device__ __forceinline__ void join_top(const StatArgs &a, size_t row, const Ro
                 for (int j = 0; j < U; ++j) k += v[j].v >= low && v[j].i != 0x7fffffff;
                 return static_cast<unsigned>(group_all<IntSumOp, G>(k, lds_i));
             };
-            fits = have + passing() <= kCap<G>;
+            fits = have + passing() <= CAP;
             if (!fits) {  // without those that the wave's own best ones leave out
                 float w[U];
 #pragma unroll
                 for (int j = 0; j < U; ++j) w[j] = v[j].v;
                 low = fmax3(low, threshold<DT, U>(w, a.top, a.top + a.top / 8));
-                fits = have + passing() <= kCap<G>;
+                fits = have + passing() <= CAP;
             }
         }
         if (!fits && !done) counted();
-        if (done || (!fits && have + G > kCap<G>)) {  // (at most G more each time)
-            have = keep_top<DT, G>(room, have, a.top, lane);
+        if (done || (!fits && have + G > CAP)) {  // (at most G more each time)
+            have = keep_top<DT, G, CAP>(room, have, a.top, lane);
             if (done) break;
             if (lane == 0) *room.count = static_cast<int>(have);
             group_sync<G>();
@@ -571,19 +581,33 @@ __global__ __launch_bounds__(kBlock) void k_vocab_stats(StatArgs a) {
         const unsigned near = 2 * n0 * VE <= held && 2 * n0 <= G ? n0 + n0 / 8 + 4 : 0;
         if constexpr (G == kBlock) {
             constexpr int NW = kBlock / kWave;
-            peaks[lane] = from;
+            // Few tokens: of the largest values of 64 groups of four lanes, as good a bar for a quarter of the work,
+            // which the workgroup waits for (each instruction of one wave costs the turns of the SIMD's others).
+            const bool few = a.top <= 24;
+            float m = fmax3(from, dpp<kQuadXor1>(from));
+            m = fmax3(m, dpp<kQuadXor2>(m));
+            if (!few) peaks[lane] = from;
+            else if (lane % 4 == 0) peaks[lane / 4] = m;
             __syncthreads();
             if (lane / kWave == number % NW) {
-                float v[NW];
+                float t, second = -INFINITY;
+                const bool join = a.in.nseg >= 16;
+                if (few) {
+                    const float v[1] = {peaks[lane % kWave]};
+                    t = threshold<DT, 1>(v, n0, 2 * n0 * 4 * VE <= held ? n0 + n0 / 8 + 2 : 0);
+                    if (join) second = threshold<DT, 1>(v, a.rth, a.rth);
+                } else {
+                    float v[NW];
 #pragma unroll
-                for (int j = 0; j < NW; ++j) v[j] = peaks[j * kWave + lane % kWave];
-                const float t = threshold<DT, NW>(v, n0, near);
-                const float most = wave_reduce<InfMaxOp>(fmax3(fmax3(v[0], v[1]), fmax3(v[2], v[3])));
+                    for (int j = 0; j < NW; ++j) v[j] = peaks[j * kWave + lane % kWave];
+                    t = threshold<DT, NW>(v, n0, near);
+                    if (join) second = threshold<DT, NW>(v, a.rth, a.rth);
+                }
                 if (lane % kWave == 0) {
                     bars[0] = t;
                     if (a.in.nseg > 1) {
                         st_dev(a.bars + 2 * (row * a.in.nseg + number), n0 < a.top ? -INFINITY : t);
-                        st_dev(a.bars + 2 * (row * a.in.nseg + number) + 1, most);
+                        st_dev(a.bars + 2 * (row * a.in.nseg + number) + 1, second);
                     }
                 }
             }
@@ -667,7 +691,7 @@ __global__ __launch_bounds__(kBlock) void k_vocab_stats(StatArgs a) {
                 exact_top<DT, VE, G, C>(c, seg, n0, room, lane, lds_i);
                 n = n0;
             }
-            if (G != kBlock || a.in.nseg == 1 || n > a.keep) n = keep_top<DT, G>(room, n, n0, lane);
+            if (G != kBlock || a.in.nseg == 1 || n > a.keep) n = keep_top<DT, G, CAP>(room, n, n0, lane);
         }
     }
     if constexpr (G == kBlock) {
@@ -703,9 +727,9 @@ __global__ __launch_bounds__(kBlock) void k_vocab_stats(StatArgs a) {
             if constexpr (TOP) {
                 if (a.in.nseg * a.keep <= 512) {  // few enough for one wave, without barriers
                     if (lane >= kWave) return;
-                    if (!__builtin_isnan(p.m)) join_top<DT, kWave>(a, row, room, lane, lds_f, lds_i);
+                    if (!__builtin_isnan(p.m)) join_top<DT, kWave, CAP>(a, row, room, lane, lds_f, lds_i);
                 } else {
-                    if (!__builtin_isnan(p.m)) join_top<DT, G>(a, row, room, lane, lds_f, lds_i);
+                    if (!__builtin_isnan(p.m)) join_top<DT, G, CAP>(a, row, room, lane, lds_f, lds_i);
                 }
             }
         }
@@ -857,10 +881,10 @@ __global__ __launch_bounds__(kBlock) void k_vocab_grad(GradArgs a) {
 
 // Cuts rows into segments of at most `most` elements, and of fewer (but a chunk
 // for every lane) where there would be fewer workgroups than fill the chip.
-void cut(Logits *in, unsigned most, unsigned least) {
+void cut(Logits *in, unsigned most, unsigned least, size_t wgs) {
     const size_t all = static_cast<size_t>(in->vocab) + in->odd;
     size_t nseg = (all + most - 1) / most;
-    const size_t want = (4 * device_cus() + in->rows - 1) / in->rows, can = (all + least - 1) / least;
+    const size_t want = (wgs + in->rows - 1) / in->rows, can = (all + least - 1) / least;
     if (nseg < want) nseg = want < can ? want : can;
     const size_t len = (all + nseg - 1) / nseg;
     in->seglen = static_cast<unsigned>((len + 63) / 64 * 64);
@@ -886,7 +910,9 @@ int stats(StatArgs a, cxm_stream_t st) {
     a.in.nseg = 1;
     a.in.seglen = (a.in.vocab + a.in.odd + 63) / 64 * 64;
     const bool wave = a.in.vocab < static_cast<unsigned>(VE) || wave_rows(a.in, VE, kStatChunks);
-    if (!wave) cut(&a.in, kBlock * VE * kStatChunks, kBlock * VE);
+    // with top tokens fewer and larger segments, since joining them takes longer: 16 rows of 131072 bf16 and 64
+    // tokens 22.9 us on 256 workgroups, 25.7 on 512
+    if (!wave) cut(&a.in, kBlock * VE * kStatChunks, kBlock * VE * (TOP ? 2 : 1), (TOP ? 1 : 4) * device_cus());
     if (a.in.nseg > most_wgs(kBlock) / a.in.rows) return CXM_E_TOO_LARGE;
     if (wave) {
         return a.in.vocab < static_cast<unsigned>(VE) ? stats_launch<DT, 1, 64, ENT, TOP>(a, hs(st))
@@ -895,7 +921,9 @@ int stats(StatArgs a, cxm_stream_t st) {
     if (a.in.nseg > 1) {
         const size_t segs = a.in.rows * a.in.nseg, o_bars = (segs * sizeof(Part) + 255) / 256 * 256;
         const size_t o_cands = o_bars + (TOP ? (segs * 2 * sizeof(float) + 255) / 256 * 256 : 0);
-        a.keep = a.top + a.top / 4 + 12;
+        a.keep = a.top + a.top / 2 + 12;
+        a.rth = (2 * a.top + a.in.nseg - 1) / a.in.nseg;
+        a.need = TOP ? (a.top + a.rth - 1) / a.rth : 0;
         Workspace ws;
         const int rc = get_workspace(st, (a.in.rows * kTicket + kCtr - 1) / kCtr,
                                      o_cands + (TOP ? segs * a.keep * sizeof(ArgPair) : 0), &ws);
@@ -935,7 +963,7 @@ int grad(GradArgs a, cxm_stream_t st) {
     a.in.nseg = 1;
     a.in.seglen = (a.in.vocab + a.in.odd + 63) / 64 * 64;
     const bool wave = a.in.vocab < static_cast<unsigned>(VE) || wave_rows(a.in, VE, kGradChunks);
-    if (!wave) cut(&a.in, kBlock * VE * kGradChunks, kBlock * VE);
+    if (!wave) cut(&a.in, kBlock * VE * kGradChunks, kBlock * VE, 4 * device_cus());
     if (a.in.nseg > most_wgs(kBlock) / a.in.rows) return CXM_E_TOO_LARGE;
     if (a.in.vocab < static_cast<unsigned>(VE)) return grad_launch<DT, 1, 64, DISTILL, ENT>(a, hs(st));
     return wave ? grad_launch<DT, VE, 64, DISTILL, ENT>(a, hs(st)) : grad_launch<DT, VE, kBlock, DISTILL, ENT>(a, hs(st));

@@ -6,11 +6,11 @@
 // Both are bound by memory.  The gradient's tokens are sorted by id first, so
 // that every row of dw is one sum in the order of the tokens (no atomics on
 // floats: the same bits every time) and is written once.  Two launches:
-//  * k_embed_sort: a workgroup owns a range of ids.  It reads all ids twice
-//    (they lie in L2), counts those below its range, which says where its part
-//    of the sorted list begins, and places those in it in order; the rows that
-//    no token has become zero in the same launch.
-//  * k_embed_sum: a wave takes up to L neighbours of the sorted list and a tile
+//  * k_embed_sort: a workgroup owns every 2^n-th id.  It reads all ids twice
+//    (they lie in L2), counts those of the owners before it, which says where its
+//    part of the sorted list begins, and places its own in order; the rows
+//    that no token has become zero in the same launch.
+//  * k_embed_sum: a wave takes up to 16 neighbours of the sorted list and a tile
 //    of columns, and writes the rows of ids that lie within its part; what an
 //    id's tokens give in several waves meets in LDS, in several workgroups in
 //    scratch, added up by the last of them to arrive, in the list's order.
@@ -21,16 +21,33 @@ namespace {
 
 inline hipStream_t hs(cxm_stream_t s) { return reinterpret_cast<hipStream_t>(s); }
 
+// Workgroup b of a grid goes to XCD b mod 8.  Row pieces of a power of two then
+// fall to an XCD with the same part of every row each time, and so to the same
+// few channels of its L2: number the workgroups so that an XCD's take
+// neighbouring pieces (32768 tokens of 2048 bf16 at 1 KiB a piece: MEASURED).
+struct Spread {
+    unsigned n, xcds, each;  // pieces, XCDs, pieces of an XCD
+    __device__ unsigned piece() const { return blockIdx.x % xcds * each + blockIdx.x / xcds; }  // n or more: none
+};
+// The grid is xcds * each workgroups.
+Spread spread_of(unsigned n) {
+    DevLayout l{0, 1};
+    const unsigned xcds = device_layout(&l) == CXM_OK && l.xccs > 0 ? static_cast<unsigned>(l.xccs) : 1;
+    return {n, xcds, (n + xcds - 1) / xcds};
+}
+
 // ---------------------------------------------------------------- forward
 
 // G lanes per row piece of G chunks, U tokens per group of lanes.
 template <int DT, int VE, int G, int U>
 __global__ __launch_bounds__(kBlock) void k_embed(const typename Elem<DT>::S *table, const int32_t *ids, float scale,
                                                   typename Elem<DT>::S *y, size_t tokens, size_t vocab, unsigned cols,
-                                                  unsigned tiles) {
+                                                  unsigned tiles, Spread spread) {
     constexpr int R = kBlock / G;
-    const size_t blk = blockIdx.x / tiles;
-    const unsigned tile = blockIdx.x - static_cast<unsigned>(blk) * tiles;
+    const unsigned piece = spread.piece();
+    if (piece >= spread.n) return;
+    const size_t blk = piece / tiles;
+    const unsigned tile = piece - static_cast<unsigned>(blk) * tiles;
     const Span s = span_of<VE>(tile * G + threadIdx.x % G, cols);
     const size_t first = (blk * R + threadIdx.x / G) * U;
     int id[U];
@@ -61,9 +78,10 @@ int fwd_launch(const void *table, const int32_t *ids, float scale, void *y, size
     using S = typename Elem<DT>::S;
     const unsigned tiles = ceil_div(ceil_div(cols, VE), G);
     const size_t blks = (tokens + static_cast<size_t>(kBlock / G) * U - 1) / (static_cast<size_t>(kBlock / G) * U);
-    if (blks > most_wgs(kBlock) / tiles) return CXM_E_TOO_LARGE;
-    hipLaunchKernelGGL((k_embed<DT, VE, G, U>), dim3(static_cast<unsigned>(blks * tiles)), dim3(kBlock), 0, s,
-                       static_cast<const S *>(table), ids, scale, static_cast<S *>(y), tokens, vocab, cols, tiles);
+    if (blks > (most_wgs(kBlock) - kCtr) / tiles) return CXM_E_TOO_LARGE;  // (fewer than 64 XCDs round the grid up)
+    const Spread spread = spread_of(static_cast<unsigned>(blks * tiles));
+    hipLaunchKernelGGL((k_embed<DT, VE, G, U>), dim3(spread.xcds * spread.each), dim3(kBlock), 0, s,
+                       static_cast<const S *>(table), ids, scale, static_cast<S *>(y), tokens, vocab, cols, tiles, spread);
     return launch_status();
 }
 
@@ -85,16 +103,27 @@ struct Place {
 };
 
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
-constexpr unsigned kSortIds = 512;  // most ids of a workgroup
-constexpr int kSortAhead = 8;       // groups of 64 ids in flight
+constexpr unsigned kSortIds = 256;  // most ids of a workgroup
+constexpr unsigned kPending = 256 + kWave;  // tokens that a wave holds back until it has 64
+constexpr int kSortAhead = 4;       // groups of 256 ids in flight
+typedef int i32x4e __attribute__((ext_vector_type(4), aligned(4)));
+
+// The sorted list's order: owner by owner (the id's low `bits` bits), an
+// owner's ids in turn.  The ids that a text uses most are neighbours (small, as
+// a rule), and so have an owner each.
+struct Order {
+    unsigned bits, range;  // 2^bits owners of at most `range` ids
+    __host__ __device__ unsigned number(unsigned id) const { return (id & ((1u << bits) - 1)) * range + (id >> bits); }
+};
 
 struct SortArgs {
     const int32_t *ids;
-    size_t tokens, vocab;
-    unsigned range;        // ids per workgroup, at most kSortIds
-    Place *sorted;         // [tokens]
-    unsigned *starts;      // [vocab + 1]: where each id's tokens begin
-    char *dw;              // null: accumulating, nothing becomes zero
+    size_t tokens;
+    unsigned vocab;
+    Order order;
+    Place *sorted;     // [tokens]
+    unsigned *starts;  // [owners * range + 1]: where each id's tokens begin
+    char *dw;          // null: accumulating, nothing becomes zero
     size_t row_bytes;
 };
 
@@ -106,45 +135,71 @@ __device__ __forceinline__ void zero_row(char *p, size_t n, unsigned lane) {
     if (at < n) *reinterpret_cast<uint16_t *>(p + at) = 0;
 }
 
+// Half of the waves write the zeros of absent ids while the other half place the
+// tokens; without zeros all of them place.
 __global__ __launch_bounds__(kSortThreads) void k_embed_sort(SortArgs a) {
-    __shared__ unsigned hist[kSortWaves][kSortIds];
+    __shared__ unsigned hist[kSortWaves * kSortIds];  // [wave][id]
     __shared__ unsigned wsum[kSortWaves], below_all;
     __shared__ unsigned long long absent[kSortIds / kWave];  // a bit for each id that no token has
-    const unsigned lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const size_t v0 = static_cast<size_t>(blockIdx.x) * a.range;
-    const unsigned range = static_cast<unsigned>(a.vocab - v0 < a.range ? a.vocab - v0 : a.range);
-    const size_t per = (a.tokens + kSortThreads - 1) / kSortThreads * kWave;  // a wave's tokens, in a row
-    const size_t t0 = wave * per < a.tokens ? wave * per : a.tokens, t1 = t0 + per < a.tokens ? t0 + per : a.tokens;
-    for (unsigned i = threadIdx.x; i < kSortWaves * kSortIds; i += kSortThreads) (&hist[0][0])[i] = 0;
+    __shared__ Place pending[kSortWaves][kPending];
+    const unsigned lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const unsigned owner = blockIdx.x, mask = (1u << a.order.bits) - 1, shift = a.order.bits, cap = a.order.range;
+    const unsigned range = owner < a.vocab ? ((a.vocab - owner - 1) >> shift) + 1 : 0;  // its ids: owner, owner + owners, ...
+    // a wave's tokens, in a row: whole groups of 4 for all lanes but the last ones
+    const size_t per = (a.tokens + 4 * kSortThreads - 1) / (4 * kSortThreads) * 4 * kWave;
+    for (unsigned i = threadIdx.x; i < kSortWaves * cap; i += kSortThreads) hist[i] = 0;
     if (threadIdx.x == 0) below_all = 0;
     __syncthreads();
-    // ids[i], or -1 (no id) past the wave's part
-    auto batch = [&](size_t at, int(&id)[kSortAhead]) {
+    // four ids a lane, -1 (no id) past a wave's part
+    auto batch = [&](size_t at, size_t end, int(&id)[kSortAhead][4]) {
 #pragma unroll
         for (int k = 0; k < kSortAhead; ++k) {
-            const size_t i = at + k * kWave + lane;
-            id[k] = i < t1 ? a.ids[i] : -1;
+            const size_t i = at + (k * kWave + lane) * 4;
+            if (i + 4 <= end) {
+                const i32x4e v = *reinterpret_cast<const i32x4e *>(a.ids + i);
+                id[k][0] = v.x; id[k][1] = v.y; id[k][2] = v.z; id[k][3] = v.w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) id[k][j] = i + j < end ? a.ids[i + j] : -1;
+            }
         }
     };
+    auto end_of = [&](size_t from) { return from + per < a.tokens ? from + per : a.tokens; };
+    // an id's owner (of no id: none)
+    auto owner_of = [&](int id) { return static_cast<unsigned>(id) < a.vocab ? static_cast<unsigned>(id) & mask : ~0u; };
     unsigned below = 0;
-    for (size_t at = t0; at < t1; at += kSortAhead * kWave) {
-        int id[kSortAhead];
-        batch(at, id);
+    for (size_t t0 = wave * per, t1 = end_of(t0), at = t0; at < t1; at += kSortAhead * kWave * 4) {
+        int id[kSortAhead][4];
+        batch(at, t1, id);
 #pragma unroll
-        for (int k = 0; k < kSortAhead; ++k) {
-            const long long r = static_cast<long long>(id[k]) - static_cast<long long>(v0);
-            below += id[k] >= 0 && r < 0;
-            if (r >= 0 && r < range) atomicAdd(&hist[wave][r], 1u);
-        }
+        for (int k = 0; k < kSortAhead; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const unsigned o = owner_of(id[k][j]);
+                below += o < owner;
+                const bool mine = o == owner;
+                const unsigned long long in = __ballot(mine);
+                if (in == 0) continue;
+                const unsigned key = static_cast<unsigned>(id[k][j]) >> shift;
+                if (__popcll(in) < 24) {
+                    if (mine) atomicAdd(&hist[wave * cap + key], 1u);
+                } else {  // those of the first one's id together: a text that is mostly one id would queue up here
+                    const unsigned one = readlane(static_cast<int>(key), __builtin_ctzll(in));
+                    const unsigned long long same = __ballot(mine && key == one);
+                    if (mine && key != one) atomicAdd(&hist[wave * cap + key], 1u);
+                    if (lane == __builtin_ctzll(same)) atomicAdd(&hist[wave * cap + one], static_cast<unsigned>(__popcll(same)));
+                }
+            }
     }
-    atomicAdd(&below_all, below);
+    for (int d = 1; d < kWave; d *= 2) below += __shfl_xor(below, d);
+    if (lane == 0) atomicAdd(&below_all, below);
     __syncthreads();
     // where each wave's tokens of each id go: ids in turn, within one the waves in turn
     const unsigned r = threadIdx.x;
     unsigned total = 0;
     if (r < range) {
 #pragma unroll
-        for (int w = 0; w < kSortWaves; ++w) total += hist[w][r];
+        for (int w = 0; w < kSortWaves; ++w) total += hist[w * cap + r];
     }
     unsigned incl = total;
 #pragma unroll
@@ -153,54 +208,93 @@ __global__ __launch_bounds__(kSortThreads) void k_embed_sort(SortArgs a) {
         if (lane >= static_cast<unsigned>(d)) incl += o;
     }
     if (lane == kWave - 1) wsum[wave] = incl;
-    __syncthreads();
-    unsigned at = below_all + incl - total;
-    for (unsigned w = 0; w < wave; ++w) at += wsum[w];
-    if (r < range) {
-        a.starts[v0 + r] = at;
-        if (v0 + r + 1 == a.vocab) a.starts[a.vocab] = at + total;
-        for (int w = 0; w < kSortWaves; ++w) {
-            const unsigned n = hist[w][r];
-            hist[w][r] = at;
-            at += n;
-        }
-    }
     const unsigned long long none = __ballot(r < range && total == 0);
     if (lane == 0 && wave < kSortIds / kWave) absent[wave] = none;
     __syncthreads();
-    const int bits = 32 - __clz((range - 1) | 1);
-    for (size_t base = t0; base < t1; base += kSortAhead * kWave) {
-        int id[kSortAhead];
-        batch(base, id);
-#pragma unroll
-        for (int k = 0; k < kSortAhead; ++k) {
-            const long long d = static_cast<long long>(id[k]) - static_cast<long long>(v0);
-            const bool in = d >= 0 && d < range;
-            unsigned long long same = __ballot(in);
-            if (same == 0) continue;
-            const unsigned key = in ? static_cast<unsigned>(d) : 0;
-            for (int b = 0; b < bits; ++b) {  // the lanes that have this lane's id
-                const unsigned long long one = __ballot(key >> b & 1);
-                same &= key >> b & 1 ? one : ~one;
+    unsigned at = below_all + incl - total;
+    for (unsigned w = 0; w < wave; ++w) at += wsum[w];
+    if (r < cap) {  // (past its last id: where the next owner's begin)
+        a.starts[owner * cap + r] = at;
+        if (owner == mask && r + 1 == cap) a.starts[owner * cap + cap] = at + total;
+    }
+    if (r < range) {
+        for (int w = 0; w < kSortWaves; ++w) {
+            const unsigned n = hist[w * cap + r];
+            hist[w * cap + r] = at;
+            at += n;
+        }
+    }
+    __syncthreads();
+    const unsigned placers = a.dw ? kSortWaves / 2 : kSortWaves;
+    if (wave >= placers) {
+        for (unsigned i = wave - placers; i < range; i += kSortWaves - placers)
+            if (absent[i / kWave] >> (i % kWave) & 1)
+                zero_row(a.dw + (owner + (static_cast<size_t>(i) << shift)) * a.row_bytes, a.row_bytes, lane);
+        return;
+    }
+    // A wave's own tokens are first put together, in order, and placed 64 at a time: the owner of a text's
+    // most frequent ids has them in every group (placed group by group, one id after the other, 131072 tokens
+    // took MEASURED us more).
+    const unsigned parts = kSortWaves / placers;
+    Place *held = pending[wave];
+    const int key_bits = 32 - __clz((cap - 1) | 1);
+    for (unsigned w = wave * parts; w < (wave + 1) * parts; ++w) {
+        unsigned have = 0;
+        auto place = [&](unsigned at, unsigned n) {  // held[at .. at + n), n <= 64
+            const Place mine = held[at + (lane < n ? lane : 0)];
+            const unsigned key = static_cast<unsigned>(mine.id) >> shift;
+            unsigned long long same = __ballot(lane < n);
+            if (__any(key != static_cast<unsigned>(readlane(static_cast<int>(key), 0)))) {
+                for (int b = 0; b < key_bits; ++b) {  // the lanes that have this lane's id
+                    const unsigned long long one = __ballot(key >> b & 1);
+                    same &= key >> b & 1 ? one : ~one;
+                }
             }
-            if (in) {
-                const unsigned rank = __popcll(same & ((1ull << lane) - 1));
-                const unsigned to = hist[wave][key] + rank;
-                a.sorted[to] = Place{id[k], static_cast<int>(base + k * kWave + lane)};
-                // one lane moves the place on, after all have read it and before the next group does
+            const unsigned rank = __popcll(same & ((1ull << lane) - 1)), to = hist[w * cap + key];
+            // every lane has read the place before it moves on, and the next reader sees it moved
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (lane < n) {
+                a.sorted[to + rank] = mine;
+                if (rank == 0) hist[w * cap + key] = to + __popcll(same);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        };
+        for (size_t t0 = w * per, t1 = end_of(t0), base = t0; base < t1; base += kSortAhead * kWave * 4) {
+            int id[kSortAhead][4];
+            batch(base, t1, id);
+#pragma unroll
+            for (int k = 0; k < kSortAhead; ++k) {
+                unsigned long long in[4], any = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) any |= in[j] = __ballot(owner_of(id[k][j]) == owner);
+                if (!any) continue;
+                unsigned rank = have, more = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    rank += __popcll(in[j] & ((1ull << lane) - 1));
+                    more += __popcll(in[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (in[j] >> lane & 1) held[rank++] = Place{id[k][j], static_cast<int>(base + (k * kWave + lane) * 4 + j)};
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                if (rank == 0) hist[wave][key] = to + __popcll(same);
+                have += more;
+                if (have < kWave) continue;
+                unsigned at = 0;
+                for (; have - at >= kWave; at += kWave) place(at, kWave);
+                have -= at;
+                const Place rest = held[at + (lane < have ? lane : 0)];
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                if (lane < have) held[lane] = rest;
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             }
         }
-    }
-    if (a.dw) {
-        for (unsigned i = wave; i < range; i += kSortWaves)
-            if (absent[i / kWave] >> (i % kWave) & 1) zero_row(a.dw + (v0 + i) * a.row_bytes, a.row_bytes, lane);
+        if (have) place(0, have);
     }
 }
 
 constexpr int kSumThreads = 512, kSumWaves = kSumThreads / kWave;
+constexpr int kPlaces = 16;     // most places of a wave, all of their rows in flight
 constexpr size_t kTicket = 16;  // words between two of its tickets
 
 struct SumArgs {
@@ -211,27 +305,33 @@ struct SumArgs {
     float *part;        // [spans][2][tiles * 64 * VE]: what an id's tokens give in a span, of the id that
                         // began before it and of the one that goes on after it
     unsigned *tickets;  // [spans * tiles], kTicket apart
-    size_t vocab;
-    unsigned cols, tiles, per;  // per: a wave's places
+    Order order;
+    unsigned ends;  // owners * range: starts[ends] places are in the list
+    unsigned tokens, cols, tiles, per;  // per: a wave's places
     float scale;
     int accumulate;
+    Spread spread;
 };
 
 template <int DT, int GT, int VE>
 __global__ __launch_bounds__(kSumThreads) void k_embed_sum(SumArgs a) {
     using S = typename Elem<DT>::S;
     using SG = typename Elem<GT>::S;
-    constexpr int AH = 8;  // rows in flight
     __shared__ float head[kSumWaves][VE][kWave], tail[kSumWaves][VE][kWave];
     // of each wave: 1 its first id began before it, 2 that id also goes on after it, 4 its last id began in it and goes on
     __shared__ int kind[kSumWaves];
-    __shared__ int last_id[kSumWaves], flag;
+    __shared__ int first_id[kSumWaves], last_id[kSumWaves], flag;
     const unsigned lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const unsigned span = blockIdx.x / a.tiles, tile = blockIdx.x - span * a.tiles;
-    const unsigned all = a.starts[a.vocab];
-    const unsigned from = span * (kSumWaves * a.per);
+    const unsigned piece = a.spread.piece();
+    if (piece >= a.spread.n) return;
+    const unsigned span = piece / a.tiles, tile = piece - span * a.tiles;
+    const unsigned places = kSumWaves * a.per, from = span * places, begin = from + wave * a.per;
+    // the wave's places, with one before them (lane 0) and one behind
+    const unsigned p = begin + lane - 1;
+    const Place mine = a.sorted[p < a.tokens ? p : 0];
+    const unsigned all = a.starts[a.ends];
     if (from >= all) return;
-    const unsigned p0 = from + wave * a.per < all ? from + wave * a.per : all, p1 = p0 + a.per < all ? p0 + a.per : all;
+    const unsigned p0 = begin < all ? begin : all, p1 = p0 + a.per < all ? p0 + a.per : all, n = p1 - p0;
     const unsigned col = tile * kWave + lane;
     const Span s = span_of<VE>(col, a.cols);
     const S *dy = static_cast<const S *>(a.dy) + s.off;
@@ -246,6 +346,7 @@ __global__ __launch_bounds__(kSumThreads) void k_embed_sum(SumArgs a) {
         for (int h = 0; h < VE / VG; ++h) {
             Chunk<GT, VG> c;
             float t[VG];
+            // (reading a wave's rows of dw with its rows of dy took no less time, in half as many waves)
             if (a.accumulate) c.load(row + s.off + h * VG);
 #pragma unroll
             for (int e = 0; e < VG; ++e) t[e] = a.accumulate ? c.get(e) + v[h * VG + e] : v[h * VG + e];
@@ -254,50 +355,48 @@ __global__ __launch_bounds__(kSumThreads) void k_embed_sum(SumArgs a) {
             store_span<GT, VG>(row, Span{s.off + h * VG, dup}, c);
         }
     };
-    float acc[VE];
-#pragma unroll
-    for (int e = 0; e < VE; ++e) acc[e] = 0.0f;
     int k = 0, cur = -1;
-    if (p0 < p1) {
-        const unsigned n = p1 - p0;
-        bool began = true;  // whether the id being added up began in this wave
-        for (unsigned b0 = 0; b0 < n; b0 += kWave) {
-            const unsigned m = n - b0 < kWave ? n - b0 : kWave;
-            const Place mine = a.sorted[p0 + b0 + (lane < m ? lane : m - 1)];
-            if (b0 == 0) {
-                cur = readlane(mine.id, 0);
-                began = a.starts[cur] == p0;
-            }
-            for (unsigned i0 = 0; i0 < m; i0 += AH) {
-                Chunk<DT, VE> c[AH];
+    if (n) {
+        Chunk<DT, VE> c[kPlaces];
+        // all row numbers before the first branch: after one the compiler waits for every load in flight before
+        // it reads the places again (the sums took 70 us instead of MEASURED)
+        unsigned row[kPlaces];
+        int ids[kPlaces];
 #pragma unroll
-                for (int u = 0; u < AH; ++u) {
-                    const unsigned i = i0 + u < m ? i0 + u : m - 1;
-                    c[u].load(dy + static_cast<size_t>(static_cast<unsigned>(readlane(mine.token, i))) * a.cols);
-                }
-#pragma unroll
-                for (int u = 0; u < AH; ++u) {
-                    if (i0 + u >= m) break;
-                    const int id = readlane(mine.id, i0 + u);
-                    if (id != cur) {
-                        if (began) {
-                            finish(cur, acc);
-                        } else {
-                            k |= 1;
-#pragma unroll
-                            for (int e = 0; e < VE; ++e) head[wave][e][lane] = acc[e];
-                        }
-#pragma unroll
-                        for (int e = 0; e < VE; ++e) acc[e] = 0.0f;
-                        cur = id;
-                        began = true;
-                    }
-#pragma unroll
-                    for (int e = 0; e < VE; ++e) acc[e] += c[u].get(e);
-                }
-            }
+        for (int u = 0; u < kPlaces; ++u) {
+            row[u] = static_cast<unsigned>(readlane(mine.token, u + 1));
+            ids[u] = readlane(mine.id, u + 1);
         }
-        const bool ends = a.starts[cur + 1] <= p1;
+#pragma unroll
+        for (int u = 0; u < kPlaces; ++u)
+            if (u < static_cast<int>(n)) c[u].load_nt(dy + static_cast<size_t>(row[u]) * a.cols);
+        float acc[VE];
+#pragma unroll
+        for (int e = 0; e < VE; ++e) acc[e] = 0.0f;
+        cur = readlane(mine.id, 1);
+        if (lane == 0) first_id[wave] = cur;
+        bool began = p0 == 0 || readlane(mine.id, 0) != cur;  // whether the id being added up began in this wave
+#pragma unroll
+        for (int u = 0; u < kPlaces; ++u) {
+            if (u >= static_cast<int>(n)) continue;
+            const int id = ids[u];
+            if (id != cur) {
+                if (began) {
+                    finish(cur, acc);
+                } else {
+                    k |= 1;
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) head[wave][e][lane] = acc[e];
+                }
+#pragma unroll
+                for (int e = 0; e < VE; ++e) acc[e] = 0.0f;
+                cur = id;
+                began = true;
+            }
+#pragma unroll
+            for (int e = 0; e < VE; ++e) acc[e] += c[u].get(e);
+        }
+        const bool ends = p1 >= all || readlane(mine.id, n + 1) != cur;
         if (began && ends) {
             finish(cur, acc);
         } else if (began) {
@@ -345,35 +444,40 @@ __global__ __launch_bounds__(kSumThreads) void k_embed_sum(SumArgs a) {
         chain(0, sum);
         publish(0, sum);
     }
-    // An id in several workgroups: the last of them to have stored its part adds them up.
-    const unsigned places = kSumWaves * a.per, to = from + places < all ? from + places : all;
-    const int ids[2] = {a.sorted[from].id, a.sorted[to - 1].id};
+    // An id in several workgroups: the last of them to have stored its part adds them up.  (0: it began before
+    // this workgroup; 1: it began here and goes on.)
+    const int last_wave = static_cast<int>(((from + places < all ? from + places : all) - from - 1) / a.per);
+    int w0 = last_wave;  // where the last id began
+    while (w0 >= 0 && (kind[w0] & 2)) --w0;
+    const bool before = kind[0] & 1, after = w0 >= 0 && (kind[w0] & 4);
     for (int which = 0; which < 2; ++which) {
-        const unsigned s0 = a.starts[ids[which]], s1 = a.starts[ids[which] + 1];
-        const unsigned g0 = s0 / places, g1 = (s1 - 1) / places;
-        // 0: it began before this workgroup; 1: it began here and goes on
-        if (which == 0 ? g0 == span : (g0 != span || g1 == span)) continue;
-        const bool last = last_block_ticket(a.tickets + (static_cast<size_t>(g0) * a.tiles + tile) * kTicket, g1 - g0 + 1, &flag);
+        if (!(which == 0 ? before : after)) continue;
+        const int id = which == 0 ? first_id[0] : last_id[last_wave];
+        const unsigned q = a.order.number(static_cast<unsigned>(id));
+        const unsigned s0 = a.starts[q], s1 = a.starts[q + 1];
+        const unsigned g0 = s0 / places, count = (s1 - 1) / places - g0 + 1;
+        const bool last = last_block_ticket(a.tickets + (static_cast<size_t>(g0) * a.tiles + tile) * kTicket, count, &flag);
         if (!last) continue;
         // each wave a run of the parts, one after the other
-        const unsigned count = g1 - g0 + 1, each = (count + kSumWaves - 1) / kSumWaves;
+        const unsigned each = (count + kSumWaves - 1) / kSumWaves;
         const unsigned c0 = wave * each < count ? wave * each : count, c1 = c0 + each < count ? c0 + each : count;
         float sum[VE];
 #pragma unroll
         for (int e = 0; e < VE; ++e) sum[e] = 0.0f;
-        for (unsigned c = c0; c < c1; c += 2) {
-            float v[2][VE];
+        constexpr int U = 8;
+        for (unsigned c = c0; c < c1; c += U) {
+            float v[U][VE];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < U; ++u) {
                 const unsigned cc = c + u < c1 ? c + u : c;
-                const float *p = a.part + (static_cast<size_t>(g0 + cc) * 2 + (cc == 0 ? 1 : 0)) * width +
-                                 static_cast<size_t>(tile) * kWave * VE + lane;
+                const float *at = a.part + (static_cast<size_t>(g0 + cc) * 2 + (cc == 0 ? 1 : 0)) * width +
+                                  static_cast<size_t>(tile) * kWave * VE + lane;
 #pragma unroll
-                for (int e = 0; e < VE; ++e) v[u][e] = ld_dev(p + e * kWave);
+                for (int e = 0; e < VE; ++e) v[u][e] = ld_dev(at + e * kWave);
             }
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                if (c + u >= c1) break;
+            for (int u = 0; u < U; ++u) {
+                if (c + u >= c1) continue;
 #pragma unroll
                 for (int e = 0; e < VE; ++e) sum[e] += v[u][e];
             }
@@ -386,7 +490,7 @@ __global__ __launch_bounds__(kSumThreads) void k_embed_sum(SumArgs a) {
             for (int w = 1; w < kSumWaves; ++w)
 #pragma unroll
                 for (int e = 0; e < VE; ++e) sum[e] += head[w][e][lane];
-            finish(ids[which], sum);
+            finish(id, sum);
         }
         __syncthreads();
     }
@@ -395,8 +499,8 @@ __global__ __launch_bounds__(kSumThreads) void k_embed_sum(SumArgs a) {
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 template <int DT, int GT, int VE>
-int sum_launch(SumArgs a, size_t wgs, hipStream_t s) {
-    hipLaunchKernelGGL((k_embed_sum<DT, GT, VE>), dim3(static_cast<unsigned>(wgs)), dim3(kSumThreads), 0, s, a);
+int sum_launch(const SumArgs &a, hipStream_t s) {
+    hipLaunchKernelGGL((k_embed_sum<DT, GT, VE>), dim3(a.spread.xcds * a.spread.each), dim3(kSumThreads), 0, s, a);
     return launch_status();
 }
 
@@ -406,17 +510,21 @@ int bwd(const int32_t *ids, const void *dy, float scale, void *dw, int accumulat
     constexpr int VE = Elem<DT>::kVec;
     const bool narrow = cols < static_cast<unsigned>(VE);
     const unsigned ve = narrow ? 1 : VE, tiles = ceil_div(ceil_div(cols, ve), kWave);
-    // ids per workgroup of the sort: one round of workgroups on the chip
+    // owners: a power of two of them, one round of workgroups on the chip unless each would have too many ids
     const size_t cus = device_cus();
-    size_t range = (vocab + cus - 1) / cus;
-    range = range < kSortIds ? range : kSortIds;
-    const size_t sorters = (vocab + range - 1) / range;
-    // a wave's places: enough waves to fill the chip, few enough that ids seldom meet in scratch
-    size_t per = tokens * tiles / (cus * 16);
-    per = per < 8 ? 8 : per > 128 ? 128 : per;
+    Order order{0, 0};
+    while ((size_t(2) << order.bits) <= vocab &&
+           ((size_t(2) << order.bits) <= cus || (vocab + (size_t(1) << order.bits) - 1) >> order.bits > kSortIds))
+        ++order.bits;
+    const size_t owners = size_t(1) << order.bits;
+    order.range = static_cast<unsigned>((vocab + owners - 1) >> order.bits);
+    // a wave's places: as many as are in flight at once, fewer where that leaves CUs without work
+    size_t per = kPlaces;
+    while (per > 4 && tokens * tiles < per * kSumWaves * cus) per /= 2;
     const size_t spans = (tokens + per * kSumWaves - 1) / (per * kSumWaves);
-    if (sorters > most_wgs(kSortThreads) || spans > most_wgs(kSumThreads) / tiles) return CXM_E_TOO_LARGE;
-    const size_t o_starts = align256(tokens * sizeof(Place)), o_part = o_starts + align256((vocab + 1) * sizeof(unsigned));
+    if (owners > most_wgs(kSortThreads) || spans > (most_wgs(kSumThreads) - kCtr) / tiles) return CXM_E_TOO_LARGE;
+    const size_t ends = owners * order.range;
+    const size_t o_starts = align256(tokens * sizeof(Place)), o_part = o_starts + align256((ends + 1) * sizeof(unsigned));
     const size_t bytes = o_part + spans * 2 * tiles * kWave * ve * sizeof(float);
     Workspace ws;
     const int rc = get_workspace(st, (spans * tiles * kTicket + kCtr - 1) / kCtr, bytes, &ws);
@@ -424,18 +532,31 @@ int bwd(const int32_t *ids, const void *dy, float scale, void *dw, int accumulat
     char *base = static_cast<char *>(ws.scratch);
     const SortArgs so{ids,
                       tokens,
-                      vocab,
-                      static_cast<unsigned>(range),
+                      static_cast<unsigned>(vocab),
+                      order,
                       reinterpret_cast<Place *>(base),
                       reinterpret_cast<unsigned *>(base + o_starts),
                       accumulate ? nullptr : static_cast<char *>(dw),
                       cols * sizeof(typename Elem<GT>::S)};
-    hipLaunchKernelGGL(k_embed_sort, dim3(static_cast<unsigned>(sorters)), dim3(kSortThreads), 0, hs(st), so);
+    hipLaunchKernelGGL(k_embed_sort, dim3(static_cast<unsigned>(owners)), dim3(kSortThreads), 0, hs(st), so);
     int r = launch_status();
     if (r || tokens == 0) return r;
-    const SumArgs sa{dy,    dw,   so.sorted, so.starts, reinterpret_cast<float *>(base + o_part), ws.counters, vocab, cols,
-                     tiles, static_cast<unsigned>(per), scale, accumulate};
-    return narrow ? sum_launch<DT, GT, 1>(sa, spans * tiles, hs(st)) : sum_launch<DT, GT, VE>(sa, spans * tiles, hs(st));
+    const SumArgs sa{dy,
+                     dw,
+                     so.sorted,
+                     so.starts,
+                     reinterpret_cast<float *>(base + o_part),
+                     ws.counters,
+                     order,
+                     static_cast<unsigned>(ends),
+                     static_cast<unsigned>(tokens),
+                     cols,
+                     tiles,
+                     static_cast<unsigned>(per),
+                     scale,
+                     accumulate,
+                     spread_of(static_cast<unsigned>(spans * tiles))};
+    return narrow ? sum_launch<DT, GT, 1>(sa, hs(st)) : sum_launch<DT, GT, VE>(sa, hs(st));
 }
 
 // Sizes that the kernels number in 32 bits, and whose bytes fit 64.

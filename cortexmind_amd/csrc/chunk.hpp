@@ -73,6 +73,10 @@ struct Chunk<CXM_DT_F32, VE> {
         if constexpr (VE == 4) *reinterpret_cast<f32x4e *>(p) = f32x4e{r[0], r[1], r[2], r[3]};
         else *p = r[0];
     }
+    __device__ __forceinline__ void store_nt(float *p) const {
+        if constexpr (VE == 4) __builtin_nontemporal_store(f32x4e{r[0], r[1], r[2], r[3]}, reinterpret_cast<f32x4e *>(p));
+        else *p = r[0];
+    }
     __device__ __forceinline__ float raw(int e) const { return r[e]; }
 };
 template <int DT, int VE>
@@ -108,6 +112,10 @@ struct Chunk {
         if constexpr (VE == 8) *reinterpret_cast<u32x4e *>(p) = u32x4e{r[0], r[1], r[2], r[3]};
         else *p = static_cast<uint16_t>(r[0]);
     }
+    __device__ __forceinline__ void store_nt(uint16_t *p) const {
+        if constexpr (VE == 8) __builtin_nontemporal_store(u32x4e{r[0], r[1], r[2], r[3]}, reinterpret_cast<u32x4e *>(p));
+        else *p = static_cast<uint16_t>(r[0]);
+    }
 };
 
 // Where chunk number c of a row of n elements (n >= VE) lies: `off`, moved
@@ -123,11 +131,12 @@ __device__ __forceinline__ Span span_of(unsigned c, unsigned n) {
     const unsigned off = col < last ? col : last;
     return {off, col - off};
 }
-// Stores a chunk's own elements.
-template <int DT, int VE>
+// Stores a chunk's own elements (NT: whole ones with the non-temporal hint).
+template <int DT, int VE, bool NT = false>
 __device__ __forceinline__ void store_span(typename Elem<DT>::S *row, Span s, const Chunk<DT, VE> &v) {
     if (s.dup == 0) {
-        v.store(row + s.off);
+        if constexpr (NT) v.store_nt(row + s.off);
+        else v.store(row + s.off);
     } else if (s.dup < VE) {
 #pragma unroll
         for (int e = 1; e < VE; ++e)

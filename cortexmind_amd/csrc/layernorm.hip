@@ -42,7 +42,9 @@ __device__ __forceinline__ float ln_rstd(float ss, unsigned cols, float eps) {
 }
 
 // G lanes per row, C chunks of VE elements per lane, NT threads.  AL: rows of
-// whole 128-byte lines, read with the non-temporal hint.
+// whole 128-byte lines, read with the non-temporal hint; other rows are written
+// with it (5000 rows of 1003 floats 10.5 -> 8.1 us, 20001 of 1003 fp16 20.7 -> 18.7;
+// whole lines 4096x8192 44.6 -> 47.4).
 template <int DT, int VE, int G, int C, int NT, bool AL>
 __global__ __launch_bounds__(NT) void k_ln_fwd(LnFwd a) {
     using S = typename Elem<DT>::S;
@@ -83,7 +85,7 @@ __global__ __launch_bounds__(NT) void k_ln_fwd(LnFwd a) {
         if (a.h && live) {
             S *h = static_cast<S *>(a.h) + base;
 #pragma unroll
-            for (int i = 0; i < C; ++i) store_span<DT, VE>(h, s[i], cx[i]);
+            for (int i = 0; i < C; ++i) store_span<DT, VE, !AL>(h, s[i], cx[i]);
         }
     }
     float v[C][VE];
@@ -122,7 +124,7 @@ __global__ __launch_bounds__(NT) void k_ln_fwd(LnFwd a) {
 #pragma unroll
         for (int i = 0; i < C; ++i) {
             cx[i].set(v[i]);
-            store_span<DT, VE>(y, s[i], cx[i]);
+            store_span<DT, VE, !AL>(y, s[i], cx[i]);
         }
     }
     if (a.q) {
@@ -322,7 +324,7 @@ __global__ __launch_bounds__(NT) void k_ln_bwd(LnBwd a) {
                 }
                 Chunk<DT, VE> c;
                 c.set(t);
-                store_span<DT, VE>(dx, s[i], c);
+                store_span<DT, VE, !AL>(dx, s[i], c);
             }
         }
     }

@@ -355,6 +355,108 @@ __global__ __launch_bounds__(NT) void k_ln_bwd(LnBwd a) {
     share(ab, part + a.ld);
 }
 
+// The same for rows of up to 2048 chunks, a workgroup of 1024 per row, whose
+// registers are half as many: chunks stay packed until the output, the weights are
+// read for each use (from L1 or L2), places are computed anew, and only in fp32 is
+// the next row loaded ahead (16-bit then spills 17 registers: 2000x12288 94 us).
+// fp32 2000x6001 53.5 us (k_ln_bwd_long 66.3), bf16 2000x12288 69.4 (76.0),
+// 2000x12001 85.5 (92.1); but 100x16000, fewer rows than CUs, 32.8 (29.1).
+template <int DT, int C, bool AL>
+__global__ __launch_bounds__(1024) void k_ln_bwd_wide(LnBwd a) {
+    using S = typename Elem<DT>::S;
+    constexpr int VE = Elem<DT>::kVec, NT = 1024;
+    constexpr bool AHEAD = DT == CXM_DT_F32;
+    __shared__ Pair lds[NT / kWave];
+    const S *w = static_cast<const S *>(a.w);
+    float aw[C][VE], ab[C][VE];
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) aw[i][e] = ab[i][e] = 0.0f;
+    auto span = [&](int i) {
+        unsigned c = i * NT + threadIdx.x;
+        asm volatile("" : "+v"(c));
+        return span_of<VE>(c, a.cols);
+    };
+    struct Row {
+        Chunk<DT, VE> h[C], d[C], a[C];
+        float rs, mu;
+    };
+    auto load = [&](Row &q, size_t row) {
+        const size_t base = row * a.cols;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const unsigned off = span(i).off;
+            load_once<AL>(q.h[i], static_cast<const S *>(a.h) + base + off);
+            load_once<AL>(q.d[i], static_cast<const S *>(a.dy) + base + off);
+            if (a.dh) load_once<AL>(q.a[i], static_cast<const S *>(a.dh) + base + off);
+        }
+        q.rs = a.rstd[row];
+        q.mu = a.mean[row];
+    };
+    Row cur, next;
+    size_t row = blockIdx.x;
+    if constexpr (AHEAD) load(next, row);
+    for (; row < a.rows; row += gridDim.x) {
+        if constexpr (AHEAD) {
+            cur = next;
+            if (row + gridDim.x < a.rows) load(next, row + gridDim.x);
+        } else {
+            load(cur, row);
+        }
+        Pair dot{0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+            const Span s = span(i);
+            Chunk<DT, VE> cw;
+            cw.load(w + s.off);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+                const float n = (cur.h[i].get(e) - cur.mu) * cur.rs;
+                const float dy = e >= static_cast<int>(s.dup) ? cur.d[i].get(e) : 0.0f, g = dy * cw.get(e);
+                aw[i][e] = fmaf(dy, n, aw[i][e]);
+                ab[i][e] += dy;
+                dot.a += g;
+                dot.b = fmaf(g, n, dot.b);
+            }
+        }
+        dot = block_reduce<PairSumOp, NT>(dot, lds);
+        const float mg = dot.a / static_cast<float>(a.cols), mgn = dot.b / static_cast<float>(a.cols);
+        S *dx = static_cast<S *>(a.dx) + row * a.cols;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            // one chunk at a time, and what it unpacks to not kept from above: else 30 registers spill
+            __builtin_amdgcn_sched_barrier(0);
+            for (auto &r : cur.h[i].r) asm volatile("" : "+v"(r));
+            for (auto &r : cur.d[i].r) asm volatile("" : "+v"(r));
+            const Span s = span(i);
+            Chunk<DT, VE> cw;
+            cw.load(w + s.off);
+            float t[VE];
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+                const float n = (cur.h[i].get(e) - cur.mu) * cur.rs, g = cur.d[i].get(e) * cw.get(e);
+                const float r = cur.rs * (fmaf(-n, mgn, g) - mg);
+                t[e] = a.dh ? r + cur.a[i].get(e) : r;
+            }
+            cw.set(t);
+            store_span<DT, VE, !AL>(dx, s, cw);
+        }
+    }
+    float *part = a.part + static_cast<size_t>(blockIdx.x) * 2 * a.ld;
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+        const Span s = span(i);
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+            if (e >= static_cast<int>(s.dup)) {
+                part[s.off + e] = aw[i][e];
+                part[a.ld + s.off + e] = ab[i][e];
+            }
+    }
+}
+
 // Rows longer than these hold: dx by a workgroup per row, which reads the row
 // twice; dw and db by k_ln_dw_part, run before it (dx may be dy or h).
 template <int DT, int NT>
@@ -497,14 +599,21 @@ template <int DT, int VE, int G, int C, int NT>
 int bwd_launch(LnBwd a, void *dw, void *db, cxm_stream_t st) {
     constexpr int R = G <= kWave ? NT / G : 1;
     constexpr size_t E = sizeof(typename Elem<DT>::S);
-    const size_t wgs = bwd_wgs(a.rows, R);
+    // A workgroup's shares are 8 bytes a column, which it writes and col_sum2 reads: from 128 chunks a row on, one
+    // workgroup per CU instead of two (bf16 8192x2048 31.7 us instead of 36.7, 4096x8192 57.7 instead of 73.3, fp32
+    // 2048x4096 29.8 instead of 34.2; but bf16 30001x771 51.9 instead of 45.5).
+    const size_t wgs = bwd_wgs(a.rows, R, G * C > 128 ? 1 : 2);
     const int rc = bwd_parts(&a, wgs, st);
     if (rc) return rc;
     const dim3 grid(static_cast<unsigned>(wgs));
-    if (whole_lines(a.h, a.cols, E) && whole_lines(a.dy, a.cols, E) && whole_lines(a.dh, a.cols, E))
-        hipLaunchKernelGGL((k_ln_bwd<DT, VE, G, C, NT, true>), grid, dim3(NT), 0, hs(st), a);
-    else
-        hipLaunchKernelGGL((k_ln_bwd<DT, VE, G, C, NT, false>), grid, dim3(NT), 0, hs(st), a);
+    const bool lines = whole_lines(a.h, a.cols, E) && whole_lines(a.dy, a.cols, E) && whole_lines(a.dh, a.cols, E);
+    if constexpr (G > 512) {
+        if (lines) hipLaunchKernelGGL((k_ln_bwd_wide<DT, C, true>), grid, dim3(NT), 0, hs(st), a);
+        else hipLaunchKernelGGL((k_ln_bwd_wide<DT, C, false>), grid, dim3(NT), 0, hs(st), a);
+    } else {
+        if (lines) hipLaunchKernelGGL((k_ln_bwd<DT, VE, G, C, NT, true>), grid, dim3(NT), 0, hs(st), a);
+        else hipLaunchKernelGGL((k_ln_bwd<DT, VE, G, C, NT, false>), grid, dim3(NT), 0, hs(st), a);
+    }
     const int r = launch_status();
     return r ? r : bwd_sums(a, wgs, dw, db, DT, st);
 }
@@ -514,12 +623,14 @@ int bwd_dispatch(LnBwd a, void *dw, void *db, cxm_stream_t st) {
     constexpr int VE = Elem<DT>::kVec;
     if (a.cols < static_cast<unsigned>(VE)) return bwd_launch<DT, 1, 16, 1, 256>(a, dw, db, st);
     const unsigned chunks = (a.cols + VE - 1) / VE;
+    const bool few = a.rows <= static_cast<size_t>(device_cus());  // 64x2048: 7.5 us with a workgroup per row, 9.2 with a wave
     if (chunks <= 16) return bwd_launch<DT, VE, 16, 1, 256>(a, dw, db, st);
     if (chunks <= 64) return bwd_launch<DT, VE, 64, 1, 256>(a, dw, db, st);
     if (chunks <= 128) return bwd_launch<DT, VE, 64, 2, 256>(a, dw, db, st);
-    if (chunks <= 256) return bwd_launch<DT, VE, 64, 4, 256>(a, dw, db, st);
+    if (chunks <= 256) return few ? bwd_launch<DT, VE, 256, 1, 256>(a, dw, db, st) : bwd_launch<DT, VE, 64, 4, 256>(a, dw, db, st);
     if (chunks <= 512) return bwd_launch<DT, VE, 256, 2, 256>(a, dw, db, st);
     if (chunks <= 1024) return bwd_launch<DT, VE, 512, 2, 512>(a, dw, db, st);
+    if (chunks <= 2048 && !few) return bwd_launch<DT, VE, 1024, 2, 1024>(a, dw, db, st);
     if (a.rows > most_wgs(1024)) return CXM_E_TOO_LARGE;
     const size_t tiles = (chunks + kBlock - 1) / kBlock;
     size_t parts = 4 * device_cus() / tiles;

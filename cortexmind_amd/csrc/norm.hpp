@@ -75,8 +75,8 @@ inline bool whole_lines(const void *p, size_t cols, size_t bytes) {
 
 // Workgroups of the backward: enough to fill the chip, few enough that their
 // shares of dw are a small part of the traffic.
-size_t bwd_wgs(size_t rows, int per_wg) {
-    const size_t need = (rows + per_wg - 1) / per_wg, most = device_cus() * 2;
+size_t bwd_wgs(size_t rows, int per_wg, size_t per_cu = 2) {
+    const size_t need = (rows + per_wg - 1) / per_wg, most = device_cus() * per_cu;
     return need < most ? need : most;
 }
 

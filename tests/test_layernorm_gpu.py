@@ -191,7 +191,8 @@ def bwd_data(rows, cols, dt, seed=30):
 
 
 @pytest.mark.parametrize("dt", DTYPES, ids=NAMES.get)
-@pytest.mark.parametrize("shape", SHAPES + [(700, 96), (513, 2048), (600, 8448)], ids=ids)
+@pytest.mark.parametrize("shape", SHAPES + [(700, 96), (513, 2048), (600, 8448), (257, 6001), (300, 16384)],
+                         ids=ids)
 def test_backward(hip, shape, dt):
     h, mean, rstd, w, dy, dh = bwd_data(*shape, dt)
     for d in (None, dh):
@@ -199,7 +200,8 @@ def test_backward(hip, shape, dt):
 
 
 @pytest.mark.parametrize("dt", DTYPES, ids=NAMES.get)
-@pytest.mark.parametrize("shape", [(5, 24), (70, 1003), (300, 2048), (3, 9000), (2, 40000)], ids=ids)
+@pytest.mark.parametrize("shape", [(5, 24), (70, 1003), (300, 2048), (3, 9000), (300, 8201), (2, 40000)],
+                         ids=ids)
 def test_backward_misaligned_and_in_place(hip, shape, dt):
     h, mean, rstd, w, dy, dh = bwd_data(*shape, dt, 50)
     want = backward(h, mean, rstd, w, dy, dh, dt)

@@ -10,8 +10,9 @@
 // backward(const Tensor&), ToString()) and adds flows for every operator on
 // the path -- MatMul, AddBias, Add, MulRow (Broadcast::row::mul), MulScalar
 // (ScalarOp::mul), ReLU / Sigmoid / Tanh, the fused AffineAct, Softmax and
-// LogSoftmax, Sum and Mean over an axis, SoftmaxCrossEntropy, RmsNorm and
-// Linear (a dense layer with bias, activation and residual) -- each
+// LogSoftmax, Sum and Mean over an axis, SoftmaxCrossEntropy, RmsNorm, LayerNorm,
+// Linear (a dense layer with bias, activation and residual), Embedding, LogProb
+// (of given tokens) and Distill -- each
 // running the library's kernels through the C ABI on hip::stream(), plus
 // backward(root[, seed]), sgd() and AdamW.  Tensors are shared handles (TensorPtr)
 // so that a flow can reach its inputs' gradients.
@@ -439,6 +440,81 @@ inline TensorPtr rms_norm(const TensorPtr &x, const TensorPtr &w, float eps = 1e
     return y;
 }
 
+// Y = (X - mean) / deviation * w + bias over the rows of X [rows, cols]
+// (cxm_layernorm_fwd_t), the bias optional: dX, dw and the bias's gradient from X
+// and the saved mean and 1 / deviation (cxm_layernorm_bwd_t).
+struct LayerNormFlow : GradientFlow {
+    TensorPtr x, w, bias;
+    Tensor mean, rstd;
+    LayerNormFlow(TensorPtr x_, TensorPtr w_, TensorPtr b_, Tensor mean_, Tensor rstd_)
+        : GradientFlow("LayerNorm"), x(std::move(x_)), w(std::move(w_)), bias(std::move(b_)), mean(std::move(mean_)),
+          rstd(std::move(rstd_)) {
+        inputs = {x, w};
+        if (bias) inputs.push_back(bias);
+    }
+    void backward(const Tensor &dy) override {
+        Tensor tx, tw, tb;
+        float *dx = grad_dst(x, tx), *dw = grad_dst(w, tw);
+        float *db = bias && needs_grad(bias) ? grad_dst(bias, tb) : nullptr;
+        check(cxm_layernorm_bwd_t(x->data(), mean.data(), rstd.data(), w->data(), dy.data(), nullptr, dx, dw, db,
+                                  rows_of(*x), cols_of(*x), CXM_DT_F32, stream()),
+              "LayerNormFlow");
+        grad_done(x, tx);
+        grad_done(w, tw);
+        if (db) grad_done(bias, tb);
+    }
+};
+inline TensorPtr layer_norm(const TensorPtr &x, const TensorPtr &w, const TensorPtr &bias = nullptr, float eps = 1e-5f) {
+    on_device({x.get(), w.get()}, "layer_norm");
+    if (bias) on_device({bias.get()}, "layer_norm");
+    if (w->len() != cols_of(*x) || (bias && bias->len() != cols_of(*x)))
+        check(CXM_E_INVALID, "layer_norm: one weight and one bias per column");
+    auto y = make_tensor(x->shape());
+    const bool grad = needs_grad(x) || needs_grad(w) || (bias && needs_grad(bias));
+    Tensor mean, rstd;
+    if (grad) {
+        mean = device_tensor({x->dim(0)});
+        rstd = device_tensor({x->dim(0)});
+    }
+    check(cxm_layernorm_fwd_t(x->data(), nullptr, w->data(), bias ? bias->data() : nullptr, eps, nullptr, y->data(), nullptr,
+                              nullptr, grad ? mean.data() : nullptr, grad ? rstd.data() : nullptr, rows_of(*x), cols_of(*x),
+                              CXM_DT_F32, stream()),
+          "layer_norm");
+    if (grad) link(y, std::make_shared<LayerNormFlow>(x, w, bias, std::move(mean), std::move(rstd)));
+    return y;
+}
+
+// Y[t] = table[ids[t]] * scale (cxm_embedding_fwd_t): the table's gradient by
+// tokens (cxm_embedding_bwd_t), added where it is to the one that the table has
+// already.  ids: device int32 [tokens], read again by the backward pass.
+struct EmbeddingFlow : GradientFlow {
+    TensorPtr table;
+    const std::int32_t *ids;
+    float scale;
+    EmbeddingFlow(TensorPtr t, const std::int32_t *ids_, float scale_)
+        : GradientFlow("Embedding"), table(std::move(t)), ids(ids_), scale(scale_) {
+        inputs = {table};
+    }
+    void backward(const Tensor &dy) override {
+        if (!needs_grad(table)) return;
+        const bool add = table->has_grad();
+        if (!add) new_grad(table);
+        check(cxm_embedding_bwd_t(ids, dy.data(), scale, table->grad().data(), add, rows_of(dy), rows_of(*table),
+                                  cols_of(*table), CXM_DT_F32, CXM_DT_F32, stream()),
+              "EmbeddingFlow");
+    }
+};
+inline TensorPtr embedding(const TensorPtr &table, const std::int32_t *ids, std::int64_t tokens, float scale = 1.0f) {
+    on_device({table.get()}, "embedding");
+    if (tokens < 0) check(CXM_E_INVALID, "embedding: fewer than no tokens");
+    auto y = make_tensor({tokens, table->dim(1)});
+    check(cxm_embedding_fwd_t(table->data(), ids, scale, y->data(), rows_of(*y), rows_of(*table), cols_of(*table), CXM_DT_F32,
+                              stream()),
+          "embedding");
+    if (needs_grad(table)) link(y, std::make_shared<EmbeddingFlow>(table, ids, scale));
+    return y;
+}
+
 // Y = act(X W + bias) + residual (cxm_linear_fwd_t), bias and residual
 // optional: the gradients of X, W and the bias from the saved X W + bias
 // (cxm_linear_bwd_t); the residual's is dY.  X W + bias is saved only where one
@@ -507,6 +583,81 @@ inline TensorPtr softmax_cross_entropy(const TensorPtr &logits, const std::int32
                                stream()),
           "softmax_cross_entropy");
     if (needs_grad(logits)) link(loss, std::make_shared<SoftmaxCrossEntropyFlow>(logits, std::move(dl)));
+    return loss;
+}
+
+// Log probabilities [rows] of tokens under softmax(scale * logits)
+// (cxm_logprob_fwd_t): the logits' gradient from them and the saved lse
+// (cxm_logprob_bwd_t).
+struct LogProbFlow : GradientFlow {
+    TensorPtr logits;
+    const std::int32_t *tokens;
+    Tensor lse;
+    float scale;
+    LogProbFlow(TensorPtr l, const std::int32_t *t, Tensor lse_, float scale_)
+        : GradientFlow("LogProb"), logits(std::move(l)), tokens(t), lse(std::move(lse_)), scale(scale_) {
+        inputs = {logits};
+    }
+    void backward(const Tensor &g) override {
+        if (!needs_grad(logits)) return;
+        const std::size_t vocab = cols_of(*logits);
+        accumulate(logits, [&](float *dl) {
+            check(cxm_logprob_bwd_t(logits->data(), vocab, tokens, scale, lse.data(), nullptr, g.data(), nullptr, dl, vocab,
+                                    rows_of(*logits), vocab, CXM_DT_F32, stream()),
+                  "LogProbFlow");
+        });
+    }
+};
+// tokens: device int32 [rows] (negative: padding, 0), read again by the backward pass.
+inline TensorPtr log_prob(const TensorPtr &logits, const std::int32_t *tokens, float scale = 1.0f) {
+    on_device({logits.get()}, "log_prob");
+    auto logp = make_tensor({logits->dim(0)});
+    Tensor lse;
+    if (needs_grad(logits)) lse = device_tensor({logits->dim(0)});
+    check(cxm_logprob_fwd_t(logits->data(), cols_of(*logits), tokens, scale, logp->data(), nullptr,
+                            lse.empty() ? nullptr : lse.data(), nullptr, nullptr, 0, rows_of(*logits), cols_of(*logits),
+                            CXM_DT_F32, stream()),
+          "log_prob");
+    if (needs_grad(logits)) link(logp, std::make_shared<LogProbFlow>(logits, tokens, std::move(lse), scale));
+    return logp;
+}
+
+// Divergence [rows] of softmax(scale * logits) from a teacher's distribution over
+// its k top tokens (cxm_distill_fwd_t); the logits' gradient (cxm_distill_bwd_t).
+struct DistillFlow : GradientFlow {
+    TensorPtr logits;
+    const std::int32_t *ids;
+    const float *teacher;
+    std::size_t k;
+    Tensor lse;
+    float scale;
+    DistillFlow(TensorPtr l, const std::int32_t *ids_, const float *teacher_, std::size_t k_, Tensor lse_, float scale_)
+        : GradientFlow("Distill"), logits(std::move(l)), ids(ids_), teacher(teacher_), k(k_), lse(std::move(lse_)),
+          scale(scale_) {
+        inputs = {logits};
+    }
+    void backward(const Tensor &g) override {
+        if (!needs_grad(logits)) return;
+        const std::size_t vocab = cols_of(*logits);
+        accumulate(logits, [&](float *dl) {
+            check(cxm_distill_bwd_t(logits->data(), vocab, ids, teacher, k, scale, lse.data(), g.data(), dl, vocab,
+                                    rows_of(*logits), vocab, CXM_DT_F32, stream()),
+                  "DistillFlow");
+        });
+    }
+};
+// ids: device int32 [rows, k] (negative: no entry), teacher: device fp32 [rows,
+// k], its logits; both are read again by the backward pass.
+inline TensorPtr distill(const TensorPtr &logits, const std::int32_t *ids, const float *teacher, std::size_t k,
+                         float scale = 1.0f) {
+    on_device({logits.get()}, "distill");
+    auto loss = make_tensor({logits->dim(0)});
+    Tensor lse;
+    if (needs_grad(logits)) lse = device_tensor({logits->dim(0)});
+    check(cxm_distill_fwd_t(logits->data(), cols_of(*logits), ids, teacher, k, scale, loss->data(),
+                            lse.empty() ? nullptr : lse.data(), rows_of(*logits), cols_of(*logits), CXM_DT_F32, stream()),
+          "distill");
+    if (needs_grad(logits)) link(loss, std::make_shared<DistillFlow>(logits, ids, teacher, k, std::move(lse), scale));
     return loss;
 }
 

@@ -95,11 +95,14 @@ __device__ __forceinline__ void drop_others(Chunk<DT, VE> &c, Own o) {
             if (!o.has(e)) c.r[e / 2] = e & 1 ? (c.r[e / 2] & 0xffffu) | inf << 16 : (c.r[e / 2] & 0xffff0000u) | inf;
     }
 }
-// Stores a chunk's own elements.
+// Stores a chunk's own elements; with the non-temporal hint, since a gradient that
+// is no longer than the cache is rare (into memory that is not in the cache, bf16
+// 2048x65500 96.1 -> 90.7 us, fp32 1000x30011 47.6 -> 45.2; into the same buffer over
+// and over, 86.0 -> 91.1 and 42.9 -> 45.5).
 template <int DT, int VE>
 __device__ __forceinline__ void store_own(typename Elem<DT>::S *row, Own o, const Chunk<DT, VE> &c) {
     if (o.lo <= 0 && o.hi == VE) {
-        c.store(row + o.off);
+        c.store_nt(row + o.off);
     } else {
 #pragma unroll
         for (int e = 0; e < VE; ++e)

@@ -40,7 +40,8 @@ Spread spread_of(unsigned n) {
 
 // G lanes per row piece of G chunks, U tokens per group of lanes.  Stores carry the
 // non-temporal hint (20001 rows of 1003 floats 30.7 -> 22.7 us, 32768 of 2048 bf16
-// 42.4 -> 31.5; the gradient's rows without it: 32768x2048 bf16 80 us, with it 92).
+// 42.4 -> 31.5).  The gradient's rows are stored without it: 32768x2048 bf16 took 92
+// with it where 94 without into memory that is not in the cache, but 92 for 80 where it is.
 template <int DT, int VE, int G, int U>
 __global__ __launch_bounds__(kBlock) void k_embed(const typename Elem<DT>::S *table, const int32_t *ids, float scale,
                                                   typename Elem<DT>::S *y, size_t tokens, size_t vocab, unsigned cols,

@@ -559,7 +559,9 @@ int cxm_linear_q8_fwd(const uint8_t *x, const float *x_scale, const uint8_t *w, 
  * NaN.  A row of the type's lowest value alone is a row of equal logits.
  * Outputs overlap nothing.  rows < 2^24, rows * segments (16384 16-bit or 8192
  * fp32 elements each, fewer in few rows) too, else CXM_E_TOO_LARGE.  Rows cut
- * into segments need scratch (see CXM_E_CAPTURE). */
+ * into segments need scratch (see CXM_E_CAPTURE).  The number of rows has its part
+ * in how a row is cut: the same call gives the same bits, a row among more or
+ * fewer others may differ in the last ones. */
 int cxm_logprob_fwd_t(const void *logits, size_t ld, const int32_t *tokens, float scale, float *logp, float *entropy,
                       float *lse, float *top_logp, int32_t *top_ids, size_t top, size_t rows, size_t vocab, int dtype,
                       cxm_stream_t s);

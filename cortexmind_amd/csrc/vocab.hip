@@ -26,7 +26,7 @@ constexpr float kLog2e = 0x1.715476p+0f, kLn2 = 0x1.62e430p-1f, kLow = -1000.0f;
 constexpr unsigned kTopMost = 64;       // tokens that a call returns
 constexpr unsigned kTeacherMost = 256;  // entries of a teacher's row
 constexpr size_t kTicket = 16;          // words between two rows' tickets
-constexpr int kStatChunks = 8, kGradChunks = 4;
+constexpr int kStatChunks = 8, kStatFew = 7, kGradChunks = 4;  // (kStatFew: held to 64 registers, 8 waves of a SIMD)
 
 __device__ __forceinline__ float fmax3(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
@@ -532,10 +532,10 @@ __device__ __forceinline__ void join_top(const StatArgs &a, size_t row, const Ro
 // A row per G lanes (nseg 1, G = 64) or a segment per workgroup; C chunks a lane.
 // One read of the logits and the exponentials' issue bound it: 2048 rows of 131072
 // bf16 distilled from 64 tokens 93.6 us (5.7 TB/s; over half of the cycles are vector
-// work), 2500 of 50001 fp16 with entropy and 5 tokens 73.3 (3.4 TB/s), 16 of 131072 bf16
+// work), 2500 of 50001 fp16 with entropy and 5 tokens 65.8 (3.8 TB/s), 16 of 131072 bf16
 // with 20 tokens 14.8, which is latency.
 template <int DT, int VE, int G, int C, bool ENT, bool TOP>
-__global__ __launch_bounds__(kBlock) void k_vocab_stats(StatArgs a) {
+__global__ __launch_bounds__(kBlock, C == kStatFew ? 8 : 1) void k_vocab_stats(StatArgs a) {
     using S = typename Elem<DT>::S;
     constexpr int NG = kBlock / G;
     __shared__ float lds_f[kBlock / kWave];
@@ -905,9 +905,8 @@ bool wave_rows(const Logits &in, unsigned chunk, unsigned chunks) {
     return in.vocab + in.odd <= 64 * chunk * chunks && (in.vocab <= 64 * chunk || in.rows >= 4 * device_cus());
 }
 
-template <int DT, int VE, int G, bool ENT, bool TOP>
+template <int DT, int VE, int G, bool ENT, bool TOP, int C = VE == 1 ? 1 : kStatChunks>
 int stats_launch(const StatArgs &a, hipStream_t s) {
-    constexpr int C = VE == 1 ? 1 : kStatChunks;
     const size_t wgs = G == kBlock ? a.in.rows * a.in.nseg : (a.in.rows + kBlock / G - 1) / (kBlock / G);
     hipLaunchKernelGGL((k_vocab_stats<DT, VE, G, C, ENT, TOP>), dim3(static_cast<unsigned>(wgs)), dim3(kBlock), 0, s, a);
     return launch_status();
@@ -941,6 +940,12 @@ int stats(StatArgs a, cxm_stream_t st) {
         a.parts = static_cast<Part *>(ws.scratch);
         a.bars = reinterpret_cast<float *>(static_cast<char *>(ws.scratch) + o_bars);
         a.cands = reinterpret_cast<ArgPair *>(static_cast<char *>(ws.scratch) + o_cands);
+    }
+    // 16-bit segments of 8 chunks a lane take 71 registers, 7 waves of a SIMD; of 7 chunks, where that holds them, 64
+    // and 8 waves: 2500 rows of 50001 fp16 and 5 tokens 66.0 us instead of 73.2 (68.3 at 66 registers and 7 waves; held
+    // to 64 registers, 8 chunks spill: 71.8 there, but 512 rows of 131072 bf16 and 20 tokens 46.3 instead of 43.8)
+    if constexpr (VE == 8 && ENT && TOP) {
+        if (a.in.seglen <= kBlock * VE * kStatFew) return stats_launch<DT, VE, kBlock, ENT, TOP, kStatFew>(a, hs(st));
     }
     return stats_launch<DT, VE, kBlock, ENT, TOP>(a, hs(st));
 }

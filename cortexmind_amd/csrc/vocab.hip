@@ -559,9 +559,10 @@ __global__ __launch_bounds__(kBlock, C == kStatFew ? 8 : 1) void k_vocab_stats(S
     for (int i = 0; i < C; ++i)
         if (i < seg.its) c[i].load_nt(x + seg.own<VE, G>(i, lane).off);
     // Without the top tokens one pass, with the largest of the wave's first chunks as m, which the others need
-    // not be below: S then says whether they are by too much (or are NaN, or infinite), and the sums are taken
-    // again from the largest of all.  With them the largest values come first, and a wave finds the bar
-    // while the others go on.  z's product with c is not rounded on its own; what m c lost is made up for.
+    // not be below: S then says whether they are by too much, and the sums are taken again from the largest of
+    // all.  With them the largest values come first, and a wave finds the bar while the others go on.  z's product
+    // with c is not rounded on its own; what m c lost is made up for where it is small (half a last place of m c:
+    // with far logits that is more octaves than an exponential holds), else the sums are taken again too.
     [[maybe_unused]] const unsigned held = seg.end - seg.begin(), n0 = held < a.top ? held : a.top;
     [[maybe_unused]] float low = -INFINITY;  // the bar: at least `top` tokens are not below it, so none below it is wanted
     float cm[C], from = -INFINITY;           // each chunk's largest, all of them's
@@ -651,8 +652,11 @@ __global__ __launch_bounds__(kBlock, C == kStatFew ? 8 : 1) void k_vocab_stats(S
             }
         }
         p = Part{from, wave_reduce<SumOp>(sum[0] + sum[1]), ENT ? wave_reduce<SumOp>(ent[0] + ent[1]) : 0.0f};
-        if (fabsf(mc) < 1e37f && p.s < 0x1p20f) {
-            const float lost = -fmaf(from, a.in.c, -mc), f = __builtin_amdgcn_exp2f(lost);
+        // 64: S keeps what lies up to 60 octaves below m, and the rounding of u, 2^-19, is 22 of S's own.  T, a sum of
+        // terms as large as lost, would lose as many times its own roundings: 1.  (NaN, and an infinite m: not below.)
+        const float lost = -fmaf(from, a.in.c, -mc);
+        if (fabsf(lost) < (ENT ? 1.0f : 64.0f) && p.s < 0x1p20f) {
+            const float f = __builtin_amdgcn_exp2f(lost);
             p = Part{from, p.s * f, fmaf(lost, p.s, p.t) * f};
         } else {
             p = again_from_the_largest<DT, VE, C, ENT>(c, seg.its, a.in.c);

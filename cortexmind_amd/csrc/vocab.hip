@@ -762,6 +762,57 @@ struct GradArgs {
     unsigned k;
 };
 
+// What a row's log probabilities are counted from: log p = scale (x - from) - less.
+struct Base {
+    float from, less;
+};
+// lse is fp32: its rounding moves every p = exp(scale x - lse) of the row by up to 2^-24 |lse| of itself, past 2^24 by
+// factors (a row of a mask's value alone, or of the type's lowest, would have p = 1 everywhere, not 1 / vocab).
+// From 2^12 on, where that is more than the roundings of fp16, a row is counted from its own largest value, as in
+// the forward pass, by one workgroup alone: in place the others' parts are gone once they have stored.  Such rows are
+// read three times.
+constexpr float kFarLse = 4096.0f;
+
+// The base of a row by G lanes: its largest value and the log of its sum, if lse is theirs, else lse (which is
+// then of more logits than these).  The same row's, summed otherwise, differ by less than 4 of lse's last places.
+template <int DT, int VE, int G, int U>
+__device__ __forceinline__ Base far_base(const Logits &in, const typename Elem<DT>::S *x, float lse, unsigned lane, float *lds) {
+    auto each = [&](auto &&take) {
+#pragma nounroll
+        for (unsigned n = 0; n < in.nseg; ++n) {
+            const Seg seg = seg_of<DT, VE, G>(in, x, n, lane);
+#pragma nounroll
+            for (int from = 0; from < seg.its; from += U) {
+                Chunk<DT, VE> c[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (from + u < seg.its) c[u].load(x + seg.own<VE, G>(from + u, lane).off);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (from + u >= seg.its) break;
+                    drop_others<DT, VE>(c[u], seg.own<VE, G>(from + u, again(lane)));
+                    take(c[u]);
+                }
+            }
+        }
+    };
+    float m = -INFINITY, s = 0.0f;
+    each([&](const Chunk<DT, VE> &c) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) m = fmax3(m, c.get(e));
+    });
+    m = group_all<InfMaxOp, G>(m, lds);
+    each([&](const Chunk<DT, VE> &c) {
+        float t = 0.0f;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) t += __builtin_amdgcn_exp2f((c.get(e) - m) * in.c);
+        s += t;
+    });
+    const float log_s = logf(group_all<SumOp, G>(s, lds)), own = fmaf(in.scale, m, log_s);
+    const bool same = own == lse || (__builtin_isfinite(lse) && fabsf(own - lse) <= fabsf(lse) * 0x1p-22f);
+    return same ? Base{m, log_s} : Base{0.0f, lse};
+}
+
 // A row per G lanes or a segment per workgroup, as above.  Each wave finds out by
 // itself whether the row has a gradient; the teacher's probabilities and the
 // gradients of its tokens in the segment are the first wave's, which stores them
@@ -774,12 +825,15 @@ __global__ __launch_bounds__(kBlock) void k_vocab_grad(GradArgs a) {
     constexpr int NG = kBlock / G, E = Teacher::E;
     __shared__ float qs[DISTILL ? NG : 1][DISTILL ? kTeacherMost : 1];
     __shared__ alignas(16) int qi[DISTILL ? NG : 1][DISTILL ? kTeacherMost : 1];
+    [[maybe_unused]] __shared__ float ql[DISTILL ? NG : 1][DISTILL ? kTeacherMost : 1];  // (of a far row)
+    __shared__ float lds[kBlock / kWave];
     const unsigned lane = threadIdx.x % G, grp = threadIdx.x / G;
     const size_t row = G == kBlock ? blockIdx.x / a.in.nseg : static_cast<size_t>(blockIdx.x) * NG + grp;
     if (row >= a.in.rows) return;  // a whole wave of a workgroup whose waves have rows of their own
     const S *x = static_cast<const S *>(a.in.x) + row * a.in.ld;
     S *dx = static_cast<S *>(a.dx) + row * a.ldd;
-    const Seg seg = seg_of<DT, VE, G>(a.in, x, G == kBlock ? blockIdx.x % a.in.nseg : 0, lane);
+    const unsigned number = G == kBlock ? blockIdx.x % a.in.nseg : 0;
+    const Seg seg = seg_of<DT, VE, G>(a.in, x, number, lane);
     Chunk<DT, VE> c[C];
     Own own[C];
 #pragma unroll
@@ -791,53 +845,15 @@ __global__ __launch_bounds__(kBlock) void k_vocab_grad(GradArgs a) {
     // d x = p (slope + bend (log p)) + what the tokens get
     float slope, bend = 0.0f, given = 0.0f;
     unsigned token = ~0u;
-    [[maybe_unused]] float late[E];  // the gradient at the teacher's tokens of this segment
+    [[maybe_unused]] float late[E], tm = -INFINITY;  // the gradient at the teacher's tokens of this segment
     [[maybe_unused]] Teacher t;
     if constexpr (DISTILL) {
         t.load(a.ids + row * a.k, a.teacher + row * a.k, a.k, lane % kWave);
-        float tm = -INFINITY;
 #pragma unroll
         for (int j = 0; j < E; ++j)
             if (t.id[j] >= 0) tm = fmax3(tm, static_cast<unsigned>(t.id[j]) < a.in.vocab ? t.v[j] : __builtin_nanf(""));
         tm = wave_reduce<InfMaxOp>(tm);
         slope = tm == -INFINITY ? 0.0f : __builtin_isnan(tm) ? tm : a.dloss[row] * a.in.scale;
-        if (lane < kWave) {
-            float at[E], q[E], z = 0.0f;
-            bool mine[E];
-#pragma unroll
-            for (int j = 0; j < E; ++j) {  // what the dense gradient may be stored over
-                mine[j] = t.id[j] >= static_cast<int>(seg.begin()) && t.id[j] < static_cast<int>(seg.end);
-                at[j] = mine[j] ? Elem<DT>::load(x[t.id[j]]) : 0.0f;
-                q[j] = t.id[j] < 0 ? 0.0f : expf((t.v[j] - (tm == -INFINITY ? 0.0f : tm)) * a.in.scale);
-                z += q[j];
-            }
-            z = wave_reduce<SumOp>(z);
-#pragma unroll
-            for (int j = 0; j < E; ++j) {
-                q[j] /= z;
-                qs[grp][j * kWave + lane] = q[j];
-                qi[grp][j * kWave + lane] = mine[j] ? t.id[j] : -1;
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-            for (int j = 0; j < E; ++j) {
-                if (!__any(mine[j])) continue;
-                // a token may be there more than once
-                int times = 0;
-                for (unsigned i = 0; i < (a.k + 3) / 4; ++i) {
-                    const int4 v = reinterpret_cast<const int4 *>(qi[grp])[i];
-                    times += (v.x == t.id[j]) + (v.y == t.id[j]) + (v.z == t.id[j]) + (v.w == t.id[j]);
-                }
-                float all = q[j];
-                if (__any(mine[j] && times > 1)) {
-                    all = 0.0f;
-                    for (unsigned i = 0; i < a.k; ++i) all += qi[grp][i] == t.id[j] ? qs[grp][i] : 0.0f;
-                }
-                const float p = __builtin_amdgcn_exp2f(fmaf(a.in.scale, at[j], -lse) * kLog2e);
-                late[j] = slope == 0.0f ? 0.0f : slope * (p - all);
-                if (!mine[j]) t.id[j] = -1;
-            }
-        }
     } else {
         const int tok = a.tokens ? a.tokens[row] : -1;
         const float g = tok < 0 || !a.dlogp ? 0.0f : static_cast<unsigned>(tok) < a.in.vocab ? a.dlogp[row] : __builtin_nanf("");
@@ -852,17 +868,12 @@ __global__ __launch_bounds__(kBlock) void k_vocab_grad(GradArgs a) {
         }
     }
     const bool none = slope == 0.0f && bend == 0.0f && given == 0.0f;  // zeros, whatever the logits are
-    if (DISTILL && a.dx == a.in.x) {  // not before the teacher's tokens have been read
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        group_sync<G>();
-    }
-#pragma unroll
-    for (int i = 0; i < C; ++i) {
-        if (i >= seg.its) break;
+    // a chunk's gradient, in its place
+    auto grad_of = [&](Chunk<DT, VE> &c, const Own &own, auto &&log_p) {
         float l[VE], p[VE], v[VE];
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
-            l[e] = fmaf(a.in.scale, c[i].get(e), -lse);
+            l[e] = log_p(c.get(e));
             if constexpr (ENT) l[e] = fmax3(l[e], kLow);
         }
 #pragma unroll
@@ -871,22 +882,139 @@ __global__ __launch_bounds__(kBlock) void k_vocab_grad(GradArgs a) {
         for (int e = 0; e < VE; ++e) {
             if constexpr (ENT) v[e] = p[e] * fmaf(bend, l[e], slope);
             else v[e] = p[e] * slope;
-            if constexpr (!DISTILL) v[e] += own[i].off + e == token ? given : 0.0f;
+            if constexpr (!DISTILL) v[e] += own.off + e == token ? given : 0.0f;
             v[e] = none ? 0.0f : v[e];
         }
-        c[i].set(v);
-        store_own<DT, VE>(dx, own[i], c[i]);
-    }
-    if constexpr (DISTILL) {
-        // over what was stored above, by whichever lane
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        group_sync<G>();
-        if (lane < kWave) {
+        c.set(v);
+        store_own<DT, VE>(dx, own, c);
+    };
+    auto usual = [&]() __attribute__((always_inline)) {
+        if constexpr (DISTILL) {
+            if (lane < kWave) {
+                float at[E], q[E], z = 0.0f;
+                bool mine[E];
 #pragma unroll
-            for (int j = 0; j < E; ++j)
-                if (t.id[j] >= static_cast<int>(seg.begin()) && t.id[j] < static_cast<int>(seg.end))
-                    dx[t.id[j]] = Elem<DT>::store(__builtin_isnan(slope) ? slope : late[j]);
+                for (int j = 0; j < E; ++j) {  // what the dense gradient may be stored over
+                    mine[j] = t.id[j] >= static_cast<int>(seg.begin()) && t.id[j] < static_cast<int>(seg.end);
+                    at[j] = mine[j] ? Elem<DT>::load(x[t.id[j]]) : 0.0f;
+                    q[j] = t.id[j] < 0 ? 0.0f : expf((t.v[j] - (tm == -INFINITY ? 0.0f : tm)) * a.in.scale);
+                    z += q[j];
+                }
+                z = wave_reduce<SumOp>(z);
+#pragma unroll
+                for (int j = 0; j < E; ++j) {
+                    q[j] /= z;
+                    qs[grp][j * kWave + lane] = q[j];
+                    qi[grp][j * kWave + lane] = mine[j] ? t.id[j] : -1;
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+                for (int j = 0; j < E; ++j) {
+                    if (!__any(mine[j])) continue;
+                    // a token may be there more than once
+                    int times = 0;
+                    for (unsigned i = 0; i < (a.k + 3) / 4; ++i) {
+                        const int4 v = reinterpret_cast<const int4 *>(qi[grp])[i];
+                        times += (v.x == t.id[j]) + (v.y == t.id[j]) + (v.z == t.id[j]) + (v.w == t.id[j]);
+                    }
+                    float all = q[j];
+                    if (__any(mine[j] && times > 1)) {
+                        all = 0.0f;
+                        for (unsigned i = 0; i < a.k; ++i) all += qi[grp][i] == t.id[j] ? qs[grp][i] : 0.0f;
+                    }
+                    const float p = __builtin_amdgcn_exp2f(fmaf(a.in.scale, at[j], -lse) * kLog2e);
+                    late[j] = slope == 0.0f ? 0.0f : slope * (p - all);
+                    if (!mine[j]) t.id[j] = -1;
+                }
+            }
         }
+        if (DISTILL && a.dx == a.in.x) {  // not before the teacher's tokens have been read
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            group_sync<G>();
+        }
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            if (i >= seg.its) break;
+            // (with a teacher the chunks' places are found anew: 64 registers, 70 where they are kept)
+            grad_of(c[i], DISTILL ? seg.own<VE, G>(i, again(lane)) : own[i], [&](float v) { return fmaf(a.in.scale, v, -lse); });
+        }
+        if constexpr (DISTILL) {
+            // over what was stored above, by whichever lane
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            group_sync<G>();
+            if (lane < kWave) {
+#pragma unroll
+                for (int j = 0; j < E; ++j)
+                    if (t.id[j] >= static_cast<int>(seg.begin()) && t.id[j] < static_cast<int>(seg.end))
+                        dx[t.id[j]] = Elem<DT>::store(__builtin_isnan(slope) ? slope : late[j]);
+            }
+        }
+    };
+    auto far_row = [&]() __attribute__((always_inline)) {
+        // one of the row's workgroups, and the chip's XCDs, which take workgroups in turn, in turn (always the first: 864 us
+        // for 2048 rows of 65500 bf16 in 8 segments, all of them on one XCD)
+        if (number != row * (a.in.nseg < 8 ? a.in.nseg : 8) / 8 % a.in.nseg) return;
+        const unsigned l = again(lane);
+        const Base base = far_base<DT, VE, G, DISTILL || C == 1 ? 1 : C>(a.in, x, lse, l, lds);
+        auto log_p = [&](float v) { return fmaf(a.in.scale, v - base.from, -base.less); };
+        auto entry = [&](unsigned i) {  // the id of the teacher's entry i, negative where there is none
+            const int id = a.ids[row * a.k + i];
+            return static_cast<unsigned>(id) < a.in.vocab ? id : -1;
+        };
+        if constexpr (DISTILL) {
+            if (l < kWave) {
+                float z = 0.0f;
+#pragma nounroll
+                for (unsigned i = l; i < a.k; i += kWave) {
+                    const int id = entry(i);
+                    const float q = id < 0 ? 0.0f : expf((a.teacher[row * a.k + i] - tm) * a.in.scale);
+                    qi[grp][i] = id;
+                    qs[grp][i] = q;
+                    z += q;
+                }
+                z = wave_reduce<SumOp>(z);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma nounroll
+                for (unsigned i = l; i < a.k; i += kWave) {
+                    const int id = qi[grp][i];
+                    if (id < 0) continue;
+                    float all = 0.0f;
+#pragma nounroll
+                    for (unsigned j = 0; j < a.k; ++j) all += qi[grp][j] == id ? qs[grp][j] : 0.0f;
+                    const float p = __builtin_amdgcn_exp2f(log_p(Elem<DT>::load(x[id])) * kLog2e);
+                    ql[grp][i] = slope * (p - all / z);
+                }
+            }
+            group_sync<G>();  // the teacher's tokens have been read
+        }
+#pragma nounroll
+        for (unsigned n = 0; n < a.in.nseg; ++n) {
+            const Seg each = seg_of<DT, VE, G>(a.in, x, n, l);
+#pragma nounroll
+            for (int i = 0; i < each.its; ++i) {
+                const Own at = each.own<VE, G>(i, l);
+                Chunk<DT, VE> v;
+                v.load(x + at.off);
+                grad_of(v, at, log_p);
+            }
+        }
+        if constexpr (DISTILL) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            group_sync<G>();
+            if (l < kWave)
+#pragma nounroll
+                for (unsigned i = l; i < a.k; i += kWave)
+                    if (qi[grp][i] >= 0) dx[qi[grp][i]] = Elem<DT>::store(ql[grp][i]);
+        }
+    };
+    // The same for all of a wave.  Said so, and asked in the way that keeps each path's registers out of the other (64 at
+    // most, 8 waves of a SIMD; the other way round up to 72).
+    if constexpr (DISTILL) {
+        if (__builtin_amdgcn_readfirstlane(none || !(fabsf(lse) >= kFarLse))) return usual();
+        far_row();
+    } else {
+        if (__builtin_amdgcn_readfirstlane(!none && fabsf(lse) >= kFarLse)) return far_row();
+        usual();
     }
 }
 

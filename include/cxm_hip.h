@@ -570,6 +570,10 @@ int cxm_logprob_fwd_t(const void *logits, size_t ld, const int32_t *tokens, floa
  * exp(scale * logits - lse):
  *   dlogits[j] = scale * (dlogp ([j == token] - p[j])
  *                         - dentropy p[j] (log p[j] + entropy)).
+ * An lse of 4096 or more in magnitude that is the row's own is not rounded to fp32
+ * in p, which is taken from the row's largest logit then, as in the forward: a row
+ * of the type's lowest value alone has p = 1 / vocab (lse may be infinite there).
+ * Any other lse, of a vocabulary of which these logits are a part, is taken as it is.
  * entropy, the forward's, is read with dentropy only.  A negative token takes no
  * part, one of vocab or more makes the row NaN.  Where dlogp (or the token's
  * part in it) and dentropy are 0 the row is zeros whatever the logits and lse
@@ -592,8 +596,8 @@ int cxm_logprob_bwd_t(const void *logits, size_t ld, const int32_t *tokens, floa
 int cxm_distill_fwd_t(const void *logits, size_t ld, const int32_t *ids, const float *teacher, size_t k, float scale,
                       float *loss, float *lse, size_t rows, size_t vocab, int dtype, cxm_stream_t s);
 /* The logits' gradient: dlogits[j] = dloss[r] * scale * (p[j] - sum of q over
- * the entries with id j); zeros where dloss is 0 or the row has no entry of q > 0,
- * NaN where an id is vocab or more.  dlogits may be logits itself (ldd == ld). */
+ * the entries with id j), p as in cxm_logprob_bwd_t; zeros where dloss is 0 or the row
+ * has no entry of q > 0, NaN where an id is vocab or more.  dlogits may be logits itself (ldd == ld). */
 int cxm_distill_bwd_t(const void *logits, size_t ld, const int32_t *ids, const float *teacher, size_t k, float scale,
                       const float *lse, const float *dloss, void *dlogits, size_t ldd, size_t rows, size_t vocab,
                       int dtype, cxm_stream_t s);

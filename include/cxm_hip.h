@@ -493,9 +493,10 @@ int cxm_layernorm_bwd_t(const void *h, const float *mean, const float *rstd, con
  * Rows of a table [vocab, cols] looked up by token and scaled, beside
  * cxm_gather_f32: y[t] = table[ids[t]] * scale, rounded once.  A negative id is
  * padding, a row of zeros; an id of vocab or more gives a row of NaN.  y must
- * not overlap the table or the ids; tokens, vocab and cols < 2^31; a scale that
- * is not finite, vocab == 0 or cols == 0 is CXM_E_INVALID; tokens == 0 does
- * nothing.  No reference counterpart (wise::gather and ScalarOp::mul). */
+ * not overlap the table or the ids; a scale that is not finite, vocab == 0 or
+ * cols == 0 is CXM_E_INVALID; tokens == 0 does nothing.  tokens, vocab and cols of
+ * 2^31 and more are CXM_E_TOO_LARGE, and so is what a grid does not hold: tokens
+ * times a row's pieces (64 chunks of 16 bytes each) from some 2^28 on.  No reference counterpart (wise::gather and ScalarOp::mul). */
 int cxm_embedding_fwd_t(const void *table, const int32_t *ids, float scale, void *y, size_t tokens, size_t vocab,
                         size_t cols, int dtype, cxm_stream_t s);
 /* The table's gradient: dw[v] = scale * sum over t with ids[t] == v of dy[t], in
@@ -503,8 +504,9 @@ int cxm_embedding_fwd_t(const void *table, const int32_t *ids, float scale, void
  * `accumulate` (1) dw[v] is added to that before the rounding, and rows that no
  * token has stay as they are (a table that is also a layer's weight).  Ids
  * outside [0, vocab) take no part.  dy is of `dtype`, dw of `g_dtype`: `dtype`
- * or CXM_DT_F32.  Needs scratch (see CXM_E_CAPTURE): 8 bytes a token, 4 an id,
- * and sums of a share of the tokens. */
+ * or CXM_DT_F32.  Sizes as above, but that a grid holds tokens times pieces to some
+ * 2^30, and vocab to 2^29.  Needs scratch (see CXM_E_CAPTURE): 8 bytes a token, 4
+ * an id, and sums of a share of the tokens. */
 int cxm_embedding_bwd_t(const int32_t *ids, const void *dy, float scale, void *dw, int accumulate, size_t tokens,
                         size_t vocab, size_t cols, int dtype, int g_dtype, cxm_stream_t s);
 

@@ -14,8 +14,9 @@
 //    of columns, and writes the rows of ids that lie within its part; what an
 //    id's tokens give in several waves meets in LDS, in several workgroups in
 //    scratch, added up by the last of them to arrive, in the list's order.
-// 32768 tokens of 2048 bf16 into 65536 rows: 49 us with 216 MB of zeros, and 46 us of
-// sums, whose rows are read at random (3.9 TB/s with what they write).
+// 32768 tokens of 2048 bf16 into 65536 rows: 48 us with 216 MB of zeros, and 46 us of
+// sums, whose rows are read at random (3.9 TB/s with what they write); accumulating,
+// without the zeros, 71 us in all.
 #include "chunk.hpp"
 
 namespace cxm {

@@ -13,8 +13,10 @@
 // squared distances from it (which the one-pass sum of squares would lose to
 // cancellation where the mean is large) and its output.  A row belongs to 16
 // or 64 lanes of a wave or to a whole workgroup; sums are fp32.  fp16 20001x1003
-// 14.1 us (5.7 TB/s), backward with dh bf16 8192x2048 26.5 us (5.1 TB/s) and 4 for the
-// sums of dw and db.
+// 14.3 us (5.6 TB/s).  Backward with dh bf16 8192x2048 27 us (5 TB/s) and 4 for the sums
+// of dw and db; vector work is a third of its cycles, so neither bounds it: its
+// workgroups are one wave per SIMD, in which a row's reduction and stores follow each
+// other with only the next row's loads beside them.
 #include "norm.hpp"
 
 namespace cxm {

@@ -532,8 +532,12 @@ __device__ __forceinline__ void join_top(const StatArgs &a, size_t row, const Ro
 // A row per G lanes (nseg 1, G = 64) or a segment per workgroup; C chunks a lane.
 // One read of the logits and the exponentials' issue bound it: 2048 rows of 131072
 // bf16 distilled from 64 tokens 93.6 us (5.7 TB/s; over half of the cycles are vector
-// work), 2500 of 50001 fp16 with entropy and 5 tokens 65.8 (3.8 TB/s), 16 of 131072 bf16
-// with 20 tokens 14.8, which is latency.
+// work), 2500 of 50001 fp16 with entropy and 5 tokens 66.2 (3.8 TB/s; 46 without tokens),
+// 16 of 131072 bf16 with 20 tokens 14.9, which is latency.  Rows with fewer unmasked
+// logits than tokens wanted in a segment take the search of exact_top in each of
+// them, and waves of -infinity (or of values far from zero) a second look at their
+// values: with 10 logits of a row unmasked 174 us (16 of 131072), 2050 (2500 of 50001),
+// and without tokens 172 for 87 (2048 of 131072); with 1000 unmasked no more than usual.
 template <int DT, int VE, int G, int C, bool ENT, bool TOP>
 __global__ __launch_bounds__(kBlock, C == kStatFew ? 8 : 1) void k_vocab_stats(StatArgs a) {
     using S = typename Elem<DT>::S;
@@ -818,7 +822,7 @@ __device__ __forceinline__ Base far_base(const Logits &in, const typename Elem<D
 // gradients of its tokens in the segment are the first wave's, which stores them
 // over the others'.  One read and one write bound it: bf16 2048x65500 with entropy
 // 91.0 us (5.9 TB/s), fp32 1000x30011 from 17 tokens 45.4 (5.3), bf16 2048x131072
-// from 64 174 (6.2).
+// from 64 178 (6.0).
 template <int DT, int VE, int G, int C, bool DISTILL, bool ENT>
 __global__ __launch_bounds__(kBlock) void k_vocab_grad(GradArgs a) {
     using S = typename Elem<DT>::S;
@@ -1075,7 +1079,9 @@ int stats(StatArgs a, cxm_stream_t st) {
     }
     // 16-bit segments of 8 chunks a lane take 71 registers, 7 waves of a SIMD; of 7 chunks, where that holds them, 64
     // and 8 waves: 2500 rows of 50001 fp16 and 5 tokens 66.0 us instead of 73.2 (68.3 at 66 registers and 7 waves; held
-    // to 64 registers, 8 chunks spill: 71.8 there, but 512 rows of 131072 bf16 and 20 tokens 46.3 instead of 43.8)
+    // to 64 registers, 8 chunks spill: 71.8 there, but 512 rows of 131072 bf16 and 20 tokens 46.3 instead of 43.8).  The
+    // cut does not aim at 7: with many rows 50001 is 4 segments of 12544, but 32000, 65536 and 131072 are segments of 16000
+    // to 16384, which have 7 waves; fewer chunks and more segments there have not been timed.
     if constexpr (VE == 8 && ENT && TOP) {
         if (a.in.seglen <= kBlock * VE * kStatFew) return stats_launch<DT, VE, kBlock, ENT, TOP, kStatFew>(a, hs(st));
     }

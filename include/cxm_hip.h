@@ -474,7 +474,8 @@ int cxm_quant_rows_t(const void *x, uint8_t *q, float *scale, size_t rows, size_
  *   h = x + res, rounded to the type (res NULL: h = x),
  *   rstd = 1 / sqrt(mean((h - mean)^2) + eps), y = (h - mean) * rstd * w + bias.
  * bias may be NULL (none), and each output but one of y and q: h [rows, cols]
- * (needs res); y; q and scale; mean and rstd [rows], for the backward. */
+ * (needs res); y; q and scale; mean and rstd [rows], for the backward.  Sums are
+ * fp32: a row whose squared distances add up past it has rstd 0. */
 int cxm_layernorm_fwd_t(const void *x, const void *res, const void *w, const void *bias, float eps, void *h, void *y,
                         uint8_t *q, float *scale, float *mean, float *rstd, size_t rows, size_t cols, int dtype,
                         cxm_stream_t s);
